@@ -12,10 +12,13 @@ STATUS_WORDS = 4
 FUSED_MAX_N = 3072
 NOALLOC_SCRATCH_BYTES = 8 << 20
 GATHER_MAX_BYTES = 1 << 20
+MAX_PAGE = 4096
 
 OK, ERR_SHAPE, ERR_ALIGN, ERR_WORLD, ERR_NULL, ERR_GRID, ERR_CUDA, ERR_WORKSPACE, ERR_TIMEOUT, ERR_ARCH, \
-    ERR_SCRATCH, ERR_OVERLAP = 0, -1, -2, -3, -4, -5, -6, -7, -8, -9, -10, -11
+    ERR_SCRATCH, ERR_OVERLAP, ERR_INDEX = 0, -1, -2, -3, -4, -5, -6, -7, -8, -9, -10, -11, -12
 REDUCE, REDUCE_NORM, REDUCE_NORM_RESIDUAL = 0, 1, 2
+BF16, F16, E4M3 = 0, 1, 2
+TYPES = {torch.bfloat16: BF16, torch.float16: F16, torch.float8_e4m3fn: E4M3}
 
 LIB_PATH = Path(__file__).resolve().parent / "libdlmrt_b200.so"
 
@@ -60,6 +63,38 @@ class DlmStatus(C.Structure):
                 ("epoch", C.c_int32)]
 
 
+class DlmPages(C.Structure):
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("status", C.c_void_p), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3), ("pages", C.c_int32),
+                ("page_size", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("type", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class DlmAppend(C.Structure):
+    _fields_ = [("cache", DlmPages), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2), ("v_strides", C.c_int64 * 2),
+                ("out_strides", C.c_int64 * 2), ("positions", C.c_void_p), ("slots", C.c_void_p), ("table", C.c_void_p),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("n", C.c_int32), ("q_heads", C.c_int32),
+                ("type", C.c_int32), ("rotated", C.c_int32), ("table_rows", C.c_int32), ("interleaved", C.c_int32),
+                ("eps", C.c_float), ("pdl", C.c_int32)]
+
+
+class DlmAttend(C.Structure):
+    _fields_ = [("cache", DlmPages), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("q_strides", C.c_int64 * 3), ("out_strides", C.c_int64 * 3), ("page_table", C.c_void_p),
+                ("lengths", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+                ("table_stride", C.c_int64), ("batch", C.c_int32), ("tokens", C.c_int32), ("q_heads", C.c_int32),
+                ("type", C.c_int32), ("table_pages", C.c_int32), ("window", C.c_int32), ("causal", C.c_int32),
+                ("scale", C.c_float), ("pdl", C.c_int32), ("reserved", C.c_int32)]
+
+
+class DlmAdapters(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("base", C.c_void_p), ("out", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p),
+                ("scales", C.c_void_p), ("ids", C.c_void_p), ("status", C.c_void_p), ("ldx", C.c_int64), ("ldb", C.c_int64),
+                ("ldo", C.c_int64), ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("rank", C.c_int32),
+                ("count", C.c_int32), ("pdl", C.c_int32)]
+
+
 class DlmLoopPart(C.Structure):
     _fields_ = [("graph", C.c_void_p), ("flag", C.c_void_p)]
 
@@ -99,6 +134,11 @@ SIGNATURES = {
     "dlm_moe_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "dlm_moe_front_nvfp4": (C.c_int, [C.POINTER(DlmMoeFront), C.c_int, C.c_void_p]),
     "dlm_route_packed": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "dlm_paged_append": (C.c_int, [C.POINTER(DlmAppend), C.c_void_p]),
+    "dlm_paged_attend": (C.c_int, [C.POINTER(DlmAttend), C.c_void_p]),
+    "dlm_paged_attend_workspace_bytes": (C.c_int64, [C.POINTER(DlmAttend)]),
+    "dlm_adapters_bf16": (C.c_int, [C.POINTER(DlmAdapters), C.c_void_p]),
+    "dlm_abi_check_serving": (C.c_int, [C.c_size_t, C.c_size_t, C.c_size_t]),
     "dlm_abi_check_front": (C.c_int, [C.c_size_t]),
     "dlm_abi_check_moe": (C.c_int, [C.c_size_t]),
     "dlm_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
@@ -129,7 +169,8 @@ def lib():
             fn.restype, fn.argtypes = res, args
         if handle.dlm_abi_check(C.sizeof(DlmComm), C.sizeof(DlmGemm), C.sizeof(DlmStatus)) != OK or \
                 handle.dlm_abi_check_moe(C.sizeof(DlmMoe)) != OK or \
-                handle.dlm_abi_check_front(C.sizeof(DlmMoeFront)) != OK:
+                handle.dlm_abi_check_front(C.sizeof(DlmMoeFront)) != OK or \
+                handle.dlm_abi_check_serving(C.sizeof(DlmAppend), C.sizeof(DlmAttend), C.sizeof(DlmAdapters)) != OK:
             raise ImportError(f"{LIB_PATH}: struct layout differs from this binding; rebuild the library")
         _lib = handle
     return _lib
@@ -141,6 +182,24 @@ def stream(tensor):
     if device < 0:
         raise ValueError("expected a CUDA tensor")
     return torch._C._cuda_getCurrentRawStream(device)
+
+
+class _Here:
+    """A context that does nothing: the device in question is the current one."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_here = _Here()
+
+
+def on(device):
+    """Makes `device` the current one, as a launch on its streams needs; next to nothing where it already is."""
+    return _here if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def scratch(held, nbytes, device):

@@ -5,6 +5,7 @@
 
 #include "../../include/dlmrt_b200.h"
 #include "kernels.cuh"
+#include "serving.cuh"
 
 using namespace dlm;
 
@@ -748,6 +749,148 @@ int dlm_rowpar_bf16_loopback(const DlmGemm* gemm, const DlmComm* comm, int nrank
     return launch_rowpar_loopback(p, grid, nranks, {static_cast<cudaStream_t>(stream), false, true});
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Paged cache, attention over it, low-rank adapters
+// ---------------------------------------------------------------------------------------------------------------------
+// log2 of the page size in *shift.
+static int check_pages(const DlmPages* c, int* shift) {
+    if (c->keys == nullptr || c->values == nullptr) return DLM_ERR_NULL;
+    if (c->type < DLM_BF16 || c->type > DLM_E4M3) return DLM_ERR_SHAPE;
+    if (c->type == DLM_E4M3 && (c->k_scale == nullptr || c->v_scale == nullptr)) return DLM_ERR_NULL;
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return DLM_ERR_SHAPE;
+    if (c->heads < 1 || c->heads > 1024 || c->pages < 1) return DLM_ERR_SHAPE;
+    if (c->page_size < 1 || c->page_size > DLM_MAX_PAGE || (c->page_size & (c->page_size - 1))) return DLM_ERR_SHAPE;
+    const int per_16_bytes = c->type == DLM_E4M3 ? 16 : 8;
+    for (int i = 0; i < 3; ++i)
+        if (c->k_strides[i] < 0 || c->v_strides[i] < 0 || c->k_strides[i] % per_16_bytes || c->v_strides[i] % per_16_bytes)
+            return DLM_ERR_ALIGN;
+    if (!aligned16(c->keys) || !aligned16(c->values)) return DLM_ERR_ALIGN;
+    *shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+    return DLM_OK;
+}
+
+static bool strides_of_8(const int64_t* strides, int n) {
+    for (int i = 0; i < n; ++i)
+        if (strides[i] < 0 || strides[i] % 8) return false;
+    return true;
+}
+
+int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
+    if (a == nullptr) return DLM_ERR_NULL;
+    if (a->n == 0) return DLM_OK;  // empty tensors have no addresses
+    if (a->k == nullptr || a->v == nullptr || a->slots == nullptr) return DLM_ERR_NULL;
+    int shift = 0;
+    int rc = check_pages(&a->cache, &shift);
+    if (rc != DLM_OK) return rc;
+    if (a->q != nullptr && a->q_out == nullptr) return DLM_ERR_NULL;
+    if (a->rotated && (a->positions == nullptr || a->table == nullptr)) return DLM_ERR_NULL;
+    if (a->type != DLM_BF16 && a->type != DLM_F16) return DLM_ERR_SHAPE;
+    if (a->cache.type != DLM_E4M3 && a->cache.type != a->type) return DLM_ERR_SHAPE;
+    if (a->n < 1 || a->n > 1 << 22 || a->rotated < 0 || a->rotated > a->cache.head_dim || a->rotated % 16) return DLM_ERR_SHAPE;
+    if (a->q != nullptr && (a->q_heads < 1 || a->q_heads > 1024)) return DLM_ERR_SHAPE;
+    if (a->rotated && a->table_rows < 1) return DLM_ERR_SHAPE;
+    if (a->interleaved < 0 || a->interleaved > 1) return DLM_ERR_SHAPE;
+    if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) || !aligned16(a->table) ||
+        !aligned16(a->q_norm) || !aligned16(a->k_norm))
+        return DLM_ERR_ALIGN;
+    if (!strides_of_8(a->k_strides, 2) || !strides_of_8(a->v_strides, 2) ||
+        (a->q != nullptr && (!strides_of_8(a->q_strides, 2) || !strides_of_8(a->out_strides, 2))))
+        return DLM_ERR_ALIGN;
+    DeviceInfo info;
+    rc = device_info(&info);
+    if (rc != DLM_OK) return rc;
+    return launch_append(*a, shift, {static_cast<cudaStream_t>(stream), a->pdl != 0, false});
+}
+
+// Everything about an attention call that its device pointers do not decide: row tiles, and the chunks of the keys.
+// A chunk is one CTA's keys. Short ones fill the GPU and even out ragged lengths, long ones spare partial results and the
+// join: as many as give kCtasPerSm CTAs for each SM if every sequence had the table's length, but at least kMinChunk keys.
+static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
+    constexpr int kMinChunk = 128, kMaxChunk = 4096, kCtasPerSm = 8;
+    int rc = check_pages(&a->cache, &d->page_shift);
+    if (rc != DLM_OK) return rc;
+    if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
+    if (a->q_heads < 1 || a->q_heads > 1024 || a->q_heads % a->cache.heads) return DLM_ERR_SHAPE;
+    const long long keys = static_cast<long long>(a->table_pages) << d->page_shift;
+    if (keys > 1 << 30 || a->window < 0 || a->causal < 0 || a->causal > 1) return DLM_ERR_SHAPE;
+    if (a->type != DLM_BF16 && a->type != DLM_F16) return DLM_ERR_SHAPE;
+    if (a->cache.type != DLM_E4M3 && a->cache.type != a->type) return DLM_ERR_SHAPE;
+    d->group = a->q_heads / a->cache.heads;
+    d->rows = a->tokens * d->group;
+    d->row_tiles = (d->rows + kRowTile - 1) / kRowTile;
+    d->rows_cap = d->rows < kRowTile ? d->rows : kRowTile;
+    if (static_cast<long long>(a->cache.heads) * d->row_tiles > 65535) return DLM_ERR_SHAPE;
+    long long span = keys;  // keys from the first that a row tile sees, aligned down, to the last
+    if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kRowTile < span)
+        span = static_cast<long long>(a->window) + a->tokens + kRowTile;
+    const long long sequences = static_cast<long long>(a->batch) * a->cache.heads * d->row_tiles;
+    long long chunk = span * sequences / (static_cast<long long>(kCtasPerSm) * sms);
+    chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : (chunk + 63) / 64 * 64;
+    d->chunk = static_cast<int>(chunk);
+    d->chunks = span > 0 ? static_cast<int>((span + chunk - 1) / chunk) : 1;
+    return DLM_OK;
+}
+
+static int64_t attend_workspace(const DlmAttend* a, const AttendDev& d) {
+    if (d.chunks == 1) return 0;
+    return static_cast<int64_t>(a->batch) * a->cache.heads * d.row_tiles * d.chunks * d.rows_cap * (a->cache.head_dim + 2) * 4;
+}
+
+int64_t dlm_paged_attend_workspace_bytes(const DlmAttend* a) {
+    if (a == nullptr) return 0;
+    DeviceInfo info;
+    AttendDev d;
+    const int sms = device_info(&info) == DLM_OK ? info.sms : 148;
+    return plan_attend(a, sms, &d) == DLM_OK ? attend_workspace(a, d) : 0;
+}
+
+int dlm_paged_attend(const DlmAttend* a, dlm_stream_t stream) {
+    if (a == nullptr) return DLM_ERR_NULL;
+    if (a->batch == 0) return DLM_OK;  // empty tensors have no addresses
+    if (a->q == nullptr || a->out == nullptr || a->lengths == nullptr) return DLM_ERR_NULL;
+    if (a->page_table == nullptr && a->table_pages > 0) return DLM_ERR_NULL;
+    AttendDev d;
+    std::memset(&d, 0, sizeof(d));
+    int rc = plan_attend(a, 148, &d);  // the arguments; the plan itself once the device is known
+    if (rc != DLM_OK) return rc;
+    if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->workspace)) return DLM_ERR_ALIGN;
+    if (!strides_of_8(a->q_strides, 3) || !strides_of_8(a->out_strides, 3) || a->table_stride < 0) return DLM_ERR_ALIGN;
+    DeviceInfo info;
+    rc = device_info(&info);
+    if (rc == DLM_OK) rc = plan_attend(a, info.sms, &d);
+    if (rc != DLM_OK) return rc;
+    const int64_t need = attend_workspace(a, d);
+    if (need > 0 && a->workspace == nullptr) return DLM_ERR_NULL;
+    if (a->workspace_bytes < need) return DLM_ERR_WORKSPACE;
+    d.a = *a;
+    d.partial = static_cast<float*>(a->workspace);
+    if (need > 0) d.stats = d.partial + need / 4 / (a->cache.head_dim + 2) * a->cache.head_dim;
+    return launch_attend(d, {static_cast<cudaStream_t>(stream), a->pdl != 0, false});
+}
+
+int dlm_adapters_bf16(const DlmAdapters* a, dlm_stream_t stream) {
+    if (a == nullptr) return DLM_ERR_NULL;
+    if (a->m == 0) return DLM_OK;  // empty tensors have no addresses
+    if (a->x == nullptr || a->base == nullptr || a->out == nullptr || a->a == nullptr || a->b == nullptr ||
+        a->scales == nullptr || a->ids == nullptr)
+        return DLM_ERR_NULL;
+    if (a->m < 1 || a->m > DLM_MAX_M || a->n < 8 || a->n % 8 || a->k < 8 || a->k % 8) return DLM_ERR_SHAPE;
+    if (a->rank < 8 || a->rank % 8 || a->rank > 128 || a->count < 1) return DLM_ERR_SHAPE;
+    if (!aligned16(a->x) || !aligned16(a->base) || !aligned16(a->out) || !aligned16(a->a) || !aligned16(a->b))
+        return DLM_ERR_ALIGN;
+    if (a->ldx % 8 || a->ldb % 8 || a->ldo % 8 || a->ldx < 0 || a->ldb < 0 || a->ldo < a->n) return DLM_ERR_ALIGN;
+    DeviceInfo info;
+    const int rc = device_info(&info);
+    if (rc != DLM_OK) return rc;
+    return launch_adapters(*a, {static_cast<cudaStream_t>(stream), a->pdl != 0, false});
+}
+
+int dlm_abi_check_serving(size_t sizeof_append, size_t sizeof_attend, size_t sizeof_adapters) {
+    return sizeof_append == sizeof(DlmAppend) && sizeof_attend == sizeof(DlmAttend) && sizeof_adapters == sizeof(DlmAdapters)
+               ? DLM_OK
+               : DLM_ERR_SHAPE;
+}
+
 // Room for kMaxSplits partial tiles whatever K, or for as many as a plain GEMM of this shape splits its K into.
 size_t dlm_workspace_bytes(int m, int n, int k) {
     if (m <= 0 || n <= 0) return 0;
@@ -810,6 +953,7 @@ const char* dlm_strerror(int code) {
         case DLM_ERR_ARCH: return "not an sm_100 device";
         case DLM_ERR_OVERLAP: return "the fused GEMM's input overlaps a buffer the same launch re-arms or writes (rearm, out)";
         case DLM_ERR_SCRATCH: return "requested K splits need more than the library's built-in scratch (DLM_NOALLOC_SCRATCH_BYTES)";
+        case DLM_ERR_INDEX: return "a slot, position, page, length or adapter index lies outside its table";
         default: return "unknown error";
     }
 }

@@ -244,6 +244,10 @@ class Group:
             self._run_alone(pending)
         return partial
 
+    def discard(self, partial):
+        """Forget a producer recorded for `partial`, whose contents the caller is about to write."""
+        self._pending.pop(partial.data_ptr(), None)
+
     def workspace(self, chain, nbytes):
         """Split-K scratch of the fused GEMMs of one chain (FP32 partial tiles + tile counters), grown on demand."""
         held = self._workspaces.get(chain)

@@ -37,7 +37,8 @@ def tile_weight(weight):
 class Linear:
     """y = x @ W^T, BF16 in and out, FP32 accumulation in increasing K (K ranges summed in order when split)."""
 
-    def __init__(self, weight, fp8=False, b200=False, group=None, tiled=True, nn=False, token_tiles=0, splits=0):
+    def __init__(self, weight, fp8=False, b200=False, group=None, tiled=True, nn=False, token_tiles=0, splits=0,
+                 adapters=None):
         if fp8:
             raise NotImplementedError("FP8 linears are not part of the row-parallel BF16 path")
         if weight.dtype != torch.bfloat16 or weight.dim() != 2:
@@ -53,6 +54,10 @@ class Linear:
         # `tiled`: stream a re-laid copy of the weight (see tile_weight) instead of the row-major matrix.
         self.tiles = tile_weight(self.weight) if tiled and self.n % 128 == 0 and self.k % 8 == 0 else None
         self.group = group
+        # Low-rank adapters of this projection (dlmrt_b200.layers.adapters.Adapters), for calls that say which row has which.
+        if adapters is not None and (adapters.n, adapters.k) != (self.n, self.k):
+            raise ValueError(f"adapters are [{adapters.n}, {adapters.k}], the weight is [{self.n}, {self.k}]")
+        self.adapters = adapters
         # Tiling of this layer's GEMM (tiles along the tokens, K splits): 0 = chosen by the library for each call.
         self.token_tiles, self.splits = token_tiles, splits
         self._workspace, self._workspaces = None, []  # split-K scratch: the newest, and all (see _lib.scratch)
@@ -103,7 +108,18 @@ class Linear:
         else:
             g.w, g.ldw, g.w_tiled = self.weight.data_ptr(), self.weight.stride(0), 0
 
-    def __call__(self, x, scales=None, out=None):
+    def __call__(self, x, scales=None, out=None, ids=None):
+        """x @ W^T; with `ids` [rows] int32 plus each row's own adapter (see Adapters). A row-parallel layer's adapters are
+        split like it: A along K, B whole, so that the sum over ranks is right for them, too. A call with ids into a group's
+        partial runs at once and is not fused into the reduction."""
+        if ids is not None:
+            if self.adapters is None:
+                raise ValueError("ids were given to a layer without adapters")
+            if out is None:
+                out = torch.empty(x.shape[0], self.n, device=x.device, dtype=torch.bfloat16)
+            elif self.group is not None and self.group.is_partial(out):
+                self.group.discard(out)
+            return self.adapters(x, ids, self.gemm(x, out), out=out)
         if out is None:
             out = torch.empty(x.shape[0], self.n, device=x.device, dtype=torch.bfloat16)
         elif self.group is not None and self.group.is_partial(out):

@@ -59,7 +59,8 @@ enum {
     DLM_ERR_TIMEOUT = -8,   /* device status: a bounded wait ran out (data from a rank never arrived) */
     DLM_ERR_ARCH = -9,      /* not an sm_100 device */
     DLM_ERR_SCRATCH = -10,  /* dlm_gemm_bf16_noalloc: the requested K splits do not fit the built-in scratch */
-    DLM_ERR_OVERLAP = -11   /* dlm_rowpar_bf16: the GEMM's input overlaps `rearm` or `out` of the same call */
+    DLM_ERR_OVERLAP = -11,  /* dlm_rowpar_bf16: the GEMM's input overlaps `rearm` or `out` of the same call */
+    DLM_ERR_INDEX = -12     /* device status: a slot, position, page, length or adapter index lies outside its table */
 };
 
 /* What follows the rank-ordered sum (tp_comm.cu:138 template <NORM, RESIDUAL>). */
@@ -300,6 +301,110 @@ DLM_API int dlm_all_gather(const void* x, int64_t bytes, const DlmComm* comm, dl
 /* All ranks in one cooperative launch on one GPU (tests), as the other *_loopback entry points. */
 DLM_API int dlm_all_gather_loopback(const void* const* x, int64_t bytes, const DlmComm* comm, int nranks,
                                     dlm_stream_t stream);
+
+/* ---- paged cache of keys and values: append with rotation, attention over it ------------------------------------
+ * What runs between the qkv projection and the o_proj of a round. Replaces the reference's QK-norm + RoPE + KV write
+ * (dlmrt/ops/triton/core.py, called at dlmrt/models/sdar/model.py:211-243) and its attention over the KV arena with a
+ * split over the keys and a combine pass (dlmrt/models/sdar/engine.py:127-132, dlmrt/ops/triton/attention.py).
+ *
+ * Indices that live on the device are checked there: an entry outside its table touches no memory, is treated as if it
+ * were not there, and leaves DLM_ERR_INDEX in the status words (block = which row or sequence, slot = which index). */
+enum { DLM_BF16 = 0, DLM_F16 = 1, DLM_E4M3 = 2 };
+
+#define DLM_MAX_PAGE 4096
+
+/* One layer's pool of pages. Element strides; the head dimension is contiguous. */
+typedef struct DlmPages {
+    void* keys;                /* element (page, head, slot, i) at page * k_strides[0] + head * k_strides[1] + slot * */
+    void* values;              /*                               k_strides[2] + i; values likewise                     */
+    const float* k_scale;      /* [heads] what a key code counts for (DLM_E4M3: required; otherwise NULL) */
+    const float* v_scale;      /* [heads] the same for values */
+    int32_t* status;           /* [DLM_STATUS_WORDS] as DlmComm.status, or NULL */
+    int64_t k_strides[3];      /* page, head, slot; multiples of 16 bytes */
+    int64_t v_strides[3];
+    int32_t pages, page_size;  /* page_size a power of two, at most DLM_MAX_PAGE */
+    int32_t heads, head_dim;   /* head_dim 64, 128 or 256 */
+    int32_t type;              /* DLM_BF16, DLM_F16 or DLM_E4M3 */
+    int32_t reserved;
+} DlmPages;
+
+/* New tokens enter the cache: k' = rotate(norm(k)) and v are stored in their slots, q' = rotate(norm(q)) in q_out.
+ *   norm    x * rsqrt(mean(x^2) + eps) * weight over a head, FP32, left out where the weight is NULL;
+ *   rotate  (a, b) -> (a cos - b sin, b cos + a sin) on the first `rotated` elements of a head, a and b being elements i
+ *           and i + rotated / 2 (interleaved 0) or 2i and 2i + 1 (interleaved 1), FP32; no rounding in between.
+ * Stored in FP8: x / scale[head], at most the largest code in magnitude.
+ * A negative slot marks a padded row: nothing is stored for it, its q_out is written. A row whose position or slot lies
+ * outside its table is left out altogether. The slots of one call must be distinct. q_out may be q. */
+typedef struct DlmAppend {
+    DlmPages cache;
+    const void* q;             /* [n, q_heads, head_dim] `type`, or NULL (then q_out is ignored) */
+    const void* k;             /* [n, heads, head_dim] */
+    const void* v;
+    void* q_out;
+    int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];  /* token, head: elements, multiples of 8 */
+    const int32_t* positions;  /* [n]; NULL where rotated is 0 */
+    const int64_t* slots;      /* [n] page * page_size + slot of the page */
+    const float* table;        /* [table_rows, rotated]: cosines of the rotated / 2 angles, then sines */
+    const void* q_norm;        /* [head_dim] `type`, or NULL */
+    const void* k_norm;
+    int32_t n, q_heads, type;  /* type of q, k, v, q_out and the norms: DLM_BF16 or DLM_F16 */
+    int32_t rotated;           /* a multiple of 16, at most head_dim; 0: no rotation */
+    int32_t table_rows, interleaved;
+    float eps;
+    int32_t pdl;
+} DlmAppend;
+
+DLM_API int dlm_paged_append(const DlmAppend* append, dlm_stream_t stream);
+
+/* out = softmax(scale q K^T + mask) V for `tokens` new tokens of each of `batch` sequences, over the first lengths[b] keys
+ * of the pages that page_table[b] lists. The new tokens are the last ones of their sequence (appended already): token i
+ * stands at lengths[b] - tokens + i. causal 0: every token sees all lengths[b] keys (a block that is refined as a whole);
+ * causal 1: the keys up to its own. window w > 0: only keys less than w positions before it. A token that sees no key
+ * (length 0, or causal and in front of the first key) gets zeros, and -inf in lse. A sequence longer than its row of the
+ * table is read as far as the table goes. Grouped heads: query head i reads key head i / (q_heads / heads).
+ * Keys past the end, pages that are not there and places that the mask hides never reach the result, whatever they hold.
+ * Products of `type` with FP32 accumulation, softmax in FP32; FP8 entries are widened exactly. */
+typedef struct DlmAttend {
+    DlmPages cache;
+    const void* q;             /* [batch, tokens, q_heads, head_dim] `type` */
+    void* out;
+    float* lse;                /* [batch, tokens, q_heads] natural logarithm of the softmax's denominator, or NULL */
+    int64_t q_strides[3], out_strides[3];  /* sequence, token, head: elements, multiples of 8 */
+    const int32_t* page_table; /* [batch, table_pages], rows table_stride apart */
+    const int32_t* lengths;    /* [batch] keys of each sequence, the new ones included */
+    void* workspace;           /* dlm_paged_attend_workspace_bytes() bytes, 16-byte aligned; nothing is kept in it */
+    int64_t workspace_bytes;
+    int64_t table_stride;
+    int32_t batch, tokens, q_heads, type;
+    int32_t table_pages, window, causal;
+    float scale;
+    int32_t pdl, reserved;
+} DlmAttend;
+
+DLM_API int dlm_paged_attend(const DlmAttend* attend, dlm_stream_t stream);
+/* Workspace that this call needs (device pointers are not looked at): 0 when no sequence of the table's size is split. */
+DLM_API int64_t dlm_paged_attend_workspace_bytes(const DlmAttend* attend);
+
+/* ---- low-rank adapters of many requests beside a shared projection ----------------------------------------------
+ * out[i] = base[i] + scales[ids[i]] * (x[i] * A[ids[i]]^T) * B[ids[i]]^T; rows with a negative id: out[i] = base[i].
+ * No counterpart in the reference. x W^T comes from dlm_gemm_bf16; out may be base. FP32 accumulation, one rounding. */
+typedef struct DlmAdapters {
+    const void* x;             /* [m, k] BF16, rows ldx apart */
+    const void* base;          /* [m, n] BF16, rows ldb apart */
+    void* out;                 /* [m, n] BF16, rows ldo apart */
+    const void* a;             /* [count, rank, k] BF16 contiguous */
+    const void* b;             /* [count, n, rank] BF16 contiguous */
+    const float* scales;       /* [count] */
+    const int32_t* ids;        /* [m] adapter of each row, any order; negative: none */
+    int32_t* status;           /* [DLM_STATUS_WORDS] or NULL; an id past `count` is DLM_ERR_INDEX and counts as none */
+    int64_t ldx, ldb, ldo;     /* multiples of 8 */
+    int32_t m, n, k, rank;     /* 1 <= m <= 256; n, k, rank multiples of 8; rank <= 128 */
+    int32_t count, pdl;
+} DlmAdapters;
+
+DLM_API int dlm_adapters_bf16(const DlmAdapters* adapters, dlm_stream_t stream);
+
+DLM_API int dlm_abi_check_serving(size_t sizeof_append, size_t sizeof_attend, size_t sizeof_adapters);
 
 /* Bytes of workspace (FP32 split-K partial tiles + tile counters) a GEMM of this shape needs: for 8 splits, or for as
  * many as dlm_gemm_bf16 splits the K of this shape into. */
