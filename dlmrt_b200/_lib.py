@@ -72,25 +72,25 @@ class DlmPages(C.Structure):
 
 class DlmAppend(C.Structure):
     _fields_ = [("cache", DlmPages), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
-                ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2), ("v_strides", C.c_int64 * 2),
-                ("out_strides", C.c_int64 * 2), ("positions", C.c_void_p), ("slots", C.c_void_p), ("table", C.c_void_p),
-                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("n", C.c_int32), ("q_heads", C.c_int32),
+                ("positions", C.c_void_p), ("slots", C.c_void_p), ("table", C.c_void_p), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2),
+                ("v_strides", C.c_int64 * 2), ("out_strides", C.c_int64 * 2), ("n", C.c_int32), ("q_heads", C.c_int32),
                 ("type", C.c_int32), ("rotated", C.c_int32), ("table_rows", C.c_int32), ("interleaved", C.c_int32),
                 ("eps", C.c_float), ("pdl", C.c_int32)]
 
 
 class DlmAttend(C.Structure):
-    _fields_ = [("cache", DlmPages), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
-                ("q_strides", C.c_int64 * 3), ("out_strides", C.c_int64 * 3), ("page_table", C.c_void_p),
+    _fields_ = [("cache", DlmPages), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("page_table", C.c_void_p),
                 ("lengths", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
-                ("table_stride", C.c_int64), ("batch", C.c_int32), ("tokens", C.c_int32), ("q_heads", C.c_int32),
-                ("type", C.c_int32), ("table_pages", C.c_int32), ("window", C.c_int32), ("causal", C.c_int32),
-                ("scale", C.c_float), ("pdl", C.c_int32), ("reserved", C.c_int32)]
+                ("q_strides", C.c_int64 * 3), ("out_strides", C.c_int64 * 3), ("table_stride", C.c_int64),
+                ("batch", C.c_int32), ("tokens", C.c_int32), ("q_heads", C.c_int32), ("type", C.c_int32),
+                ("table_pages", C.c_int32), ("window", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float),
+                ("pdl", C.c_int32), ("reserved", C.c_int32)]
 
 
 class DlmAdapters(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("base", C.c_void_p), ("out", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p),
-                ("scales", C.c_void_p), ("ids", C.c_void_p), ("status", C.c_void_p), ("ldx", C.c_int64), ("ldb", C.c_int64),
+    _fields_ = [("x", C.c_void_p), ("base", C.c_void_p), ("out", C.c_void_p), ("ids", C.c_void_p), ("a", C.c_void_p),
+                ("b", C.c_void_p), ("scales", C.c_void_p), ("status", C.c_void_p), ("ldx", C.c_int64), ("ldb", C.c_int64),
                 ("ldo", C.c_int64), ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("rank", C.c_int32),
                 ("count", C.c_int32), ("pdl", C.c_int32)]
 
@@ -184,22 +184,14 @@ def stream(tensor):
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-class _Here:
-    """A context that does nothing: the device in question is the current one."""
-
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *_):
-        pass
-
-
-_here = _Here()
-
-
-def on(device):
-    """Makes `device` the current one, as a launch on its streams needs; next to nothing where it already is."""
-    return _here if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+def launch(name, descriptor, device):
+    """Calls the entry point `name` with `descriptor` on the current stream of `device`, which is made the current device for
+    the call where it is not. Returns the code."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return getattr(_lib, name)(descriptor, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return getattr(_lib, name)(descriptor, torch._C._cuda_getCurrentRawStream(index))
 
 
 def scratch(held, nbytes, device):

@@ -802,11 +802,9 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
     return launch_append(*a, shift, {static_cast<cudaStream_t>(stream), a->pdl != 0, false});
 }
 
-// Everything about an attention call that its device pointers do not decide: row tiles, and the chunks of the keys.
-// A chunk is one CTA's keys. Short ones fill the GPU and even out ragged lengths, long ones spare partial results and the
-// join: as many as give kCtasPerSm CTAs for each SM if every sequence had the table's length, but at least kMinChunk keys.
+// Everything about an attention call that its device pointers do not decide.
 static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
-    constexpr int kMinChunk = 128, kMaxChunk = 4096, kCtasPerSm = 8;
+    constexpr int kWholeKeys = 512, kLeastUnits = 2;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
@@ -819,21 +817,26 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->rows = a->tokens * d->group;
     d->row_tiles = (d->rows + kRowTile - 1) / kRowTile;
     d->rows_cap = d->rows < kRowTile ? d->rows : kRowTile;
-    if (static_cast<long long>(a->cache.heads) * d->row_tiles > 65535) return DLM_ERR_SHAPE;
-    long long span = keys;  // keys from the first that a row tile sees, aligned down, to the last
-    if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kRowTile < span)
-        span = static_cast<long long>(a->window) + a->tokens + kRowTile;
-    const long long sequences = static_cast<long long>(a->batch) * a->cache.heads * d->row_tiles;
-    long long chunk = span * sequences / (static_cast<long long>(kCtasPerSm) * sms);
-    chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : (chunk + 63) / 64 * 64;
-    d->chunk = static_cast<int>(chunk);
-    d->chunks = span > 0 ? static_cast<int>((span + chunk - 1) / chunk) : 1;
+    if (static_cast<long long>(a->cache.heads) * d->row_tiles > 1 << 20) return DLM_ERR_SHAPE;
+    d->items = a->cache.heads * d->row_tiles;
+    long long span = keys;  // from the first key that some token sees, aligned down, to the last
+    if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kUnitKeys < span)
+        span = static_cast<long long>(a->window) + a->tokens + kUnitKeys;
+    d->ctas = sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
+    d->least_units = kLeastUnits;
+    d->unit = kUnitKeys;
+    if (span <= kWholeKeys) {
+        d->unit = static_cast<int>(span < kUnitKeys ? kUnitKeys : (span + kUnitKeys - 1) / kUnitKeys * kUnitKeys);
+        d->least_units = 1;
+        const long long items = static_cast<long long>(a->batch) * d->items;
+        if (items < d->ctas) d->ctas = static_cast<int>(items);
+    }
     return DLM_OK;
 }
 
 static int64_t attend_workspace(const DlmAttend* a, const AttendDev& d) {
-    if (d.chunks == 1) return 0;
-    return static_cast<int64_t>(a->batch) * a->cache.heads * d.row_tiles * d.chunks * d.rows_cap * (a->cache.head_dim + 2) * 4;
+    if (d.unit != kUnitKeys) return 0;
+    return static_cast<int64_t>(d.ctas) * 2 * d.rows_cap * (a->cache.head_dim + 2) * 4;
 }
 
 int64_t dlm_paged_attend_workspace_bytes(const DlmAttend* a) {
@@ -863,8 +866,10 @@ int dlm_paged_attend(const DlmAttend* a, dlm_stream_t stream) {
     if (need > 0 && a->workspace == nullptr) return DLM_ERR_NULL;
     if (a->workspace_bytes < need) return DLM_ERR_WORKSPACE;
     d.a = *a;
-    d.partial = static_cast<float*>(a->workspace);
-    if (need > 0) d.stats = d.partial + need / 4 / (a->cache.head_dim + 2) * a->cache.head_dim;
+    if (need > 0) {
+        d.partial = static_cast<float*>(a->workspace);
+        d.stats = d.partial + need / 4 / (a->cache.head_dim + 2) * a->cache.head_dim;
+    }
     return launch_attend(d, {static_cast<cudaStream_t>(stream), a->pdl != 0, false});
 }
 

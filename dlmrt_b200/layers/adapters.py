@@ -6,11 +6,17 @@
 a batch holds. `Linear(weight, adapters=...)` does both in one call (see there). The reference has no adapters.
 """
 
+from struct import Struct
+
 import torch
 
 from .. import _lib
 from .._lib import DlmAdapters
 from ..ops.paged_kv import _index_error
+
+# The pointers that every call brings, which lie side by side in the descriptor.
+_CALL, _CALL_AT = Struct("4Q"), DlmAdapters.x.offset
+_MOST_PLANS = 4096
 
 
 class Adapters:
@@ -35,6 +41,7 @@ class Adapters:
         d = self._call = DlmAdapters()  # what every call starts from
         d.a, d.b, d.scales, d.status = a.data_ptr(), b.data_ptr(), scales.data_ptr(), self.status.data_ptr()
         d.n, d.k, d.rank, d.count, d.pdl = self.n, self.k, self.rank, self.count, 1
+        self._plans = {}  # everything of a call's arguments but addresses -> its checked descriptor without these
         _lib.lib()
 
     def check(self):
@@ -45,23 +52,35 @@ class Adapters:
         """out = base + each row's own adapter applied to x. `x` [rows, K], `base` and `out` [rows, N] BF16 with contiguous
         rows (`out` may be `base`; by default a new tensor), at most 256 rows; `ids` [rows] int32 in any order, negative for
         a row without adapter."""
+        key = (x.shape, x.stride(), x.dtype, x.device, ids.shape, ids.stride(), ids.dtype, ids.device, base.shape, base.stride(),
+               base.dtype, base.device, None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plan(x, ids, base, out)
+            if len(self._plans) >= _MOST_PLANS:
+                self._plans.clear()
+            self._plans[key] = plan
+        if out is None:
+            out = torch.empty_like(base, memory_format=torch.contiguous_format)
+        d = DlmAdapters.from_buffer_copy(plan)
+        _CALL.pack_into(d, _CALL_AT, x.data_ptr(), base.data_ptr(), out.data_ptr(), ids.data_ptr())
+        code = _lib.launch("dlm_adapters_bf16", d, self.device)
+        if code:
+            _lib.check(code, f"adapters [{x.shape[0]}, {self.n}, {self.k}] of rank {self.rank}")
+        return out
+
+    def _plan(self, x, ids, base, out):
+        """The checked descriptor of a call, without the addresses that it brings."""
         if x.dim() != 2 or x.shape[1] != self.k or base.shape != (x.shape[0], self.n):
             raise ValueError(f"Adapters [{self.n}, {self.k}]: x {tuple(x.shape)}, base {tuple(base.shape)}")
-        if out is None:
-            out = torch.empty(base.shape, device=base.device, dtype=base.dtype)
-        elif out.shape != base.shape:
+        if out is not None and out.shape != base.shape:
             raise ValueError(f"out {tuple(out.shape)}: expected {tuple(base.shape)}")
         m = x.shape[0]
-        for t in (x, base, out):
+        for t in (x, base) if out is None else (x, base, out):
             if t.dtype != torch.bfloat16 or t.stride(1) != 1 or t.device != self.device:
                 raise ValueError(f"x, base and out must be BF16 with contiguous rows on {self.device}")
         if ids.dtype != torch.int32 or ids.shape != (m,) or not ids.is_contiguous() or ids.device != self.device:
             raise ValueError(f"ids must be a contiguous int32 [{m}] tensor on {self.device}")
         d = DlmAdapters.from_buffer_copy(self._call)
-        d.x, d.base, d.out, d.ids, d.m = x.data_ptr(), base.data_ptr(), out.data_ptr(), ids.data_ptr(), m
-        d.ldx, d.ldb, d.ldo = x.stride(0), base.stride(0), out.stride(0)
-        with _lib.on(self.device):
-            code = _lib.lib().dlm_adapters_bf16(d, _lib.stream(x))
-        if code:
-            _lib.check(code, f"adapters [{m}, {self.n}, {self.k}] of rank {self.rank}")
-        return out
+        d.m, d.ldx, d.ldb, d.ldo = m, x.stride(0), base.stride(0), self.n if out is None else out.stride(0)
+        return d

@@ -18,11 +18,17 @@ outside its table touches no memory, and `PagedKV.check()` raises IndexError for
 """
 
 import ctypes as C
+from struct import Struct
 
 import torch
 
 from .. import _lib
 from .._lib import DlmAppend, DlmAttend, DlmPages, DlmStatus
+
+# The pointers that every call brings, which lie side by side in the descriptors.
+_APPEND, _APPEND_AT = Struct("9Q"), DlmAppend.q.offset
+_ATTEND, _ATTEND_AT = Struct("7Q"), DlmAttend.q.offset
+_MOST_PLANS = 4096  # of one cache: sizes of calls that are remembered
 
 _INDEX = {1: "slot", 2: "position", 3: "page", 4: "length", 5: "adapter"}
 
@@ -87,7 +93,9 @@ class PagedKV:
         self._append, self._attend = DlmAppend(), DlmAttend()  # what every call starts from
         self._append.cache = self._attend.cache = p
         self._append.pdl = self._attend.pdl = 1
-        self._room = {}  # (sizes of an attention call) -> bytes of its scratch
+        # Everything of a call's arguments but addresses -> its descriptor, checked and filled in but for these. Calls copy
+        # it, so concurrent callers share nothing. Checking and filling anew took 10 of a small call's 16 us.
+        self._plans = {}
         _lib.lib()
 
     def check(self):
@@ -115,6 +123,37 @@ class PagedKV:
         `table` (see `rotary_table`, whose width says how many elements of a head are rotated; None: no rotation).
         `interleaved`: pairs are neighbours, not a half apart. `q_norm`, `k_norm` [head dim]: weights of an RMSNorm over each
         head in front of the rotation. `q_out` may be `q`; by default a new contiguous tensor."""
+        key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, slots.shape, slots.stride(),
+               slots.dtype, slots.device, eps, interleaved,
+               None if table is None else (table.shape, table.stride(), table.dtype, table.device, positions.shape,
+                                           positions.stride(), positions.dtype, positions.device),
+               None if q is None else (q.shape, q.stride(), q.dtype, q.device),
+               None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.device),
+               None if q_norm is None else (q_norm.shape, q_norm.stride(), q_norm.dtype, q_norm.device),
+               None if k_norm is None else (k_norm.shape, k_norm.stride(), k_norm.dtype, k_norm.device))
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plan_append(k, v, positions, slots, table, q, q_out, q_norm, k_norm, eps, interleaved)
+            self._remember(key, plan)
+        if q is not None and q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        a = DlmAppend.from_buffer_copy(plan)
+        _APPEND.pack_into(a, _APPEND_AT, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                          0 if q is None else q_out.data_ptr(), 0 if table is None else positions.data_ptr(), slots.data_ptr(),
+                          0 if table is None else table.data_ptr(), 0 if q_norm is None else q_norm.data_ptr(),
+                          0 if k_norm is None else k_norm.data_ptr())
+        code = _lib.launch("dlm_paged_append", a, self.device)
+        if code:
+            _lib.check(code, f"PagedKV.append of {k.shape[0]} tokens")
+        return q_out
+
+    def _remember(self, key, plan):
+        if len(self._plans) >= _MOST_PLANS:
+            self._plans.clear()
+        self._plans[key] = plan
+
+    def _plan_append(self, k, v, positions, slots, table, q, q_out, q_norm, k_norm, eps, interleaved):
+        """The checked descriptor of an append, without addresses."""
         n = k.shape[0]
         shape = (n, self.heads, self.head_dim)
         a = DlmAppend.from_buffer_copy(self._append)
@@ -126,42 +165,37 @@ class PagedKV:
         vt, vh, v1 = v.stride()
         if k1 != 1 or v1 != 1 or not slots.is_contiguous():
             raise ValueError("k and v must have a contiguous head dimension, slots must be contiguous")
-        a.k, a.v, a.slots, a.n, a.eps = k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, eps
-        a.k_strides[0], a.k_strides[1], a.v_strides[0], a.v_strides[1] = kt, kh, vt, vh
+        a.n, a.eps = n, eps
+        a.k_strides[:], a.v_strides[:] = (kt, kh), (vt, vh)
         if table is not None:
             self._given("table", table, torch.float32, table.shape)
             self._given("positions", positions, torch.int32, (n,))
             if table.dim() != 2 or not table.is_contiguous() or not positions.is_contiguous():
                 raise ValueError("table must be contiguous [positions, rotated], positions contiguous")
-            a.table, a.table_rows, a.rotated = table.data_ptr(), table.shape[0], table.shape[1]
-            a.positions, a.interleaved = positions.data_ptr(), interleaved
+            if not table.shape[0] or not 16 <= table.shape[1] <= self.head_dim or table.shape[1] % 16:
+                raise ValueError(f"table {tuple(table.shape)}: its width is a multiple of 16 up to {self.head_dim}")
+            a.table_rows, a.rotated = table.shape
+            a.interleaved = bool(interleaved)
         for name, norm in (("q_norm", q_norm), ("k_norm", k_norm)):
             if norm is not None:
                 self._given(name, norm, k.dtype, (self.head_dim,))
                 if not norm.is_contiguous():
                     raise ValueError(f"{name} must be contiguous")
-                setattr(a, name, norm.data_ptr())
         if q is not None:
             if q.dim() != 3:
                 raise ValueError(f"q must be [n, query heads, head dim], got {tuple(q.shape)}")
             self._given("q", q, k.dtype, (n, q.shape[1], self.head_dim))
-            if q_out is None:
-                q_out = torch.empty(q.shape, device=self.device, dtype=q.dtype)
-            else:
+            if q_out is not None:
                 self._given("q_out", q_out, q.dtype, q.shape)
             qt, qh, q1 = q.stride()
-            ot, oh, o1 = q_out.stride()
+            ot, oh, o1 = (q.shape[1] * q.shape[2], q.shape[2], 1) if q_out is None else q_out.stride()
             if q1 != 1 or o1 != 1:
                 raise ValueError("q and q_out must have a contiguous head dimension")
-            a.q, a.q_out, a.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-            a.q_strides[0], a.q_strides[1], a.out_strides[0], a.out_strides[1] = qt, qh, ot, oh
+            a.q_heads = q.shape[1]
+            a.q_strides[:], a.out_strides[:] = (qt, qh), (ot, oh)
         elif q_out is not None or q_norm is not None:
             raise ValueError("q_out and q_norm come with q")
-        with _lib.on(self.device):
-            code = _lib.lib().dlm_paged_append(a, _lib.stream(k))
-        if code:
-            _lib.check(code, f"PagedKV.append of {n} tokens")
-        return q_out
+        return a
 
     def attend(self, q, pages, lengths, out=None, lse=None, scale=None, window=0, causal=False):
         """Attention of the last `tokens` tokens of each sequence over its cached keys; returns `out`, shaped like `q`.
@@ -173,10 +207,31 @@ class PagedKV:
         positions before it. A token that sees none gets zeros. `scale`: of the scores, head dim ** -0.5 by default. `out`
         may be `q`. `lse` [batch, tokens, query heads] FP32, if given, takes the logarithm of the softmax's denominator
         (-inf for a token that sees no key): what is needed to join the result with attention over other keys."""
-        if q.dim() == 3:
-            q4, single = q.unsqueeze(1), True
-        else:
-            q4, single = q, False
+        key = (q.shape, q.stride(), q.dtype, q.device, pages.shape, pages.stride(), pages.dtype, pages.device, lengths.shape,
+               lengths.stride(), lengths.dtype, lengths.device, scale, window, causal,
+               None if out is None else (out.shape, out.stride(), out.dtype, out.device),
+               None if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.device))
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plan_attend(q, pages, lengths, out, lse, scale, window, causal)
+            self._remember(key, plan)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        a = DlmAttend.from_buffer_copy(plan)
+        room = plan.workspace_bytes
+        # Scratch is of this call alone: calls on other streams, and captured graphs, have their own.
+        scratch = torch.empty(room, device=self.device, dtype=torch.uint8) if room else None
+        _ATTEND.pack_into(a, _ATTEND_AT, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), pages.data_ptr(),
+                          lengths.data_ptr(), scratch.data_ptr() if room else 0, room)
+        code = _lib.launch("dlm_paged_attend", a, self.device)
+        if code:
+            _lib.check(code, f"PagedKV.attend of {tuple(q.shape)} over {tuple(pages.shape)} pages")
+        return out
+
+    def _plan_attend(self, q, pages, lengths, out, lse, scale, window, causal):
+        """The checked descriptor of an attention call, without addresses; its workspace_bytes are what the call needs."""
+        single = q.dim() == 3
+        q4 = q.unsqueeze(1) if single else q
         if q4.dim() != 4 or q4.shape[3] != self.head_dim:
             raise ValueError(f"q must be [batch, tokens, query heads, {self.head_dim}], got {tuple(q.shape)}")
         b, t, hq, d = q4.shape
@@ -190,35 +245,22 @@ class PagedKV:
             raise ValueError(f"pages must be [{b}, most pages], got {tuple(pages.shape)}")
         self._given("pages", pages, torch.int32, pages.shape)
         self._given("lengths", lengths, torch.int32, (b,))
-        if out is None:
-            out = torch.empty(q.shape, device=self.device, dtype=q.dtype)
-        else:
+        if out is not None:
             self._given("out", out, q.dtype, q.shape)
-        out4 = out.unsqueeze(1) if single else out
-        (qb, qt, qh, q1), (ob, ot, oh, o1), (pb, p1) = q4.stride(), out4.stride(), pages.stride()
+            out4 = out.unsqueeze(1) if single else out
+        (qb, qt, qh, q1), (pb, p1) = q4.stride(), pages.stride()
+        ob, ot, oh, o1 = (t * hq * d, hq * d, d, 1) if out is None else out4.stride()
         if q1 != 1 or o1 != 1 or (p1 != 1 and pages.shape[1] > 1) or not lengths.is_contiguous():
             raise ValueError("q and out must have a contiguous head dimension, pages contiguous rows; lengths are contiguous")
         if lse is not None:
             self._given("lse", lse, torch.float32, (b, hq) if single else (b, t, hq))
             if not lse.is_contiguous():
                 raise ValueError("lse must be contiguous")
-            a.lse = lse.data_ptr()
         if window < 0:
             raise ValueError(f"window {window}: expected the number of keys, or 0 for all")
-        a.q, a.out, a.page_table, a.lengths = q.data_ptr(), out.data_ptr(), pages.data_ptr(), lengths.data_ptr()
         a.q_strides[:], a.out_strides[:] = (qb, qt, qh), (ob, ot, oh)
         a.table_stride, a.table_pages = pb, pages.shape[1]
-        a.batch, a.tokens, a.q_heads, a.window, a.causal = b, t, hq, window, causal
+        a.batch, a.tokens, a.q_heads, a.window, a.causal = b, t, hq, window, bool(causal)
         a.scale = d ** -0.5 if scale is None else scale
-        with _lib.on(self.device):
-            key = b, t, hq, pages.shape[1], window, q.dtype
-            room = self._room.get(key)
-            if room is None:
-                room = self._room[key] = _lib.lib().dlm_paged_attend_workspace_bytes(a)
-            if room:  # of this call alone: calls on other streams, and captured graphs, have their own
-                workspace = torch.empty(room, device=self.device, dtype=torch.uint8)
-                a.workspace, a.workspace_bytes = workspace.data_ptr(), room
-            code = _lib.lib().dlm_paged_attend(a, _lib.stream(q))
-        if code:
-            _lib.check(code, f"PagedKV.attend of {tuple(q.shape)} over {tuple(pages.shape)} pages")
-        return out
+        a.workspace_bytes = _lib.lib().dlm_paged_attend_workspace_bytes(a)
+        return a

@@ -341,12 +341,12 @@ typedef struct DlmAppend {
     const void* k;             /* [n, heads, head_dim] */
     const void* v;
     void* q_out;
-    int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];  /* token, head: elements, multiples of 8 */
     const int32_t* positions;  /* [n]; NULL where rotated is 0 */
     const int64_t* slots;      /* [n] page * page_size + slot of the page */
     const float* table;        /* [table_rows, rotated]: cosines of the rotated / 2 angles, then sines */
     const void* q_norm;        /* [head_dim] `type`, or NULL */
     const void* k_norm;
+    int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];  /* token, head: elements, multiples of 8 */
     int32_t n, q_heads, type;  /* type of q, k, v, q_out and the norms: DLM_BF16 or DLM_F16 */
     int32_t rotated;           /* a multiple of 16, at most head_dim; 0: no rotation */
     int32_t table_rows, interleaved;
@@ -369,11 +369,11 @@ typedef struct DlmAttend {
     const void* q;             /* [batch, tokens, q_heads, head_dim] `type` */
     void* out;
     float* lse;                /* [batch, tokens, q_heads] natural logarithm of the softmax's denominator, or NULL */
-    int64_t q_strides[3], out_strides[3];  /* sequence, token, head: elements, multiples of 8 */
     const int32_t* page_table; /* [batch, table_pages], rows table_stride apart */
     const int32_t* lengths;    /* [batch] keys of each sequence, the new ones included */
     void* workspace;           /* dlm_paged_attend_workspace_bytes() bytes, 16-byte aligned; nothing is kept in it */
     int64_t workspace_bytes;
+    int64_t q_strides[3], out_strides[3];  /* sequence, token, head: elements, multiples of 8 */
     int64_t table_stride;
     int32_t batch, tokens, q_heads, type;
     int32_t table_pages, window, causal;
@@ -392,10 +392,10 @@ typedef struct DlmAdapters {
     const void* x;             /* [m, k] BF16, rows ldx apart */
     const void* base;          /* [m, n] BF16, rows ldb apart */
     void* out;                 /* [m, n] BF16, rows ldo apart */
+    const int32_t* ids;        /* [m] adapter of each row, any order; negative: none */
     const void* a;             /* [count, rank, k] BF16 contiguous */
     const void* b;             /* [count, n, rank] BF16 contiguous */
     const float* scales;       /* [count] */
-    const int32_t* ids;        /* [m] adapter of each row, any order; negative: none */
     int32_t* status;           /* [DLM_STATUS_WORDS] or NULL; an id past `count` is DLM_ERR_INDEX and counts as none */
     int64_t ldx, ldb, ldo;     /* multiples of 8 */
     int32_t m, n, k, rank;     /* 1 <= m <= 256; n, k, rank multiples of 8; rank <= 128 */
