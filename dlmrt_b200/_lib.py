@@ -12,7 +12,7 @@ STATUS_WORDS = 4
 FUSED_MAX_N = 3072
 NOALLOC_SCRATCH_BYTES = 8 << 20
 GATHER_MAX_BYTES = 1 << 20
-MAX_PAGE = 4096
+MIN_PAGE, MAX_PAGE = 8, 4096
 
 OK, ERR_SHAPE, ERR_ALIGN, ERR_WORLD, ERR_NULL, ERR_GRID, ERR_CUDA, ERR_WORKSPACE, ERR_TIMEOUT, ERR_ARCH, \
     ERR_SCRATCH, ERR_OVERLAP, ERR_INDEX = 0, -1, -2, -3, -4, -5, -6, -7, -8, -9, -10, -11, -12

@@ -752,6 +752,13 @@ int dlm_rowpar_bf16_loopback(const DlmGemm* gemm, const DlmComm* comm, int nrank
 // ---------------------------------------------------------------------------------------------------------------------
 // Paged cache, attention over it, low-rank adapters
 // ---------------------------------------------------------------------------------------------------------------------
+// Strides are multiples of `of` elements and at least `least`; one along which there is a single step may be anything.
+static bool strides_ok(const int64_t* strides, const int* extents, int n, int of, int least) {
+    for (int i = 0; i < n; ++i)
+        if (extents[i] > 1 && (strides[i] < least || strides[i] % of)) return false;
+    return true;
+}
+
 // log2 of the page size in *shift.
 static int check_pages(const DlmPages* c, int* shift) {
     if (c->keys == nullptr || c->values == nullptr) return DLM_ERR_NULL;
@@ -759,20 +766,14 @@ static int check_pages(const DlmPages* c, int* shift) {
     if (c->type == DLM_E4M3 && (c->k_scale == nullptr || c->v_scale == nullptr)) return DLM_ERR_NULL;
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return DLM_ERR_SHAPE;
     if (c->heads < 1 || c->heads > 1024 || c->pages < 1) return DLM_ERR_SHAPE;
-    if (c->page_size < 1 || c->page_size > DLM_MAX_PAGE || (c->page_size & (c->page_size - 1))) return DLM_ERR_SHAPE;
+    if (c->page_size < DLM_MIN_PAGE || c->page_size > DLM_MAX_PAGE || (c->page_size & (c->page_size - 1))) return DLM_ERR_SHAPE;
     const int per_16_bytes = c->type == DLM_E4M3 ? 16 : 8;
-    for (int i = 0; i < 3; ++i)
-        if (c->k_strides[i] < 0 || c->v_strides[i] < 0 || c->k_strides[i] % per_16_bytes || c->v_strides[i] % per_16_bytes)
-            return DLM_ERR_ALIGN;
+    const int extents[3] = {c->pages, c->heads, c->page_size};
+    if (!strides_ok(c->k_strides, extents, 3, per_16_bytes, 1) || !strides_ok(c->v_strides, extents, 3, per_16_bytes, 1))
+        return DLM_ERR_ALIGN;
     if (!aligned16(c->keys) || !aligned16(c->values)) return DLM_ERR_ALIGN;
     *shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
     return DLM_OK;
-}
-
-static bool strides_of_8(const int64_t* strides, int n) {
-    for (int i = 0; i < n; ++i)
-        if (strides[i] < 0 || strides[i] % 8) return false;
-    return true;
 }
 
 int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
@@ -793,8 +794,9 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) || !aligned16(a->table) ||
         !aligned16(a->q_norm) || !aligned16(a->k_norm))
         return DLM_ERR_ALIGN;
-    if (!strides_of_8(a->k_strides, 2) || !strides_of_8(a->v_strides, 2) ||
-        (a->q != nullptr && (!strides_of_8(a->q_strides, 2) || !strides_of_8(a->out_strides, 2))))
+    const int kv_extents[2] = {a->n, a->cache.heads}, q_extents[2] = {a->n, a->q_heads};
+    if (!strides_ok(a->k_strides, kv_extents, 2, 8, 0) || !strides_ok(a->v_strides, kv_extents, 2, 8, 0) ||
+        (a->q != nullptr && (!strides_ok(a->q_strides, q_extents, 2, 8, 0) || !strides_ok(a->out_strides, q_extents, 2, 8, 1))))
         return DLM_ERR_ALIGN;
     DeviceInfo info;
     rc = device_info(&info);
@@ -820,23 +822,46 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     if (static_cast<long long>(a->cache.heads) * d->row_tiles > 1 << 20) return DLM_ERR_SHAPE;
     d->items = a->cache.heads * d->row_tiles;
     long long span = keys;  // from the first key that some token sees, aligned down, to the last
-    if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kUnitKeys < span)
-        span = static_cast<long long>(a->window) + a->tokens + kUnitKeys;
-    d->ctas = sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
-    d->least_units = kLeastUnits;
-    d->unit = kUnitKeys;
-    if (span <= kWholeKeys) {
-        d->unit = static_cast<int>(span < kUnitKeys ? kUnitKeys : (span + kUnitKeys - 1) / kUnitKeys * kUnitKeys);
-        d->least_units = 1;
-        const long long items = static_cast<long long>(a->batch) * d->items;
-        if (items < d->ctas) d->ctas = static_cast<int>(items);
+    if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kTileKeys < span)
+        span = static_cast<long long>(a->window) + a->tokens + kTileKeys;
+    const bool whole = span <= kWholeKeys;
+    d->unit_shift = whole ? 31 : kUnitShift;
+    d->least_units = whole ? 1 : kLeastUnits;
+    d->sms = sms;
+    d->resident = sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
+    const long long units = whole ? 1 : (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
+    const Cut cut = attend_cut(units * a->batch * d->items, d->resident, d->least_units);
+    d->grid = cut.across * cut.waves;
+    d->by_item = static_cast<long long>(a->batch) * d->items < d->grid;
+    return DLM_OK;
+}
+
+// The pool as TMA reads it for the attention kernel: boxes of up to 128 bytes x up to kTileKeys slots of one head and page.
+static int make_map_pages(CUtensorMap* map, const void* base, const DlmPages& c, const int64_t* strides) {
+    EncodeTiled fn = encode_tiled();
+    if (fn == nullptr) return DLM_ERR_CUDA;
+    const int size = c.type == DLM_E4M3 ? 1 : 2, row_bytes = c.head_dim * size;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(c.heads), static_cast<cuuint64_t>(c.pages)};
+    auto bytes = [&](int64_t stride, int extent) { return static_cast<cuuint64_t>(extent > 1 ? stride * size : row_bytes); };
+    const cuuint64_t steps[3] = {bytes(strides[2], c.page_size), bytes(strides[1], c.heads), bytes(strides[0], c.pages)};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(row_bytes < 128 ? c.head_dim : 128 / size),
+                               static_cast<cuuint32_t>(c.page_size < kTileKeys ? c.page_size : kTileKeys), 1, 1};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base),
+                          dims, steps, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          row_bytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        g_last_cuda_error = 100000 + static_cast<int>(r);
+        return DLM_ERR_CUDA;
     }
     return DLM_OK;
 }
 
 static int64_t attend_workspace(const DlmAttend* a, const AttendDev& d) {
-    if (d.unit != kUnitKeys) return 0;
-    return static_cast<int64_t>(d.ctas) * 2 * d.rows_cap * (a->cache.head_dim + 2) * 4;
+    if (d.unit_shift != kUnitShift || d.grid == 1) return 0;
+    return static_cast<int64_t>(d.grid) * 2 * d.rows_cap * (a->cache.head_dim + 2) * 4;
 }
 
 int64_t dlm_paged_attend_workspace_bytes(const DlmAttend* a) {
@@ -857,7 +882,9 @@ int dlm_paged_attend(const DlmAttend* a, dlm_stream_t stream) {
     int rc = plan_attend(a, 148, &d);  // the arguments; the plan itself once the device is known
     if (rc != DLM_OK) return rc;
     if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->workspace)) return DLM_ERR_ALIGN;
-    if (!strides_of_8(a->q_strides, 3) || !strides_of_8(a->out_strides, 3) || a->table_stride < 0) return DLM_ERR_ALIGN;
+    const int extents[3] = {a->batch, a->tokens, a->q_heads};
+    if (!strides_ok(a->q_strides, extents, 3, 8, 0) || !strides_ok(a->out_strides, extents, 3, 8, 1) || a->table_stride < 0)
+        return DLM_ERR_ALIGN;
     DeviceInfo info;
     rc = device_info(&info);
     if (rc == DLM_OK) rc = plan_attend(a, info.sms, &d);
@@ -870,6 +897,9 @@ int dlm_paged_attend(const DlmAttend* a, dlm_stream_t stream) {
         d.partial = static_cast<float*>(a->workspace);
         d.stats = d.partial + need / 4 / (a->cache.head_dim + 2) * a->cache.head_dim;
     }
+    rc = make_map_pages(&d.tm_k, a->cache.keys, a->cache, a->cache.k_strides);
+    if (rc == DLM_OK) rc = make_map_pages(&d.tm_v, a->cache.values, a->cache, a->cache.v_strides);
+    if (rc != DLM_OK) return rc;
     return launch_attend(d, {static_cast<cudaStream_t>(stream), a->pdl != 0, false});
 }
 

@@ -8,14 +8,20 @@
 //
 // The rows that share a key head are its query heads times the new tokens; 16 of them make the M of an mma.sync. A single
 // token fills a few rows and is bound by reading the cache, so the tensor instructions only have to keep up with HBM.
-// Each of a CTA's four warps takes every fourth tile of 16 keys through a ring of its own (cp.async, no block-wide step in
-// the main loop), with its own maximum, sum and output in registers; the four are joined in shared memory.
 //
-// Work is dealt out evenly, whatever the lengths: the keys of all items (an item: one sequence, key head and row tile) are
-// lined up in units of 64, and each of as many CTAs as the GPU holds at once takes one contiguous run of units. It goes
-// through the items of its run without draining the ring in between, so one item's end overlaps the next one's loads. An
-// item that lies in several runs leaves a partial result in each, which join_kernel adds up in order. Every CTA reads all
-// lengths and works its run out by itself.
+//   warp 4     deals out the work and requests keys and values: steps of 64 keys into a ring of stages, as TMA boxes of a
+//              page's slots (pages in any order; up to 64 slots a box).
+//   warps 0-3  take 16 keys of every step each, with their own maximum, sum and output in registers: no step in which they
+//              wait for one another but an item's end, where the four are joined in shared memory.
+//
+// An item is one sequence, key head and row tile. The keys of all items are lined up in units of 64 keys and cut into runs,
+// whatever the lengths of the sequences. The first runs, half of the line, go to as many CTAs as the GPU holds; a CTA that is
+// done takes over the run of a CTA that was not launched yet (cluster launch control). Runs get shorter towards the line's
+// end, because SMs do not read equally fast: with one run for each CTA the slowest came in 30 % behind the others. Requests
+// go on across items and runs. An item that lies in several runs leaves a partial result in each, which join_kernel adds up
+// in their order: the result does not depend on which CTA took which run.
+#include <climits>
+
 #include "mma.cuh"
 #include "serving.cuh"
 
@@ -23,10 +29,10 @@ namespace dlm {
 
 namespace {
 
-constexpr int kAttendWarps = 4;
-constexpr int kAttendThreads = kAttendWarps * 32;
-constexpr int kTileKeys = 16;
-constexpr int kJoinRows = 4;  // rows of a tile that the warps exchange at a time
+constexpr int kConsumers = 4;                            // warps that compute
+constexpr int kAttendThreads = (kConsumers + 1) * 32;
+constexpr int kWarpKeys = kTileKeys / kConsumers;        // 16
+constexpr int kWorkSlots = 4;                            // items that may be announced ahead
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A sequence's keys: how many, the position of its first new token, where its units begin, and how many an item of it has.
@@ -41,92 +47,101 @@ __device__ __forceinline__ Sequence sequence_of(const AttendDev& p, int index, b
     s.length = length < 0 ? 0 : length > room ? static_cast<int>(room) : length;
     if (tell && s.length != length) report_index(p.a.cache.status, index, kIndexLength, length);
     s.first_pos = s.length - p.a.tokens;
-    s.base = (p.a.window > 0 ? max(0, s.first_pos - p.a.window + 1) : 0) & ~(kUnitKeys - 1);
-    s.units = max(1, (s.length - s.base + p.unit - 1) / p.unit);
+    s.base = (p.a.window > 0 ? max(0, s.first_pos - p.a.window + 1) : 0) & ~(kTileKeys - 1);
+    s.units = max(1, static_cast<int>((static_cast<uint32_t>(s.length - s.base) + (1u << p.unit_shift) - 1) >> p.unit_shift));
     return s;
 }
 // Keys that a token sees: [seen_from, seen_to).
-__device__ __forceinline__ int seen_from(const AttendDev& p, const Sequence& s, int token) {
-    return p.a.window > 0 ? max(0, s.first_pos + token - p.a.window + 1) : 0;
+__device__ __forceinline__ int seen_from(const AttendDev& p, int first_pos, int token) {
+    return p.a.window > 0 ? max(0, first_pos + token - p.a.window + 1) : 0;
 }
-__device__ __forceinline__ int seen_to(const AttendDev& p, const Sequence& s, int token) {
-    return p.a.causal ? min(s.length, s.first_pos + token + 1) : s.length;
+__device__ __forceinline__ int seen_to(const AttendDev& p, int first_pos, int length, int token) {
+    return p.a.causal ? min(length, first_pos + token + 1) : length;
 }
 
-// The line of units: `total` of them over `ctas` CTAs, the first `extra` of which have one more than `each`.
+// a / b of what is nearly always below 2^32: a 64-bit division takes a hundred instructions.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+// The line of units and its runs (see attend_cut). Every warp that needs it works it out for itself: a lane looks at a range
+// of the sequences.
 struct Line {
-    long long total, each;
-    int ctas, extra;
-    __device__ long long begin(int cta) const { return each * cta + min(cta, extra); }
-    __device__ int owner(long long unit) const {
-        const long long longer = (each + 1) * extra;
-        return static_cast<int>(unit < longer ? unit / (each + 1) : extra + (unit - longer) / each);
-    }
-};
+    long long total;
+    Cut cut;
+    int runs;
+    int first, last;    // this lane's sequences
+    long long before;   // units in front of them
+    long long mine;     // units of them
 
-struct Place {  // of a unit: its sequence, and the units in front of that sequence
-    int sequence;
-    long long before;
-};
-
-// Works out the line, and where unit `of(line)` lies. All threads of the block (a multiple of 32, at most 256).
-template <int kThreads, typename F>
-__device__ __forceinline__ Line lay_out(const AttendDev& p, int ctas, bool tell, F of, long long* unit, Place* place) {
-    __shared__ long long warp_sum[kThreads / 32];
-    __shared__ Place found;
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int per = (p.a.batch + kThreads - 1) / kThreads;
-    const int first = min(tid * per, p.a.batch), last = min(first + per, p.a.batch);
-    long long mine = 0;
-    for (int i = first; i < last; ++i) mine += static_cast<long long>(sequence_of(p, i, tell).units) * p.items;
-    long long before = mine;
+    __device__ __forceinline__ Line(const AttendDev& p, bool tell) {
+        const int lane = threadIdx.x & 31;
+        const int per = (p.a.batch + 31) / 32;
+        first = min(lane * per, p.a.batch), last = min(first + per, p.a.batch);
+        mine = 0;
+        for (int i = first; i < last; ++i) mine += sequence_of(p, i, tell).units;
+        mine *= p.items;
+        before = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xFFFFFFFFu, before, o);
-        if (lane >= o) before += up;
-    }
-    if (lane == 31) warp_sum[tid >> 5] = before;
-    before -= mine;
-    if (tid == 0) found.sequence = p.a.batch, found.before = 0;
-    __syncthreads();
-    Line line;
-    line.total = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-        if (w == tid >> 5) before += line.total;
-        line.total += warp_sum[w];
-    }
-    const long long most = (line.total + p.least_units - 1) / p.least_units;
-    line.ctas = static_cast<int>(most < ctas ? most : ctas);
-    line.each = line.total / line.ctas;
-    line.extra = static_cast<int>(line.total % line.ctas);
-    *unit = of(line);
-    if (*unit >= before && *unit < before + mine) {
-        for (int i = first; i < last; ++i) {
-            const long long units = static_cast<long long>(sequence_of(p, i, false).units) * p.items;
-            if (*unit < before + units) {
-                found.sequence = i, found.before = before;
-                break;
-            }
-            before += units;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xFFFFFFFFu, before, o);
+            if (lane >= o) before += up;
         }
+        total = __shfl_sync(0xFFFFFFFFu, before, 31);
+        before -= mine;
+        cut = attend_cut(total, p.resident, p.least_units);
+        runs = cut.across * cut.waves;
     }
-    __syncthreads();
-    *place = found;
-    return line;
-}
+    __device__ __forceinline__ long long wave_begin(int wave) const { return wave < cut.waves ? total - (total >> wave) : total; }
+    __device__ __forceinline__ long long begin(int run) const {  // rounded down: no run of a wave is empty
+        const int wave = run / cut.across, i = run - wave * cut.across;
+        const long long from = wave_begin(wave);
+        return from + (i == 0 ? 0 : divide((wave_begin(wave + 1) - from) * i, cut.across));
+    }
+    __device__ __forceinline__ int run_of(long long unit) const {
+        int wave = 0;
+        while (wave + 1 < cut.waves && unit >= wave_begin(wave + 1)) ++wave;
+        const long long from = wave_begin(wave);
+        return wave * cut.across + static_cast<int>(divide((unit - from + 1) * cut.across - 1, wave_begin(wave + 1) - from));
+    }
+    // The units in front of a sequence. All lanes of the warp.
+    __device__ __forceinline__ long long in_front_of(const AttendDev& p, int sequence) const {
+        const int per = (p.a.batch + 31) / 32, holder = sequence / per;
+        long long front = __shfl_sync(0xFFFFFFFFu, before, holder);
+        for (int i = holder * per; i < sequence; ++i) front += static_cast<long long>(sequence_of(p, i, false).units) * p.items;
+        return front;
+    }
+    // The sequence that holds a unit, and the units in front of that sequence. All lanes of the warp.
+    __device__ __forceinline__ int sequence_at(const AttendDev& p, long long unit, long long* in_front) const {
+        int sequence = first;
+        long long front = before;
+        const bool here = unit >= before && unit < before + mine;
+        if (here) {
+            for (; sequence < last - 1; ++sequence) {
+                const long long units = static_cast<long long>(sequence_of(p, sequence, false).units) * p.items;
+                if (unit < front + units) break;
+                front += units;
+            }
+        }
+        const uint32_t holder = __ballot_sync(0xFFFFFFFFu, here);
+        const int from = holder ? __ffs(holder) - 1 : 0;
+        *in_front = __shfl_sync(0xFFFFFFFFu, front, from);
+        return __shfl_sync(0xFFFFFFFFu, sequence, from);
+    }
+};
 
-// One warp's stage: 16 keys, then 16 values, rows of head_dim elements in 16-byte pieces whose order is permuted by row so
-// that ldmatrix (and, for FP8 keys, 16-byte loads of four lanes per row) meets each bank once.
+// A stage: 64 keys, then 64 values, as TMA writes them: column blocks of up to 128 bytes, in each the rows one after the
+// other with their 16-byte pieces permuted by row (the 128- or 64-byte swizzle), so that ldmatrix meets each bank once.
 template <int D, bool kCodes>
 struct Stage {
-    static constexpr int kPieces = D * (kCodes ? 1 : 2) / 16;  // of a row
-    static constexpr int kBytes = kTileKeys * kPieces * 16;     // of the keys, or of the values
-    __device__ static __forceinline__ int value_piece(int row, int c) {
-        return kPieces == 4 ? c ^ ((row >> 1) & 3) : c ^ (row & 7);
-    }
-    __device__ static __forceinline__ int key_piece(int row, int c) {
-        return !kCodes || kPieces == 4 ? value_piece(row, c) : c ^ ((row & 1) << 2);
+    static constexpr int kPieces = D * (kCodes ? 1 : 2) / 16;           // 16-byte pieces of a row
+    static constexpr int kBytes = kTileKeys * kPieces * 16;              // of the keys, or of the values
+    static constexpr int kAcross = kPieces < 8 ? kPieces : 8;            // pieces of a column block's row
+    static constexpr int kBlocks = kPieces / kAcross;
+    static constexpr int kBlockBytes = kTileKeys * kAcross * 16;
+    __device__ static __forceinline__ int at(int row, int piece) {
+        const int turn = kAcross == 8 ? row & 7 : (row >> 1) & 3;
+        return (piece / kAcross) * kBlockBytes + row * (kAcross * 16) + ((piece % kAcross) ^ turn) * 16;
     }
 };
 
@@ -138,21 +153,73 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return __vcmpeq2(w & kExponent, kExponent);
 }
 
-constexpr int kStages = 3;
-
-// Dynamic shared memory: the warps' rings, four rows of each warp's output, and (kQueriesInShared) the A operands of all
-// k16 steps, in the order of the lanes.
+// Shared memory of a CTA, and how many CTAs an SM holds of it (registers are held to what they leave each other).
 template <int D, bool kCodes>
 struct AttendSmem {
-    static constexpr bool kQueriesInShared = D == 256;  // 64 registers of queries and 128 of output leave too few
-    static constexpr int kRing = kStages * kAttendWarps * 2 * Stage<D, kCodes>::kBytes;
+    static constexpr int kCtas = D == 64 ? 3 : D == 256 && !kCodes ? 1 : 2;
+    static constexpr int kStages = D == 64 ? (kCodes ? 6 : 4) : D == 128 && kCodes ? 6 : 3;
+    static constexpr int kRing = kStages * 2 * Stage<D, kCodes>::kBytes;
     static constexpr int kPitch = D + 4;
-    static constexpr int kJoin = kAttendWarps * kJoinRows * kPitch * 4;
-    static constexpr int kQueries = kQueriesInShared ? D / 16 * 512 : 0;
-    static constexpr int kBytes = kRing + kJoin + kQueries;
-    // CTAs that an SM holds; registers are held to what they leave each other.
-    static constexpr int kCtas = D == 256 ? (kCodes ? 2 : 1) : D == 128 ? (kCodes ? 3 : 2) : 4;
+    static constexpr int kJoinRows = D == 256 ? 2 : 4;  // rows of a tile that the warps exchange at a time
+    static constexpr int kJoin = kConsumers * kJoinRows * kPitch * 4;
+    static constexpr bool kQueriesInShared = D == 256;  // 64 registers of queries and 128 of output leave too few
+    static constexpr int kQueries = kQueriesInShared ? D / 16 * 512 : 0;  // A operands of all k16 steps, in the order of lanes
+    static constexpr int kWeights = kConsumers * kRowTile * (kWarpKeys + 1) * 4;
+    static constexpr int kUsed = kQueries + kWeights;    // while keys are read; the join uses the same bytes afterwards
+    static constexpr int kBytes = kRing + (kJoin > kUsed ? kJoin : kUsed) + 1024;  // the ring begins at a multiple of 1024
 };
+
+// What the consumers have to know of an item in a run.
+struct Work {
+    int sequence, head, row_tile;  // head -1: there is no more work
+    int length, first_pos;
+    int start, end, tiles;         // keys of this run, steps of 64 of them
+    int whole;                     // all keys of the item are in this run
+    int piece;                     // otherwise: index of its partial result
+};
+
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
+
+__device__ __forceinline__ bool consumers_any(bool vote) {
+    int any;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.s32 p, %1, 0;\n"
+        "barrier.cta.red.or.pred q, 1, %2, p;\n"
+        "selp.s32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(any)
+        : "r"(static_cast<int>(vote)), "n"(kConsumers * 32)
+        : "memory");
+    return any != 0;
+}
+
+// Asks for the block index of a CTA that was not launched yet, which then never will be: 16 bytes that arrive on `bar`.
+__device__ __forceinline__ void ask_for_cta(uint4* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The block index of an answer, or -1 where every CTA has been launched.
+__device__ __forceinline__ int cta_of(const uint4* answer) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n"
+        ".reg .b128 a;\n"
+        ".reg .pred p;\n"
+        ".reg .b32 y, z, w;\n"
+        "ld.shared.b128 a, [%2];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
+        "selp.u32 %1, 1, 0, p;\n"
+        "mov.u32 %0, 0;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, a;\n"
+        "}\n"
+        : "=&r"(x), "=&r"(got)
+        : "r"(smem_u32(answer))
+        : "memory");
+    return got ? static_cast<int>(x) : -1;
+}
 
 }  // namespace
 
@@ -176,147 +243,202 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     using M = typename std::conditional<kCodes, __half, T>::type;
     using S = Stage<D, kCodes>;
     using Shared = AttendSmem<D, kCodes>;
+    constexpr int kStages = Shared::kStages;
     constexpr int kSteps = D / 16;       // k16 steps of q . k
     constexpr int kOut = D / 8;          // n8 tiles of the output
     constexpr int kElem = kCodes ? 1 : 2;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float warp_stats[kAttendWarps][kRowTile][2];
-    __shared__ uint32_t present_keys[kAttendWarps][4];
-    __shared__ float weights_of_tile[kAttendWarps][kRowTile][kTileKeys + 1];
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full[kStages], empty[kStages], work_full[kWorkSlots], work_empty[kWorkSlots], answered;
+    __shared__ uint4 answer;
+    __shared__ Work works[kWorkSlots];
+    __shared__ uint64_t present_keys[kStages];
+    __shared__ float warp_stats[kConsumers][kRowTile][2];
 
     const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    const int g = lane >> 2, t = lane & 3;
-    const int cta = blockIdx.x;
+    const bool leader = elect_one();
+    if (warp == kConsumers && leader) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], kConsumers);
+        for (int i = 0; i < kWorkSlots; ++i) mbar_init(&work_full[i], 1), mbar_init(&work_empty[i], kConsumers);
+        mbar_init(&answered, 1);
+        fence_barrier_init();
+        tma_prefetch_descriptor(&p.tm_k);
+        tma_prefetch_descriptor(&p.tm_v);
+    }
+    __syncthreads();
+    const long long deadline = globaltimer() + kDefaultTimeoutNs;
     pdl_wait();
     pdl_launch_dependents();
-    long long unit;
-    Place place;
-    const Line line = lay_out<kAttendThreads>(p, gridDim.x, cta == 0, [&](const Line& l) { return l.begin(cta); }, &unit, &place);
-    if (cta >= line.ctas) return;
-    const long long last_unit = line.begin(cta + 1);
+    // A wait that runs out is reported; what follows is computed from whatever is there, and nothing more is requested.
+    auto stalled = [&](int who, int at) { report(p.a.cache.status, kErrTimeout, who, kPhasePipeline, at); };
 
-    // Where an item of this run is, and which of its keys are in it.
-    struct Item {
-        Sequence s;
-        int sequence, index;     // index: key head * row tiles + row tile
-        int head, row_tile;
-        int first, units;        // units of this run
-        int start, end;          // their keys, as far as some row of the tile sees them
-        int tiles;               // of 16 keys
-        int lo;                  // first key that some row sees
-    };
-    auto narrow_to_run = [&](Item& item, long long left) {
-        item.head = item.index / p.row_tiles, item.row_tile = item.index - item.head * p.row_tiles;
-        item.units = static_cast<int>(left < item.s.units - item.first ? left : item.s.units - item.first);
-        const int first_row = item.row_tile * kRowTile, last_row = min(first_row + kRowTile, p.rows) - 1;
-        item.lo = seen_from(p, item.s, first_row / p.group);
-        const int hi = seen_to(p, item.s, last_row / p.group);
-        const long long to = item.s.base + static_cast<long long>(item.first + item.units) * p.unit;
-        item.start = max(item.s.base + item.first * p.unit, item.lo & ~(kTileKeys - 1));
-        item.end = static_cast<int>(to < hi ? to : hi);
-        item.tiles = item.end > item.start ? (item.end - item.start + kTileKeys - 1) / kTileKeys : 0;
-    };
-    auto next_item = [&](Item& item, long long left) {
-        item.first = 0;
-        if (++item.index == p.items) {
-            item.index = 0;
-            item.s = sequence_of(p, ++item.sequence, false);
-        }
-        narrow_to_run(item, left);
-    };
-    Item item;
-    item.sequence = place.sequence;
-    item.s = sequence_of(p, item.sequence, false);
-    {
-        const long long inside = unit - place.before;
-        item.index = static_cast<int>(inside / item.s.units);
-        item.first = static_cast<int>(inside - static_cast<long long>(item.index) * item.s.units);
-    }
-    narrow_to_run(item, last_unit - unit);
-
-    // -- the ring: this warp's tiles of all items of the run, one after the other ----------------------------------------
-    uint8_t* ring = smem + warp * (kStages * 2 * S::kBytes);
-    const uint32_t ring_u32 = smem_u32(ring);
-    const long long k_page = p.a.cache.k_strides[0] * kElem, k_slot = p.a.cache.k_strides[2] * kElem;
-    const long long v_page = p.a.cache.v_strides[0] * kElem, v_slot = p.a.cache.v_strides[2] * kElem;
-    const int slot_mask = (1 << p.page_shift) - 1;
-    Item ahead = item;                       // the item whose tiles are being requested
-    long long ahead_left = last_unit - unit; // units of the run from its beginning on
-    int ahead_tile = warp;
-    int page_ahead = -1;                     // lane r of the lower half: page of key r of the tile to be requested next
-    auto settle = [&]() -> bool {            // moves `ahead` to an item that still has a tile for this warp; fetches its pages
-        while (ahead_tile >= ahead.tiles) {
-            ahead_left -= ahead.units;
-            if (ahead_left <= 0) return false;
-            next_item(ahead, ahead_left);
-            ahead_tile = warp;
-        }
-        const int key = ahead.start + ahead_tile * kTileKeys + lane;
-        page_ahead = -1;
-        if (lane < kTileKeys && key < ahead.end) {
-            const int page = p.a.page_table[ahead.sequence * p.a.table_stride + (key >> p.page_shift)];
-            if (page >= 0 && page < p.a.cache.pages) page_ahead = page;
-            else if (key >= ahead.lo) report_index(p.a.cache.status, ahead.sequence, kIndexPage, page);
-        }
-        return true;
-    };
-    bool more = settle();
-    auto issue = [&](int stage) {
-        if (more) {
-            const int page = page_ahead;
-            const uint32_t present = __ballot_sync(0xFFFFFFFFu, page >= 0);
-            if (lane == 0) present_keys[warp][stage] = present;
-            const int key0 = ahead.start + ahead_tile * kTileKeys;
-            const uint8_t* keys = static_cast<const uint8_t*>(p.a.cache.keys) + ahead.head * p.a.cache.k_strides[1] * kElem;
-            const uint8_t* values = static_cast<const uint8_t*>(p.a.cache.values) + ahead.head * p.a.cache.v_strides[1] * kElem;
-            const uint32_t to = ring_u32 + stage * 2 * S::kBytes;
-            constexpr int kRowsAtOnce = 32 / S::kPieces;
-            const int c = lane % S::kPieces, r0 = lane / S::kPieces;
-#pragma unroll
-            for (int i = 0; i < kTileKeys / kRowsAtOnce; ++i) {
-                const int r = r0 + i * kRowsAtOnce;
-                const int id = __shfl_sync(0xFFFFFFFFu, page, r);
-                const bool there = id >= 0;
-                const long long at = there ? id : 0;
-                const int slot = (key0 + r) & slot_mask;
-                cp_async_16(to + (r * S::kPieces + S::key_piece(r, c)) * 16, keys + at * k_page + slot * k_slot + c * 16, there);
-                cp_async_16(to + S::kBytes + (r * S::kPieces + S::value_piece(r, c)) * 16,
-                            values + at * v_page + slot * v_slot + c * 16, there);
+    if (warp == kConsumers) {
+        // -- the producer -------------------------------------------------------------------------------------------
+        const Line line(p, blockIdx.x == 0);
+        const int box_keys = min(kTileKeys, 1 << p.page_shift), boxes = kTileKeys / box_keys;
+        const int slot_mask = (1 << p.page_shift) - 1;
+        int stage = 0, slot = 0, run = blockIdx.x;
+        uint32_t parity = 1, slot_parity = 1, answer_parity = 0;  // the first lap of a ring waits for nothing
+        bool failed = false;
+        auto announce = [&](const Work& work) {
+            if (!mbar_wait_warp(&work_empty[slot], slot_parity, deadline) && !failed) {
+                failed = true;
+                if (leader) stalled(0, run);
             }
-            ahead_tile += kAttendWarps;
-            more = settle();
-        }
-        cp_async_commit();
-    };
+            if (leader) {
+                works[slot] = work;
+                mbar_arrive(&work_full[slot]);
+            }
+            if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
+        };
+        // Where the next step is: a run, an item in it, a step of 64 keys in that. Its pages are looked up a step ahead of its
+        // use, across items and runs: lane j asks for the page of box j.
+        long long unit = 0, last_unit = 0;
+        int sequence = 0, index = 0, first = 0, units = 0, lo = 0, tile = 0, page = INT_MIN;
+        Sequence s{};
+        Work work{};
+        auto look_up = [&]() {
+            const int key = work.start + tile * kTileKeys + lane * box_keys;
+            page = lane < boxes && key < work.end ? p.a.page_table[sequence * p.a.table_stride + (key >> p.page_shift)] : INT_MIN;
+        };
+        auto begin_item = [&]() {
+            units = static_cast<int>(last_unit - unit < s.units - first ? last_unit - unit : s.units - first);
+            work.sequence = sequence, work.length = s.length, work.first_pos = s.first_pos;
+            work.head = index / p.row_tiles, work.row_tile = index - work.head * p.row_tiles;
+            const int first_row = work.row_tile * kRowTile, last_row = min(first_row + kRowTile, p.rows) - 1;
+            lo = seen_from(p, s.first_pos, first_row / p.group);
+            const int hi = seen_to(p, s.first_pos, s.length, last_row / p.group);
+            work.whole = units == s.units;
+            work.piece = run * 2 + (first == 0);  // a run has at most one that began before it and one that goes on
+            work.start = max(s.base + (first << p.unit_shift), lo & ~(kTileKeys - 1));  // first is 0 if units are whole items
+            work.end = first + units == s.units ? hi : min(hi, s.base + ((first + units) << p.unit_shift));
+            work.tiles = work.end > work.start ? (work.end - work.start + kTileKeys - 1) / kTileKeys : 0;
+            tile = 0;
+            look_up();
+        };
+        auto begin_run = [&]() -> bool {
+            if (run < 0 || run >= line.runs) return false;
+            if (leader) {
+                fence_proxy_async();  // the last answer has been read
+                mbar_expect_tx(&answered, sizeof(answer));
+                ask_for_cta(&answer, &answered);
+            }
+            unit = line.begin(run), last_unit = line.begin(run + 1);
+            long long in_front;
+            sequence = line.sequence_at(p, unit, &in_front);
+            s = sequence_of(p, sequence, false);
+            index = static_cast<int>(divide(unit - in_front, s.units));  // key head * row tiles + row tile
+            first = static_cast<int>(unit - in_front - static_cast<long long>(index) * s.units);
+            begin_item();
+            return true;
+        };
+        auto advance = [&]() -> bool {
+            if (++tile < work.tiles) {
+                look_up();
+                return true;
+            }
+            unit += units;
+            if (unit < last_unit) {
+                first = 0;
+                if (++index == p.items) index = 0, s = sequence_of(p, ++sequence, false);
+                begin_item();
+                return true;
+            }
+            if (!mbar_wait_warp(&answered, answer_parity, deadline)) {
+                if (leader) stalled(2, run);
+                return false;
+            }
+            answer_parity ^= 1;
+            run = cta_of(&answer);
+            __syncwarp();
+            return begin_run();
+        };
+        bool more = begin_run();
+        while (more) {
+            const Work now = work;
+            const int now_tile = tile, now_lo = lo;
+            int now_page = page;
+            more = advance();
+            if (now_tile == 0) announce(now);
+            if (now.tiles == 0) continue;
+            const int key0 = now.start + now_tile * kTileKeys;
+            const bool in_pool = now_page >= 0 && now_page < p.a.cache.pages;
+            if (!in_pool && now_page != INT_MIN && key0 + (lane + 1) * box_keys > now_lo)
+                report_index(p.a.cache.status, now.sequence, kIndexPage, now_page);
+            const uint32_t there = __ballot_sync(0xFFFFFFFFu, in_pool);
+            if (!in_pool) now_page = p.a.cache.pages;  // past the pool's end: the box is filled with zeros
+            if (!mbar_wait_warp(&empty[stage], parity, deadline) && !failed) {
+                failed = true;
+                if (leader) stalled(1, now_tile);
+            }
+            uint8_t* to = smem + stage * 2 * S::kBytes;
+            uint64_t* bar = &full[stage];
+            if (leader) {
+                uint64_t present = 0;
+                const uint64_t box_bits = box_keys == 64 ? ~0ull : (1ull << box_keys) - 1;
+                for (int j = 0; j < boxes; ++j)
+                    if (there >> j & 1) present |= box_bits << (j * box_keys);
+                if (now.end - key0 < kTileKeys) present &= (1ull << (now.end - key0)) - 1;
+                present_keys[stage] = present;
+                if (failed) mbar_arrive(bar);
+                else mbar_expect_tx(bar, 2 * S::kBytes);
+            }
+            for (int j = 0; j < boxes; ++j) {
+                const int from = __shfl_sync(0xFFFFFFFFu, now_page, j);
+                const int at = (key0 + j * box_keys) & slot_mask, row = j * box_keys * S::kAcross * 16;
+                if (leader && !failed) {
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) issue(s);
-    int stage = 0, fill = kStages - 1;
+                    for (int c = 0; c < S::kBlocks; ++c) {
+                        tma_load_4d(to + c * S::kBlockBytes + row, &p.tm_k, bar, c * (128 / kElem), at, now.head, from, kEvictNormal);
+                        tma_load_4d(to + S::kBytes + c * S::kBlockBytes + row, &p.tm_v, bar, c * (128 / kElem), at, now.head, from,
+                                    kEvictNormal);
+                    }
+                }
+            }
+            if (++stage == kStages) stage = 0, parity ^= 1;
+        }
+        Work none;
+        none.head = -1;
+        announce(none);
+        return;
+    }
 
+    // -- the consumers --------------------------------------------------------------------------------------------------
+    const int g = lane >> 2, t = lane & 3;
+    int stage = 0, slot = 0;
+    uint32_t parity = 0, slot_parity = 0;
     while (true) {
+    const bool announced = mbar_wait_warp(&work_full[slot], slot_parity, deadline);
+    if (!announced && leader) stalled(3, slot);
+    if (consumers_any(!announced)) return;  // none of the warps may wait for the others any more
+    const Work item = works[slot];
+    __syncwarp();
+    if (leader) mbar_arrive(&work_empty[slot]);
+    if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
+    if (item.head < 0) return;
     const int sequence = item.sequence, head = item.head, row_tile = item.row_tile;
     // This thread's two rows: g and g + 8 of the tile.
     const int row0 = row_tile * kRowTile + g, row1 = row0 + 8;
     const int token0 = min(row0, p.rows - 1) / p.group, token1 = min(row1, p.rows - 1) / p.group;
-    const int from0 = seen_from(p, item.s, token0), to0 = seen_to(p, item.s, token0);
-    const int from1 = seen_from(p, item.s, token1), to1 = seen_to(p, item.s, token1);
+    const int from0 = seen_from(p, item.first_pos, token0), to0 = seen_to(p, item.first_pos, item.length, token0);
+    const int from1 = seen_from(p, item.first_pos, token1), to1 = seen_to(p, item.first_pos, item.length, token1);
     const int last_row = min(row_tile * kRowTile + kRowTile, p.rows) - 1;
-    const int all_from = seen_from(p, item.s, last_row / p.group);               // from here on every row sees the keys
-    const int all_to = seen_to(p, item.s, (row_tile * kRowTile) / p.group);      // up to here
+    const int all_from = seen_from(p, item.first_pos, last_row / p.group);                          // from here on every row sees
+    const int all_to = seen_to(p, item.first_pos, item.length, (row_tile * kRowTile) / p.group);    // the keys, up to here
 
     auto q_row = [&](int row) -> const T* {
         const int token = row / p.group, of = row - token * p.group;
         return static_cast<const T*>(p.a.q) + sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
                static_cast<long long>(head * p.group + of) * p.a.q_strides[2];
     };
-    // Queries as the A operand. With FP8 keys the contraction runs in the order in which a lane's 16-byte piece of a key
-    // row holds them: step 4s + j of lane t covers elements 64 s + 16 t + 4 j .. + 3.
+    // Queries as the A operand. With FP8 keys a lane's elements of a k16 step are four neighbours (see below).
     uint32_t q[kSteps][4];
     const bool has0 = row0 < p.rows, has1 = row1 < p.rows;
     const T* q0 = has0 ? q_row(row0) : nullptr;
     const T* q1 = has1 ? q_row(row1) : nullptr;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-        const int at0 = kCodes ? (s / 4) * 64 + t * 16 + (s % 4) * 4 : s * 16 + t * 2;
+        const int at0 = s * 16 + t * (kCodes ? 4 : 2);
         const int at1 = at0 + (kCodes ? 2 : 8);
         q[s][0] = has0 ? *reinterpret_cast<const uint32_t*>(q0 + at0) : 0;
         q[s][1] = has1 ? *reinterpret_cast<const uint32_t*>(q1 + at0) : 0;
@@ -364,13 +486,13 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
 
     const uint32_t* shared_q = nullptr;
     if constexpr (Shared::kQueriesInShared) {
-        uint32_t* to = reinterpret_cast<uint32_t*>(smem + Shared::kRing + Shared::kJoin);
+        uint32_t* to = reinterpret_cast<uint32_t*>(smem + Shared::kRing);
         if (warp == 0) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
                 *reinterpret_cast<uint4*>(to + (s * 32 + lane) * 4) = make_uint4(q[s][0], q[s][1], q[s][2], q[s][3]);
         }
-        __syncthreads();
+        consumers_sync();
         shared_q = to + lane * 4;
     }
 
@@ -379,14 +501,13 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     for (int i = 0; i < kOut; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-    for (int tile = warp; tile < item.tiles; tile += kAttendWarps) {
-        cp_async_wait<kStages - 2>();
-        __syncwarp();  // every lane's copies of this stage have landed, and every lane is done with the stage before
-        issue(fill);
-        const int key0 = item.start + tile * kTileKeys;
-        const uint8_t* stage_k = ring + stage * 2 * S::kBytes;
-        const uint32_t stage_k32 = ring_u32 + stage * 2 * S::kBytes, stage_v32 = stage_k32 + S::kBytes;
-        const uint32_t present = present_keys[warp][stage];
+    for (int tile = 0; tile < item.tiles; ++tile) {
+        if (!mbar_wait_warp(&full[stage], parity, deadline) && leader) stalled(4, tile);
+        const int key0 = item.start + tile * kTileKeys + warp * kWarpKeys;
+        uint8_t* stage_k = smem + stage * 2 * S::kBytes;
+        const uint32_t stage_k32 = smem_u32(stage_k), stage_v32 = stage_k32 + S::kBytes;
+        const uint32_t present = static_cast<uint32_t>(present_keys[stage] >> (warp * kWarpKeys)) & 0xFFFFu;
+        const int row_base = warp * kWarpKeys;
 
         auto query_step = [&](int k, uint32_t (&a)[4]) {
             if constexpr (Shared::kQueriesInShared) {
@@ -400,33 +521,37 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         // scores: columns are keys, 0..7 in s[0], 8..15 in s[1]
         float s[2][4] = {};
         if constexpr (!kCodes) {
-            const int r = (lane & 7) + ((lane >> 4) << 3);
+            const int r = row_base + (lane & 7) + ((lane >> 4) << 3);
+            float more_s[2][4] = {};  // odd steps: half as long a chain of dependent products
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 uint32_t a[4], b[4];
                 query_step(k, a);
-                ldmatrix_x4(b, stage_k32 + (r * S::kPieces + S::key_piece(r, 2 * k + ((lane >> 3) & 1))) * 16);
-                mma_16816<M>(s[0], a, b[0], b[1]);
-                mma_16816<M>(s[1], a, b[2], b[3]);
+                ldmatrix_x4(b, stage_k32 + S::at(r, 2 * k + ((lane >> 3) & 1)));
+                mma_16816<M>(k & 1 ? more_s[0] : s[0], a, b[0], b[1]);
+                mma_16816<M>(k & 1 ? more_s[1] : s[1], a, b[2], b[3]);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i], s[1][i] += more_s[1][i];
         } else {
+            // A 16-byte piece of a key row is one k16 step: lane t of a row holds its elements 4t .. 4t + 3.
+            const int r = row_base + (lane & 7) + (((lane >> 3) & 1) << 3);
+            float more_s[2][4] = {};
 #pragma unroll
-            for (int k4 = 0; k4 < kSteps / 4; ++k4) {
-                uint32_t a[4][4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) query_step(4 * k4 + j, a[j]);
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int r = g + 8 * n;
-                    const uint4 w = *reinterpret_cast<const uint4*>(stage_k + (r * S::kPieces + S::key_piece(r, 4 * k4 + t)) * 16);
-                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        mma_16816<M>(s[n], a[j], e4m3x2_to_f16x2(words[j] & 0xFFFFu), e4m3x2_to_f16x2(words[j] >> 16));
-                }
+            for (int k = 0; k < kSteps; k += 2) {
+                uint32_t a0[4], a1[4], b[4];
+                query_step(k, a0);
+                query_step(k + 1, a1);
+                ldmatrix_x4(b, stage_k32 + S::at(r, k + (lane >> 4)));
+                mma_16816<M>(s[0], a0, e4m3x2_to_f16x2(b[0] & 0xFFFFu), e4m3x2_to_f16x2(b[0] >> 16));
+                mma_16816<M>(s[1], a0, e4m3x2_to_f16x2(b[1] & 0xFFFFu), e4m3x2_to_f16x2(b[1] >> 16));
+                mma_16816<M>(more_s[0], a1, e4m3x2_to_f16x2(b[2] & 0xFFFFu), e4m3x2_to_f16x2(b[2] >> 16));
+                mma_16816<M>(more_s[1], a1, e4m3x2_to_f16x2(b[3] & 0xFFFFu), e4m3x2_to_f16x2(b[3] >> 16));
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i], s[1][i] += more_s[1][i];
         }
-        const bool by_row = key0 < all_from || key0 + kTileKeys > all_to;  // rows see different keys of this tile
+        const bool by_row = key0 < all_from || key0 + kWarpKeys > all_to;  // rows see different keys of this tile
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             s[n][0] *= scale0, s[n][1] *= scale0, s[n][2] *= scale1, s[n][3] *= scale1;
@@ -466,14 +591,19 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             l0 += s[n][0] + s[n][1], l1 += s[n][2] + s[n][3];
         }
 
-        // Values that are not finite, in a key that some rows see and others do not: 0 * inf would reach the others. They
-        // are added here to the rows that see them, and are zero in the product below.
-        if (by_row) {
-            uint32_t* words = reinterpret_cast<uint32_t*>(ring + stage * 2 * S::kBytes + S::kBytes);
+        // Values that are not finite, in a key that some rows see and others do not, or that is not there at all: 0 * inf
+        // would reach the result. They are added here to the rows that see them, and are zero in the product below.
+        if (by_row || present != 0xFFFFu) {
+            // This warp's 16 rows, word by word.
+            constexpr int kWords = kWarpKeys * S::kPieces * 4;
+            auto word = [&](int i) {
+                return reinterpret_cast<uint32_t*>(stage_k + S::kBytes + S::at(row_base + i / (S::kPieces * 4), i / 4 % S::kPieces) + i % 4 * 4);
+            };
             bool apart = false;
-            for (int i = lane; i < S::kBytes / 4; i += 32) apart |= not_finite<M, kCodes>(words[i]) != 0;
+            for (int i = lane; i < kWords; i += 32) apart |= not_finite<M, kCodes>(*word(i)) != 0;
             if (__any_sync(0xFFFFFFFFu, apart)) {
-                float (&w)[kRowTile][kTileKeys + 1] = weights_of_tile[warp];
+                float* weights = reinterpret_cast<float*>(smem + Shared::kRing + Shared::kQueries);
+                float(&w)[kRowTile][kWarpKeys + 1] = reinterpret_cast<float(*)[kRowTile][kWarpKeys + 1]>(weights)[warp];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     w[g][8 * n + 2 * t] = s[n][0], w[g][8 * n + 2 * t + 1] = s[n][1];
@@ -481,7 +611,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 }
                 __syncwarp();
 #pragma unroll 1
-                for (int c = 0; c < kTileKeys; ++c) {
+                for (int c = 0; c < kWarpKeys; ++c) {
                     const int key = key0 + c;
                     const bool there = (present >> c) & 1;
                     const bool see0 = there && key >= from0 && key < to0, see1 = there && key >= from1 && key < to1;
@@ -491,7 +621,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const int byte = (kCodes ? (i / 2) * 16 + 4 * t + 2 * e + (i & 1) : 8 * i + 2 * t + e) * kElem;
-                            const uint8_t* at = stage_k + S::kBytes + (c * S::kPieces + S::value_piece(c, byte / 16)) * 16 + byte % 16;
+                            const uint8_t* at = stage_k + S::kBytes + S::at(row_base + c, byte / 16) + byte % 16;
                             float v;
                             if constexpr (kCodes) v = widen2<__half>(e4m3x2_to_f16x2(*at)).x;
                             else v = widen2<M>(*reinterpret_cast<const uint16_t*>(at)).x;
@@ -503,18 +633,19 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                     }
                 }
                 __syncwarp();
-                for (int i = lane; i < S::kBytes / 4; i += 32) words[i] &= ~not_finite<M, kCodes>(words[i]);
+                for (int i = lane; i < kWords; i += 32) *word(i) &= ~not_finite<M, kCodes>(*word(i));
+                fence_proxy_async();  // these writes come before TMA's next ones
                 __syncwarp();
             }
         }
         {
             uint32_t a[4] = {narrow2<M>(s[0][0], s[0][1]), narrow2<M>(s[0][2], s[0][3]), narrow2<M>(s[1][0], s[1][1]),
                              narrow2<M>(s[1][2], s[1][3])};
-            const int r = (lane & 7) + (((lane >> 3) & 1) << 3);
+            const int r = row_base + (lane & 7) + (((lane >> 3) & 1) << 3);
 #pragma unroll
             for (int i = 0; i < S::kPieces / 2; ++i) {
                 uint32_t b[4];
-                ldmatrix_x4_trans(b, stage_v32 + (r * S::kPieces + S::value_piece(r, 2 * i + (lane >> 4))) * 16);
+                ldmatrix_x4_trans(b, stage_v32 + S::at(r, 2 * i + (lane >> 4)));
                 if constexpr (!kCodes) {
                     mma_16816<M>(o[2 * i], a, b[0], b[1]);
                     mma_16816<M>(o[2 * i + 1], a, b[2], b[3]);
@@ -531,11 +662,12 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 }
             }
         }
-        if (++stage == kStages) stage = 0;
-        if (++fill == kStages) fill = 0;
+        __syncwarp();
+        if (leader) mbar_arrive(&empty[stage]);
+        if (++stage == kStages) stage = 0, parity ^= 1;
     }
 
-    // -- the four warps' results, four rows at a time ---------------------------------------------------------------
+    // -- the four warps' results, a few rows at a time ---------------------------------------------------------------
 #pragma unroll
     for (int x = 1; x < 4; x <<= 1) {
         l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, x);
@@ -545,23 +677,22 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         warp_stats[warp][g][0] = m0, warp_stats[warp][g][1] = l0;
         warp_stats[warp][g + 8][0] = m1, warp_stats[warp][g + 8][1] = l1;
     }
-    __syncthreads();
+    consumers_sync();
     {
         float n0 = -INFINITY, n1 = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kAttendWarps; ++w) n0 = fmaxf(n0, warp_stats[w][g][0]), n1 = fmaxf(n1, warp_stats[w][g + 8][0]);
+        for (int w = 0; w < kConsumers; ++w) n0 = fmaxf(n0, warp_stats[w][g][0]), n1 = fmaxf(n1, warp_stats[w][g + 8][0]);
         // A warp that met no visible key has all zeros, or NaN times zero from a score that was NaN: kept as it is.
         const float f0 = m0 == -INFINITY ? 0.f : exp2_approx(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2_approx(m1 - n1);
 #pragma unroll
         for (int i = 0; i < kOut; ++i) o[i][0] *= f0, o[i][1] *= f0, o[i][2] *= f1, o[i][3] *= f1;
     }
     const int rows = min(kRowTile, p.rows - row_tile * kRowTile);
-    const bool whole = item.units == item.s.units;
     const float value_scale = kCodes ? p.a.cache.v_scale[head] : 1.f;
     float* joined = reinterpret_cast<float*>(smem + Shared::kRing);
-    for (int r0 = 0; r0 < rows; r0 += kJoinRows) {
-        if ((g & ~(kJoinRows - 1)) == (r0 & 7)) {
-            float* to = joined + (warp * kJoinRows + (g & (kJoinRows - 1))) * Shared::kPitch;
+    for (int r0 = 0; r0 < rows; r0 += Shared::kJoinRows) {
+        if ((g & ~(Shared::kJoinRows - 1)) == (r0 & 7)) {
+            float* to = joined + (warp * Shared::kJoinRows + (g & (Shared::kJoinRows - 1))) * Shared::kPitch;
 #pragma unroll
             for (int i = 0; i < kOut; ++i) {
                 const float x = r0 < 8 ? o[i][0] : o[i][2], y = r0 < 8 ? o[i][1] : o[i][3];
@@ -573,107 +704,150 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 }
             }
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < min(kJoinRows, rows - r0) * (D / 4); i += kAttendThreads) {
+        consumers_sync();
+        for (int i = threadIdx.x; i < min(Shared::kJoinRows, rows - r0) * (D / 4); i += kConsumers * 32) {
             const int r = r0 + i / (D / 4), d = (i % (D / 4)) * 4;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
             float top = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttendWarps; ++w) {
-                const float4 v = *reinterpret_cast<const float4*>(joined + (w * kJoinRows + (r - r0)) * Shared::kPitch + d);
+            for (int w = 0; w < kConsumers; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(joined + (w * Shared::kJoinRows + (r - r0)) * Shared::kPitch + d);
                 sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
                 top = fmaxf(top, warp_stats[w][r][0]);
             }
 #pragma unroll
-            for (int w = 0; w < kAttendWarps; ++w) {
+            for (int w = 0; w < kConsumers; ++w) {
                 const float m = warp_stats[w][r][0];
                 l += warp_stats[w][r][1] * (m == -INFINITY ? 0.f : exp2_approx(m - top));
             }
-            if (whole) {
+            if (item.whole) {
                 finish_row<T>(p, sequence, head, row_tile * kRowTile + r, d, sum, top, l, value_scale);
-            } else {  // a run has at most two partial results: of an item that began in front of it, and of one that goes on
-                const int piece = (cta * 2 + (item.first == 0)) * p.rows_cap + r;
+            } else {
+                const int piece = item.piece * p.rows_cap + r;
                 *reinterpret_cast<float4*>(p.partial + static_cast<size_t>(piece) * D + d) = sum;
                 if (d == 0) *reinterpret_cast<float2*>(p.stats + piece * 2) = make_float2(top, l);
             }
         }
-        __syncthreads();
+        consumers_sync();
     }
-    unit += item.units;
-    if (unit >= last_unit) break;
-    next_item(item, last_unit - unit);
     }
-    cp_async_wait<0>();
 }
 
-// Joins the partial results of the item that begins in run blockIdx.x and goes on in later ones: for each of its rows,
-// out = sum_c exp2(m_c - m) o_c / sum_c exp2(m_c - m) l_c. D / 4 threads cover a row, the others further partial results.
-// gridDim.y blocks share the rows of an item.
-constexpr int kJoinThreads = 256;
+// Joins the partial results of an item that lies in several runs: item blockIdx.x, or (with more items than runs) the one that
+// begins in run blockIdx.x and goes on. For each of its rows, out = sum_c exp2(m_c - m) o_c / sum_c exp2(m_c - m) l_c. The rows
+// are shared by gridDim.y blocks; in a block D / 4 threads take a row, and those that are left over further partial results
+// of the same rows.
+constexpr int kJoinMostThreads = 1024;
+constexpr int kJoinAhead = 4;  // partial results that a thread has on the way at once
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttendDev p) {
-    constexpr int kAcross = D / 4, kDeep = kJoinThreads / kAcross;
-    __shared__ float4 sums[kDeep][kAcross];
-    __shared__ float ls[kDeep];
-    const int cta = blockIdx.x;
+__global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_constant__ AttendDev p) {
+    constexpr int kAcross = D / 4;
+    __shared__ float4 sums[kJoinMostThreads / kAcross][kAcross];
+    __shared__ float2 stats[kJoinMostThreads / kAcross];
+    const int lines = blockDim.x / kAcross;
     // The lengths are older than the kernel in front, whose blocks waited for them before this one could start.
-    long long unit;
-    Place place;
-    const Line line = lay_out<kJoinThreads>(p, gridDim.x, false, [&](const Line& l) { return l.begin(min(cta, l.ctas - 1) + 1) - 1; },
-                                            &unit, &place);
-    if (cta + 1 >= line.ctas) return;
-    const Sequence s = sequence_of(p, place.sequence, false);
-    const int index = static_cast<int>((unit - place.before) / s.units);
-    const long long begin = place.before + static_cast<long long>(index) * s.units;
+    const Line line(p, false);
+    int sequence, index, run, last;
+    long long begin;
+    if (p.by_item) {
+        sequence = blockIdx.x / p.items, index = blockIdx.x - sequence * p.items;
+        const Sequence s = sequence_of(p, sequence, false);
+        begin = line.in_front_of(p, sequence) + static_cast<long long>(index) * s.units;
+        run = line.run_of(begin), last = line.run_of(begin + s.units - 1);
+    } else {
+        run = blockIdx.x;
+        if (run + 1 >= line.runs) return;
+        const long long unit = line.begin(run + 1) - 1;
+        long long in_front;
+        sequence = line.sequence_at(p, unit, &in_front);
+        const Sequence s = sequence_of(p, sequence, false);
+        index = static_cast<int>(divide(unit - in_front, s.units));
+        begin = in_front + static_cast<long long>(index) * s.units;
+        last = line.run_of(begin + s.units - 1);
+        if (begin < line.begin(run)) return;
+    }
+    if (last == run) return;
     const int head = index / p.row_tiles, first_row = (index - head * p.row_tiles) * kRowTile;
-    const int last = line.owner(begin + s.units - 1);
-    if (begin < line.begin(cta) || last == cta) return;
     pdl_wait();
     pdl_launch_dependents();
-    const int x = threadIdx.x % kAcross, y = threadIdx.x / kAcross;
-    for (int r = blockIdx.y; r < p.rows_cap && first_row + r < p.rows; r += gridDim.y) {
-        auto piece = [&](int c) { return (c * 2 + (c == cta)) * p.rows_cap + r; };
-        float top = -INFINITY;
-        for (int c = cta; c <= last; ++c) top = fmaxf(top, __ldcg(p.stats + piece(c) * 2));
+    const int per_block = (p.rows_cap + gridDim.y - 1) / gridDim.y;
+    const int row_begin = blockIdx.y * per_block, row_end = min(min(row_begin + per_block, p.rows_cap), p.rows - first_row);
+    const int deep = max(1, lines / per_block);  // threads along the partial results of a row
+    const int x = threadIdx.x % kAcross, at = threadIdx.x / kAcross, y = at / per_block;
+    const float value_scale = p.a.cache.type == DLM_E4M3 ? p.a.cache.v_scale[head] : 1.f;
+    for (int r0 = row_begin; r0 < row_end; r0 += deep == 1 ? lines : per_block) {
+        const int r = r0 + (deep == 1 ? at : at % per_block);
+        const bool takes_part = r < row_end && (deep == 1 || y < deep);
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-#pragma unroll 4
-        for (int c = cta + y; c <= last; c += kDeep) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.stats + piece(c) * 2));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial + static_cast<size_t>(piece(c)) * D + x * 4));
-            const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
-            l += ml.y * f;
-            sum.x += v.x * f, sum.y += v.y * f, sum.z += v.z * f, sum.w += v.w * f;
-        }
-        sums[y][x] = sum;
-        if (x == 0) ls[y] = l;
-        __syncthreads();
-        if (y == 0) {
+        float top = -INFINITY, l = 0.f;
+        if (takes_part) {
+            for (int c0 = run + (deep == 1 ? 0 : y); c0 <= last; c0 += deep * kJoinAhead) {
+                float2 ml[kJoinAhead];
+                float4 v[kJoinAhead];
 #pragma unroll
-            for (int i = 1; i < kDeep; ++i) {
-                const float4 v = sums[i][x];
-                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-                l += ls[i];
+                for (int i = 0; i < kJoinAhead; ++i) {
+                    const int c = c0 + i * deep;
+                    ml[i] = make_float2(-INFINITY, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (c <= last) {
+                        const size_t piece = static_cast<size_t>(c * 2 + (c == run)) * p.rows_cap + r;
+                        ml[i] = __ldcg(reinterpret_cast<const float2*>(p.stats + piece * 2));
+                        v[i] = __ldcg(reinterpret_cast<const float4*>(p.partial + piece * D + x * 4));
+                    }
+                }
+                float n = top;
+#pragma unroll
+                for (int i = 0; i < kJoinAhead; ++i) n = fmaxf(n, ml[i].x);
+                const float keep = top == -INFINITY ? 0.f : exp2_approx(top - n);
+                // No visible key so far: zeros, or NaN from a score that was NaN, which stays.
+                sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep, l *= keep;
+                top = n;
+#pragma unroll
+                for (int i = 0; i < kJoinAhead; ++i) {
+                    const float f = ml[i].x == -INFINITY ? 0.f : exp2_approx(ml[i].x - n);
+                    l += ml[i].y * f;
+                    sum.x += v[i].x * f, sum.y += v[i].y * f, sum.z += v[i].z * f, sum.w += v[i].w * f;
+                }
             }
-            finish_row<T>(p, place.sequence, head, first_row + r, x * 4, sum, top, l,
-                          p.a.cache.type == DLM_E4M3 ? p.a.cache.v_scale[head] : 1.f);
         }
-        __syncthreads();
+        if (deep > 1) {  // the same for every thread of the block
+            sums[at][x] = sum;
+            if (x == 0) stats[at] = make_float2(top, l);
+            __syncthreads();
+            if (takes_part && y == 0) {
+                for (int i = 1; i < deep; ++i) top = fmaxf(top, stats[at + i * per_block].x);
+                sum = make_float4(0.f, 0.f, 0.f, 0.f), l = 0.f;
+                for (int i = 0; i < deep; ++i) {
+                    const float2 ml = stats[at + i * per_block];
+                    const float4 v = sums[at + i * per_block][x];
+                    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+                    l += ml.y * f;
+                    sum.x += v.x * f, sum.y += v.y * f, sum.z += v.z * f, sum.w += v.w * f;
+                }
+            }
+            __syncthreads();
+        }
+        if (takes_part && (deep == 1 || y == 0))
+            finish_row<T>(p, sequence, head, first_row + r, x * 4, sum, top, l, value_scale);
     }
 }
 
 template <typename T, int D, bool kCodes>
 static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
     void* args[] = {const_cast<AttendDev*>(&p)};
-    const int rc = launch_kernel<attend_kernel<T, D, kCodes>>(dim3(p.ctas), dim3(kAttendThreads), AttendSmem<D, kCodes>::kBytes,
+    const int rc = launch_kernel<attend_kernel<T, D, kCodes>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes>::kBytes,
                                                               args, o);
     if (rc != 0 || p.partial == nullptr) return rc;
-    // Few items: many partial results each, a block for every row. Many items: one or two each, and a block has to find out
-    // first whether there is anything to join (0.5 us, and 9000 blocks took 25).
-    const bool few = static_cast<long long>(p.a.batch) * p.items * 4 <= p.ctas;
-    return launch_kernel<join_kernel<T, D>>(dim3(p.ctas, few ? p.rows_cap : 1), dim3(kJoinThreads), 0, args,
-                                            {o.stream, true, false});  // always a dependent launch of the kernel above
+    // With fewer items than runs an item may have hundreds of partial results: large blocks, one for each row. Otherwise it has
+    // two or three, and most blocks only find out that there is nothing to join (0.5 us; 9000 blocks took 25).
+    const long long items = static_cast<long long>(p.a.batch) * p.items;
+    const LaunchOpts dependent{o.stream, true, false};  // always a dependent launch of the kernel above
+    if (p.by_item) {
+        const int rows = p.sms * 2 / items < 1 ? 1 : static_cast<int>(p.sms * 2 / items);
+        return launch_kernel<join_kernel<T, D>>(dim3(static_cast<unsigned>(items), rows < p.rows_cap ? rows : p.rows_cap),
+                                                dim3(p.grid >= 16 * items ? kJoinMostThreads : 256), 0, args, dependent);
+    }
+    return launch_kernel<join_kernel<T, D>>(dim3(p.grid), dim3(256), 0, args, dependent);
 }
 
 // Calls f with the type and the sizes of a call as compile-time constants.

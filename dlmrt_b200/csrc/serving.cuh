@@ -21,9 +21,10 @@ __device__ __forceinline__ void report_index(int* status, int row, int kind, int
 }
 
 constexpr int kRowTile = 16;   // rows of an item: the M of its matrix instructions
-constexpr int kUnitKeys = 64;  // keys of the smallest piece of work that items are cut into
+constexpr int kUnitShift = 6, kTileKeys = 1 << kUnitShift;  // keys of a step, and of the units that items are cut into
 
-struct AttendDev {
+struct alignas(64) AttendDev {
+    CUtensorMap tm_k, tm_v;  // (head_dim, page size, heads, pages), boxes of up to 128 bytes x min(page size, kTileKeys) slots
     DlmAttend a;
     float* partial;    // [cta][2][rows_cap][head_dim] unnormalised outputs of items that lie in several CTAs' runs, or null
     float* stats;      // the same without head_dim, 2: running maximum (base 2) and sum
@@ -33,10 +34,31 @@ struct AttendDev {
     int row_tiles;     // of kRowTile rows
     int rows_cap;      // rows of a tile that exist: min(kRowTile, rows)
     int items;         // of one sequence: key heads * row tiles
-    int unit;          // keys of a unit; the table's length where items are not split
+    int unit_shift;    // log2 of the keys of a unit: kUnitKeys, or more than there are where items are not split
     int least_units;   // of a run
-    int ctas;
+    int resident;      // CTAs that the GPU holds
+    int grid;          // runs that there are at most
+    int by_item;       // the join has a block for each item, not for each run
+    int sms;
 };
+
+// How a line of `total` units is cut into runs: `waves` waves of `across` runs each. The first wave takes half of the line, the
+// second a quarter and so on, the last what is left: CTAs take runs in order as they get done, and what they take last is
+// short. A run has at least `least` units (the line's last one excepted), and no wave is shorter than two units a run.
+struct Cut {
+    int across, waves;
+};
+constexpr int kMostWaves = 5;
+
+__host__ __device__ inline Cut attend_cut(long long total, int resident, int least) {
+    Cut c{resident, 1};
+    while (c.waves < kMostWaves && (total >> c.waves) >= 2ll * resident) ++c.waves;
+    if (c.waves == 1) {
+        const long long most = (total + least - 1) / least;
+        if (most < c.across) c.across = most < 1 ? 1 : static_cast<int>(most);
+    }
+    return c;
+}
 
 int launch_append(const DlmAppend& p, int page_shift, const LaunchOpts& o);
 int launch_attend(const AttendDev& p, const LaunchOpts& o);

@@ -60,7 +60,8 @@ class PagedKV:
 
     `keys`, `values`: [pages, kv heads, page size, head dim], BF16 or FP16 (the type of the queries, too) or FP8 E4M3 with
     `k_scale`, `v_scale` [kv heads] FP32: a code counts for code * scale of its head. The head dimension (64, 128 or 256) is
-    contiguous, the other strides are free (multiples of 16 bytes), the page size is a power of two."""
+    contiguous, the other strides are free (multiples of 16 bytes), the page size is a power of two from 8 to
+    4096."""
 
     def __init__(self, keys, values, k_scale=None, v_scale=None):
         if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != values.dtype or keys.device != values.device:
@@ -71,9 +72,9 @@ class PagedKV:
         if keys.stride(3) != 1 or values.stride(3) != 1:
             raise ValueError("keys and values must have a contiguous head dimension")
         pages, heads, page_size, head_dim = keys.shape
-        if head_dim not in (64, 128, 256) or page_size & (page_size - 1) or not 1 <= page_size <= _lib.MAX_PAGE:
+        if head_dim not in (64, 128, 256) or page_size & (page_size - 1) or not _lib.MIN_PAGE <= page_size <= _lib.MAX_PAGE:
             raise ValueError(f"head dimension {head_dim}, page size {page_size}: expected 64, 128 or 256, and a power of two "
-                             f"up to {_lib.MAX_PAGE}")
+                             f"from {_lib.MIN_PAGE} to {_lib.MAX_PAGE}")
         coded = keys.dtype == torch.float8_e4m3fn
         for scale in (k_scale, v_scale):
             if coded != (scale is not None):

@@ -311,6 +311,7 @@ DLM_API int dlm_all_gather_loopback(const void* const* x, int64_t bytes, const D
  * were not there, and leaves DLM_ERR_INDEX in the status words (block = which row or sequence, slot = which index). */
 enum { DLM_BF16 = 0, DLM_F16 = 1, DLM_E4M3 = 2 };
 
+#define DLM_MIN_PAGE 8
 #define DLM_MAX_PAGE 4096
 
 /* One layer's pool of pages. Element strides; the head dimension is contiguous. */
@@ -320,9 +321,9 @@ typedef struct DlmPages {
     const float* k_scale;      /* [heads] what a key code counts for (DLM_E4M3: required; otherwise NULL) */
     const float* v_scale;      /* [heads] the same for values */
     int32_t* status;           /* [DLM_STATUS_WORDS] as DlmComm.status, or NULL */
-    int64_t k_strides[3];      /* page, head, slot; multiples of 16 bytes */
+    int64_t k_strides[3];      /* page, head, slot; positive multiples of 16 bytes */
     int64_t v_strides[3];
-    int32_t pages, page_size;  /* page_size a power of two, at most DLM_MAX_PAGE */
+    int32_t pages, page_size;  /* page_size a power of two, DLM_MIN_PAGE to DLM_MAX_PAGE */
     int32_t heads, head_dim;   /* head_dim 64, 128 or 256 */
     int32_t type;              /* DLM_BF16, DLM_F16 or DLM_E4M3 */
     int32_t reserved;

@@ -35,7 +35,7 @@ CASES = [
     (1, 4, 1, 64, 16, 3, BF16, BF16, 64, False, True, "hnd"),
     (7, 8, 2, 128, 16, 4, BF16, BF16, 128, False, True, "nhd"),
     (33, 3, 3, 256, 8, 9, F16, F16, 128, True, False, "hnd"),
-    (130, 6, 2, 128, 1, 140, BF16, E4M3, 64, False, True, "hnd"),
+    (130, 6, 2, 128, 8, 18, BF16, E4M3, 64, False, True, "hnd"),
     (65, 2, 1, 64, 64, 4, F16, E4M3, 48, True, True, "nhd"),
     (40, 5, 5, 256, 32, 4, BF16, E4M3, 256, False, False, "hnd"),
     (9, 4, 2, 128, 16, 2, F16, F16, 0, False, True, "hnd"),

@@ -46,7 +46,41 @@ def test_single_tokens_of_ragged_lengths(d, dtype, cache):
     check(*args)
 
 
-@pytest.mark.parametrize("page", [1, 2, 8, 32, 128, 256])
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_sequences_that_are_split(d, dtype, cache):
+    """More than 512 keys: work is cut into units of 64 keys, over as many CTAs as the GPU holds; items begin and end in the
+    middle of a CTA's share, empty ones and ones of a single key among them."""
+    args = setup([700, 0, 1, 1500, 64, 129, 0, 2000], 1, 8, 2, d, 16, dtype, E4M3 if cache == "e4m3" else dtype)
+    check(*args)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("window", [0, 500, 700])
+@pytest.mark.parametrize("t, hq, hk", [(1, 40, 2), (7, 4, 2), (19, 4, 1)])
+def test_split_sequences_with_masks_and_several_row_tiles(t, hq, hk, window, causal):
+    check(*setup([1100, 19, 640, 1], t, hq, hk, 64, 32, BF16, BF16), window=window, causal=causal)
+
+
+def test_many_sequences():
+    """More items than CTAs, and more sequences than a CTA has threads."""
+    lengths = [(i * 37) % 90 for i in range(700)]
+    check(*setup(lengths, 1, 2, 1, 64, 16, BF16, BF16))
+    lengths[350] = 3000
+    check(*setup(lengths, 1, 2, 1, 64, 16, BF16, BF16))
+
+
+def test_units_outnumber_what_fits():
+    """One long sequence over every CTA, and a table much wider than any sequence needs."""
+    kv, q, table, lengths = setup([9000], 1, 4, 2, 128, 64, BF16, BF16)
+    check(kv, q, table, lengths)
+    wide = torch.full((1, 100000), -1, device="cuda", dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    check(kv, q, wide, lengths)
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 128, 256])
 @pytest.mark.parametrize("layout", ["hnd", "nhd"])
 def test_page_sizes_and_layouts(page, layout):
     check(*setup([5, 130, 257], 1, 4, 2, 64, page, BF16, BF16, layout=layout))

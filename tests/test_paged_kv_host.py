@@ -29,7 +29,7 @@ def pages(**kw):
 PAGES = [
     (dict(keys=None), _lib.ERR_NULL), (dict(values=None), _lib.ERR_NULL), (dict(type=3), _lib.ERR_SHAPE),
     (dict(type=_lib.E4M3), _lib.ERR_NULL), (dict(head_dim=96), _lib.ERR_SHAPE), (dict(page_size=24), _lib.ERR_SHAPE),
-    (dict(page_size=8192), _lib.ERR_SHAPE), (dict(page_size=0), _lib.ERR_SHAPE), (dict(pages=0), _lib.ERR_SHAPE),
+    (dict(page_size=8192), _lib.ERR_SHAPE), (dict(page_size=0), _lib.ERR_SHAPE), (dict(page_size=4), _lib.ERR_SHAPE), (dict(pages=0), _lib.ERR_SHAPE),
     (dict(heads=0), _lib.ERR_SHAPE), (dict(k_strides=(2048, 1024, 68)), _lib.ERR_ALIGN), (dict(v_strides=(-8, 8, 8)), _lib.ERR_ALIGN),
     (dict(keys=0x1008), _lib.ERR_ALIGN),
     (dict(type=_lib.E4M3, k_scale=0x10, v_scale=0x10, k_strides=(2048, 1024, 72)), _lib.ERR_ALIGN),
@@ -89,7 +89,7 @@ def test_append_refuses(kw, code):
     (dict(tokens=0), _lib.ERR_SHAPE), (dict(batch=-1), _lib.ERR_SHAPE), (dict(batch=65536), _lib.ERR_SHAPE),
     (dict(table_pages=1 << 27), _lib.ERR_SHAPE), (dict(window=-1), _lib.ERR_SHAPE), (dict(causal=2), _lib.ERR_SHAPE),
     (dict(type=_lib.F16), _lib.ERR_SHAPE), (dict(q=0x3004), _lib.ERR_ALIGN), (dict(q_strides=(256, 256, 68)), _lib.ERR_ALIGN),
-    (dict(out_strides=(256, -8, 64)), _lib.ERR_ALIGN), (dict(batch=0, q=None), _lib.OK),
+    (dict(out_strides=(256, 256, -64)), _lib.ERR_ALIGN), (dict(q_strides=(-3, 256, 64)), _lib.ERR_ALIGN), (dict(batch=0, q=None), _lib.OK),
 ])
 def test_attend_refuses(kw, code):
     assert _lib.lib().dlm_paged_attend(attend(**kw), None) == code
