@@ -806,7 +806,7 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
 
 // Everything about an attention call that its device pointers do not decide.
 static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
-    constexpr int kWholeKeys = 512, kLeastUnits = 2;
+    constexpr int kWholeKeys = 512;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
@@ -826,29 +826,34 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
         span = static_cast<long long>(a->window) + a->tokens + kTileKeys;
     const bool whole = span <= kWholeKeys;
     d->unit_shift = whole ? 31 : kUnitShift;
-    d->least_units = whole ? 1 : kLeastUnits;
+    d->least_shift = whole ? 0 : 1;
     d->sms = sms;
     d->resident = sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
     const long long units = whole ? 1 : (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
-    const Cut cut = attend_cut(units * a->batch * d->items, d->resident, d->least_units);
+    if (units * a->batch * d->items > INT32_MAX) return DLM_ERR_SHAPE;
+    const Cut cut = attend_cut(static_cast<uint32_t>(units * a->batch * d->items), d->resident, d->least_shift);
     d->grid = cut.across * cut.waves;
     d->by_item = static_cast<long long>(a->batch) * d->items < d->grid;
     return DLM_OK;
 }
 
-// The pool as TMA reads it for the attention kernel: boxes of up to 128 bytes x up to kTileKeys slots of one head and page.
+// The pool as TMA reads it for the attention kernel: whole slots of one head and page, up to kTileKeys at once, in column
+// blocks of 128 bytes (the width of the swizzle) or of a head's 64.
 static int make_map_pages(CUtensorMap* map, const void* base, const DlmPages& c, const int64_t* strides) {
     EncodeTiled fn = encode_tiled();
     if (fn == nullptr) return DLM_ERR_CUDA;
-    const int size = c.type == DLM_E4M3 ? 1 : 2, row_bytes = c.head_dim * size;
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
-                                static_cast<cuuint64_t>(c.heads), static_cast<cuuint64_t>(c.pages)};
+    const int size = c.type == DLM_E4M3 ? 1 : 2, row_bytes = c.head_dim * size, block_bytes = row_bytes < 128 ? row_bytes : 128;
+    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(block_bytes / size), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(row_bytes / block_bytes), static_cast<cuuint64_t>(c.heads),
+                                static_cast<cuuint64_t>(c.pages)};
     auto bytes = [&](int64_t stride, int extent) { return static_cast<cuuint64_t>(extent > 1 ? stride * size : row_bytes); };
-    const cuuint64_t steps[3] = {bytes(strides[2], c.page_size), bytes(strides[1], c.heads), bytes(strides[0], c.pages)};
-    const cuuint32_t box[4] = {static_cast<cuuint32_t>(row_bytes < 128 ? c.head_dim : 128 / size),
-                               static_cast<cuuint32_t>(c.page_size < kTileKeys ? c.page_size : kTileKeys), 1, 1};
-    const cuuint32_t elem[4] = {1, 1, 1, 1};
-    const CUresult r = fn(map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base),
+    const cuuint64_t steps[4] = {bytes(strides[2], c.page_size), static_cast<cuuint64_t>(block_bytes), bytes(strides[1], c.heads),
+                                 bytes(strides[0], c.pages)};
+    const cuuint32_t box[5] = {static_cast<cuuint32_t>(block_bytes / size),
+                               static_cast<cuuint32_t>(c.page_size < kTileKeys ? c.page_size : kTileKeys),
+                               static_cast<cuuint32_t>(row_bytes / block_bytes), 1, 1};
+    const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, const_cast<void*>(base),
                           dims, steps, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           row_bytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -59,24 +59,22 @@ __device__ __forceinline__ int seen_to(const AttendDev& p, int first_pos, int le
     return p.a.causal ? min(length, first_pos + token + 1) : length;
 }
 
-// a / b of what is nearly always below 2^32: a 64-bit division takes a hundred instructions.
-__device__ __forceinline__ long long divide(long long a, long long b) {
-    return ((a | b) >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
-}
+// The token that a row (query head of the group, token) belongs to.
+__device__ __forceinline__ int token_of(const AttendDev& p, int row) { return p.a.tokens == 1 ? 0 : row / p.group; }
 
 // The line of units and its runs (see attend_cut). Every warp that needs it works it out for itself: a lane looks at a range
-// of the sequences.
+// of the sequences. The host has seen to it that there are fewer than 2^31 units.
 struct Line {
-    long long total;
+    uint32_t total;
     Cut cut;
     int runs;
     int first, last;    // this lane's sequences
-    long long before;   // units in front of them
-    long long mine;     // units of them
+    uint32_t before;    // units in front of them
+    uint32_t mine;      // units of them
 
     __device__ __forceinline__ Line(const AttendDev& p, bool tell) {
         const int lane = threadIdx.x & 31;
-        const int per = (p.a.batch + 31) / 32;
+        const int per = (p.a.batch + 31) >> 5;
         first = min(lane * per, p.a.batch), last = min(first + per, p.a.batch);
         mine = 0;
         for (int i = first; i < last; ++i) mine += sequence_of(p, i, tell).units;
@@ -84,41 +82,44 @@ struct Line {
         before = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xFFFFFFFFu, before, o);
+            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, before, o);
             if (lane >= o) before += up;
         }
         total = __shfl_sync(0xFFFFFFFFu, before, 31);
         before -= mine;
-        cut = attend_cut(total, p.resident, p.least_units);
+        cut = attend_cut(total, p.resident, p.least_shift);
         runs = cut.across * cut.waves;
     }
-    __device__ __forceinline__ long long wave_begin(int wave) const { return wave < cut.waves ? total - (total >> wave) : total; }
-    __device__ __forceinline__ long long begin(int run) const {  // rounded down: no run of a wave is empty
-        const int wave = run / cut.across, i = run - wave * cut.across;
-        const long long from = wave_begin(wave);
-        return from + (i == 0 ? 0 : divide((wave_begin(wave + 1) - from) * i, cut.across));
+    __device__ __forceinline__ uint32_t wave_begin(int wave) const { return wave < cut.waves ? total - (total >> wave) : total; }
+    // The units [begin, end) of a run: a wave's are dealt out evenly, rounded down, and no run is empty.
+    __device__ __forceinline__ void range(int run, uint32_t* begin, uint32_t* end) const {
+        const uint32_t across = cut.across, wave = static_cast<uint32_t>(run) / across, i = run - wave * across;
+        const uint32_t from = wave_begin(wave), units = wave_begin(wave + 1) - from, each = units / across, over = units - each * across;
+        *begin = from + each * i + over * i / across;
+        *end = from + each * (i + 1) + over * (i + 1) / across;
     }
-    __device__ __forceinline__ int run_of(long long unit) const {
+    __device__ __forceinline__ int run_of(uint32_t unit) const {
         int wave = 0;
         while (wave + 1 < cut.waves && unit >= wave_begin(wave + 1)) ++wave;
-        const long long from = wave_begin(wave);
-        return wave * cut.across + static_cast<int>(divide((unit - from + 1) * cut.across - 1, wave_begin(wave + 1) - from));
+        const uint32_t from = wave_begin(wave);
+        return wave * cut.across +
+               static_cast<int>((static_cast<unsigned long long>(unit - from + 1) * cut.across - 1) / (wave_begin(wave + 1) - from));
     }
     // The units in front of a sequence. All lanes of the warp.
-    __device__ __forceinline__ long long in_front_of(const AttendDev& p, int sequence) const {
-        const int per = (p.a.batch + 31) / 32, holder = sequence / per;
-        long long front = __shfl_sync(0xFFFFFFFFu, before, holder);
-        for (int i = holder * per; i < sequence; ++i) front += static_cast<long long>(sequence_of(p, i, false).units) * p.items;
+    __device__ __forceinline__ uint32_t in_front_of(const AttendDev& p, int sequence) const {
+        const int per = (p.a.batch + 31) >> 5, holder = sequence / per;
+        uint32_t front = __shfl_sync(0xFFFFFFFFu, before, holder);
+        for (int i = holder * per; i < sequence; ++i) front += static_cast<uint32_t>(sequence_of(p, i, false).units) * p.items;
         return front;
     }
     // The sequence that holds a unit, and the units in front of that sequence. All lanes of the warp.
-    __device__ __forceinline__ int sequence_at(const AttendDev& p, long long unit, long long* in_front) const {
+    __device__ __forceinline__ int sequence_at(const AttendDev& p, uint32_t unit, uint32_t* in_front) const {
         int sequence = first;
-        long long front = before;
+        uint32_t front = before;
         const bool here = unit >= before && unit < before + mine;
         if (here) {
             for (; sequence < last - 1; ++sequence) {
-                const long long units = static_cast<long long>(sequence_of(p, sequence, false).units) * p.items;
+                const uint32_t units = static_cast<uint32_t>(sequence_of(p, sequence, false).units) * p.items;
                 if (unit < front + units) break;
                 front += units;
             }
@@ -130,18 +131,24 @@ struct Line {
     }
 };
 
-// A stage: 64 keys, then 64 values, as TMA writes them: column blocks of up to 128 bytes, in each the rows one after the
-// other with their 16-byte pieces permuted by row (the 128- or 64-byte swizzle), so that ldmatrix meets each bank once.
+// A stage: 64 keys, then 64 values, as TMA writes them: box by box (a page's slots, at most 64), in a box column blocks of up
+// to 128 bytes, in each the rows one after the other with their 16-byte pieces permuted by row (the 128- or 64-byte swizzle),
+// so that ldmatrix meets each bank once.
 template <int D, bool kCodes>
 struct Stage {
     static constexpr int kPieces = D * (kCodes ? 1 : 2) / 16;           // 16-byte pieces of a row
     static constexpr int kBytes = kTileKeys * kPieces * 16;              // of the keys, or of the values
     static constexpr int kAcross = kPieces < 8 ? kPieces : 8;            // pieces of a column block's row
-    static constexpr int kBlocks = kPieces / kAcross;
-    static constexpr int kBlockBytes = kTileKeys * kAcross * 16;
-    __device__ static __forceinline__ int at(int row, int piece) {
+    int first;   // offset of a warp's first row
+    int half;    // from its row r to row r + 8: in the same box, or (pages of 8) in the next
+    int block;   // from a column block to the next
+    __device__ __forceinline__ Stage(int box_keys, int row)
+        : first(row / box_keys * box_keys * kPieces * 16 + row % box_keys * kAcross * 16),
+          half(box_keys == 8 ? 8 * kPieces * 16 : 8 * kAcross * 16), block(box_keys * kAcross * 16) {}
+    // Offset of a piece of the warp's row `row`, 0 to 15.
+    __device__ __forceinline__ int at(int row, int piece) const {
         const int turn = kAcross == 8 ? row & 7 : (row >> 1) & 3;
-        return (piece / kAcross) * kBlockBytes + row * (kAcross * 16) + ((piece % kAcross) ^ turn) * 16;
+        return first + (piece / kAcross) * block + (row >> 3) * half + (row & 7) * (kAcross * 16) + ((piece % kAcross) ^ turn) * 16;
     }
 };
 
@@ -228,7 +235,7 @@ template <typename T>
 __device__ __forceinline__ void finish_row(const AttendDev& p, int sequence, int head, int row, int d, const float4& sum,
                                            float top, float l, float value_scale) {
     const float inv = l == 0.f ? 0.f : value_scale / l;
-    const int token = row / p.group, query_head = head * p.group + row - token * p.group;
+    const int token = token_of(p, row), query_head = head * p.group + row - token * p.group;
     T* out = static_cast<T*>(p.a.out) + sequence * p.a.out_strides[0] + token * p.a.out_strides[1] +
              query_head * p.a.out_strides[2] + d;
     *reinterpret_cast<uint2*>(out) = make_uint2(narrow2<T>(sum.x * inv, sum.y * inv), narrow2<T>(sum.z * inv, sum.w * inv));
@@ -293,7 +300,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         };
         // Where the next step is: a run, an item in it, a step of 64 keys in that. Its pages are looked up a step ahead of its
         // use, across items and runs: lane j asks for the page of box j.
-        long long unit = 0, last_unit = 0;
+        uint32_t unit = 0, last_unit = 0;
         int sequence = 0, index = 0, first = 0, units = 0, lo = 0, tile = 0, page = INT_MIN;
         Sequence s{};
         Work work{};
@@ -302,12 +309,12 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             page = lane < boxes && key < work.end ? p.a.page_table[sequence * p.a.table_stride + (key >> p.page_shift)] : INT_MIN;
         };
         auto begin_item = [&]() {
-            units = static_cast<int>(last_unit - unit < s.units - first ? last_unit - unit : s.units - first);
+            units = min(static_cast<int>(last_unit - unit), s.units - first);
             work.sequence = sequence, work.length = s.length, work.first_pos = s.first_pos;
-            work.head = index / p.row_tiles, work.row_tile = index - work.head * p.row_tiles;
+            work.head = p.row_tiles == 1 ? index : index / p.row_tiles, work.row_tile = index - work.head * p.row_tiles;
             const int first_row = work.row_tile * kRowTile, last_row = min(first_row + kRowTile, p.rows) - 1;
-            lo = seen_from(p, s.first_pos, first_row / p.group);
-            const int hi = seen_to(p, s.first_pos, s.length, last_row / p.group);
+            lo = seen_from(p, s.first_pos, token_of(p, first_row));
+            const int hi = seen_to(p, s.first_pos, s.length, token_of(p, last_row));
             work.whole = units == s.units;
             work.piece = run * 2 + (first == 0);  // a run has at most one that began before it and one that goes on
             work.start = max(s.base + (first << p.unit_shift), lo & ~(kTileKeys - 1));  // first is 0 if units are whole items
@@ -323,12 +330,12 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 mbar_expect_tx(&answered, sizeof(answer));
                 ask_for_cta(&answer, &answered);
             }
-            unit = line.begin(run), last_unit = line.begin(run + 1);
-            long long in_front;
+            line.range(run, &unit, &last_unit);
+            uint32_t in_front;
             sequence = line.sequence_at(p, unit, &in_front);
             s = sequence_of(p, sequence, false);
-            index = static_cast<int>(divide(unit - in_front, s.units));  // key head * row tiles + row tile
-            first = static_cast<int>(unit - in_front - static_cast<long long>(index) * s.units);
+            index = static_cast<int>((unit - in_front) / static_cast<uint32_t>(s.units));  // key head * row tiles + row tile
+            first = static_cast<int>(unit - in_front) - index * s.units;
             begin_item();
             return true;
         };
@@ -362,37 +369,37 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             if (now_tile == 0) announce(now);
             if (now.tiles == 0) continue;
             const int key0 = now.start + now_tile * kTileKeys;
-            const bool in_pool = now_page >= 0 && now_page < p.a.cache.pages;
-            if (!in_pool && now_page != INT_MIN && key0 + (lane + 1) * box_keys > now_lo)
-                report_index(p.a.cache.status, now.sequence, kIndexPage, now_page);
-            const uint32_t there = __ballot_sync(0xFFFFFFFFu, in_pool);
-            if (!in_pool) now_page = p.a.cache.pages;  // past the pool's end: the box is filled with zeros
-            if (!mbar_wait_warp(&empty[stage], parity, deadline) && !failed) {
-                failed = true;
-                if (leader) stalled(1, now_tile);
-            }
-            uint8_t* to = smem + stage * 2 * S::kBytes;
-            uint64_t* bar = &full[stage];
-            if (leader) {
-                uint64_t present = 0;
+            const bool in_pool = static_cast<uint32_t>(now_page) < static_cast<uint32_t>(p.a.cache.pages);
+            uint64_t present = ~0ull;
+            if (!__all_sync(0xFFFFFFFFu, in_pool || lane >= boxes) || now.end - key0 < kTileKeys) {
+                if (!in_pool && now_page != INT_MIN && key0 + (lane + 1) * box_keys > now_lo)
+                    report_index(p.a.cache.status, now.sequence, kIndexPage, now_page);
+                const uint32_t there = __ballot_sync(0xFFFFFFFFu, in_pool);
+                if (!in_pool) now_page = p.a.cache.pages;  // past the pool's end: the box is filled with zeros
                 const uint64_t box_bits = box_keys == 64 ? ~0ull : (1ull << box_keys) - 1;
+                present = 0;
                 for (int j = 0; j < boxes; ++j)
                     if (there >> j & 1) present |= box_bits << (j * box_keys);
                 if (now.end - key0 < kTileKeys) present &= (1ull << (now.end - key0)) - 1;
+            }
+            if (!mbar_wait(&empty[stage], parity, deadline) && !failed) {
+                failed = true;
+                if (leader) stalled(1, now_tile);
+            }
+            __syncwarp();
+            uint8_t* to = smem + stage * 2 * S::kBytes;
+            uint64_t* bar = &full[stage];
+            if (leader) {
                 present_keys[stage] = present;
                 if (failed) mbar_arrive(bar);
                 else mbar_expect_tx(bar, 2 * S::kBytes);
             }
             for (int j = 0; j < boxes; ++j) {
                 const int from = __shfl_sync(0xFFFFFFFFu, now_page, j);
-                const int at = (key0 + j * box_keys) & slot_mask, row = j * box_keys * S::kAcross * 16;
+                const int at = (key0 + j * box_keys) & slot_mask, box = j * box_keys * S::kPieces * 16;
                 if (leader && !failed) {
-#pragma unroll
-                    for (int c = 0; c < S::kBlocks; ++c) {
-                        tma_load_4d(to + c * S::kBlockBytes + row, &p.tm_k, bar, c * (128 / kElem), at, now.head, from, kEvictNormal);
-                        tma_load_4d(to + S::kBytes + c * S::kBlockBytes + row, &p.tm_v, bar, c * (128 / kElem), at, now.head, from,
-                                    kEvictNormal);
-                    }
+                    tma_load_5d(to + box, &p.tm_k, bar, 0, at, 0, now.head, from, kEvictNormal);
+                    tma_load_5d(to + S::kBytes + box, &p.tm_v, bar, 0, at, 0, now.head, from, kEvictNormal);
                 }
             }
             if (++stage == kStages) stage = 0, parity ^= 1;
@@ -405,6 +412,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
 
     // -- the consumers --------------------------------------------------------------------------------------------------
     const int g = lane >> 2, t = lane & 3;
+    const S rows_of_stage(min(kTileKeys, 1 << p.page_shift), warp * kWarpKeys);
     int stage = 0, slot = 0;
     uint32_t parity = 0, slot_parity = 0;
     while (true) {
@@ -419,15 +427,15 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     const int sequence = item.sequence, head = item.head, row_tile = item.row_tile;
     // This thread's two rows: g and g + 8 of the tile.
     const int row0 = row_tile * kRowTile + g, row1 = row0 + 8;
-    const int token0 = min(row0, p.rows - 1) / p.group, token1 = min(row1, p.rows - 1) / p.group;
+    const int token0 = token_of(p, min(row0, p.rows - 1)), token1 = token_of(p, min(row1, p.rows - 1));
     const int from0 = seen_from(p, item.first_pos, token0), to0 = seen_to(p, item.first_pos, item.length, token0);
     const int from1 = seen_from(p, item.first_pos, token1), to1 = seen_to(p, item.first_pos, item.length, token1);
     const int last_row = min(row_tile * kRowTile + kRowTile, p.rows) - 1;
-    const int all_from = seen_from(p, item.first_pos, last_row / p.group);                          // from here on every row sees
-    const int all_to = seen_to(p, item.first_pos, item.length, (row_tile * kRowTile) / p.group);    // the keys, up to here
+    const int all_from = seen_from(p, item.first_pos, token_of(p, last_row));                          // from here on every row sees
+    const int all_to = seen_to(p, item.first_pos, item.length, token_of(p, row_tile * kRowTile));    // the keys, up to here
 
     auto q_row = [&](int row) -> const T* {
-        const int token = row / p.group, of = row - token * p.group;
+        const int token = token_of(p, row), of = row - token * p.group;
         return static_cast<const T*>(p.a.q) + sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
                static_cast<long long>(head * p.group + of) * p.a.q_strides[2];
     };
@@ -507,7 +515,6 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         uint8_t* stage_k = smem + stage * 2 * S::kBytes;
         const uint32_t stage_k32 = smem_u32(stage_k), stage_v32 = stage_k32 + S::kBytes;
         const uint32_t present = static_cast<uint32_t>(present_keys[stage] >> (warp * kWarpKeys)) & 0xFFFFu;
-        const int row_base = warp * kWarpKeys;
 
         auto query_step = [&](int k, uint32_t (&a)[4]) {
             if constexpr (Shared::kQueriesInShared) {
@@ -521,13 +528,13 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         // scores: columns are keys, 0..7 in s[0], 8..15 in s[1]
         float s[2][4] = {};
         if constexpr (!kCodes) {
-            const int r = row_base + (lane & 7) + ((lane >> 4) << 3);
+            const int r = (lane & 7) + ((lane >> 4) << 3);
             float more_s[2][4] = {};  // odd steps: half as long a chain of dependent products
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 uint32_t a[4], b[4];
                 query_step(k, a);
-                ldmatrix_x4(b, stage_k32 + S::at(r, 2 * k + ((lane >> 3) & 1)));
+                ldmatrix_x4(b, stage_k32 + rows_of_stage.at(r, 2 * k + ((lane >> 3) & 1)));
                 mma_16816<M>(k & 1 ? more_s[0] : s[0], a, b[0], b[1]);
                 mma_16816<M>(k & 1 ? more_s[1] : s[1], a, b[2], b[3]);
             }
@@ -535,14 +542,14 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i], s[1][i] += more_s[1][i];
         } else {
             // A 16-byte piece of a key row is one k16 step: lane t of a row holds its elements 4t .. 4t + 3.
-            const int r = row_base + (lane & 7) + (((lane >> 3) & 1) << 3);
+            const int r = (lane & 7) + (((lane >> 3) & 1) << 3);
             float more_s[2][4] = {};
 #pragma unroll
             for (int k = 0; k < kSteps; k += 2) {
                 uint32_t a0[4], a1[4], b[4];
                 query_step(k, a0);
                 query_step(k + 1, a1);
-                ldmatrix_x4(b, stage_k32 + S::at(r, k + (lane >> 4)));
+                ldmatrix_x4(b, stage_k32 + rows_of_stage.at(r, k + (lane >> 4)));
                 mma_16816<M>(s[0], a0, e4m3x2_to_f16x2(b[0] & 0xFFFFu), e4m3x2_to_f16x2(b[0] >> 16));
                 mma_16816<M>(s[1], a0, e4m3x2_to_f16x2(b[1] & 0xFFFFu), e4m3x2_to_f16x2(b[1] >> 16));
                 mma_16816<M>(more_s[0], a1, e4m3x2_to_f16x2(b[2] & 0xFFFFu), e4m3x2_to_f16x2(b[2] >> 16));
@@ -597,7 +604,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             // This warp's 16 rows, word by word.
             constexpr int kWords = kWarpKeys * S::kPieces * 4;
             auto word = [&](int i) {
-                return reinterpret_cast<uint32_t*>(stage_k + S::kBytes + S::at(row_base + i / (S::kPieces * 4), i / 4 % S::kPieces) + i % 4 * 4);
+                return reinterpret_cast<uint32_t*>(stage_k + S::kBytes + rows_of_stage.at(i / (S::kPieces * 4), i / 4 % S::kPieces) + i % 4 * 4);
             };
             bool apart = false;
             for (int i = lane; i < kWords; i += 32) apart |= not_finite<M, kCodes>(*word(i)) != 0;
@@ -621,7 +628,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const int byte = (kCodes ? (i / 2) * 16 + 4 * t + 2 * e + (i & 1) : 8 * i + 2 * t + e) * kElem;
-                            const uint8_t* at = stage_k + S::kBytes + S::at(row_base + c, byte / 16) + byte % 16;
+                            const uint8_t* at = stage_k + S::kBytes + rows_of_stage.at(c, byte / 16) + byte % 16;
                             float v;
                             if constexpr (kCodes) v = widen2<__half>(e4m3x2_to_f16x2(*at)).x;
                             else v = widen2<M>(*reinterpret_cast<const uint16_t*>(at)).x;
@@ -641,11 +648,11 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         {
             uint32_t a[4] = {narrow2<M>(s[0][0], s[0][1]), narrow2<M>(s[0][2], s[0][3]), narrow2<M>(s[1][0], s[1][1]),
                              narrow2<M>(s[1][2], s[1][3])};
-            const int r = row_base + (lane & 7) + (((lane >> 3) & 1) << 3);
+            const int r = (lane & 7) + (((lane >> 3) & 1) << 3);
 #pragma unroll
             for (int i = 0; i < S::kPieces / 2; ++i) {
                 uint32_t b[4];
-                ldmatrix_x4_trans(b, stage_v32 + S::at(r, 2 * i + (lane >> 4)));
+                ldmatrix_x4_trans(b, stage_v32 + rows_of_stage.at(r, 2 * i + (lane >> 4)));
                 if constexpr (!kCodes) {
                     mma_16816<M>(o[2 * i], a, b[0], b[1]);
                     mma_16816<M>(o[2 * i + 1], a, b[2], b[3]);
@@ -749,23 +756,23 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
     // The lengths are older than the kernel in front, whose blocks waited for them before this one could start.
     const Line line(p, false);
     int sequence, index, run, last;
-    long long begin;
+    uint32_t begin, run_begin, run_end;
     if (p.by_item) {
         sequence = blockIdx.x / p.items, index = blockIdx.x - sequence * p.items;
         const Sequence s = sequence_of(p, sequence, false);
-        begin = line.in_front_of(p, sequence) + static_cast<long long>(index) * s.units;
+        begin = line.in_front_of(p, sequence) + index * s.units;
         run = line.run_of(begin), last = line.run_of(begin + s.units - 1);
     } else {
         run = blockIdx.x;
         if (run + 1 >= line.runs) return;
-        const long long unit = line.begin(run + 1) - 1;
-        long long in_front;
-        sequence = line.sequence_at(p, unit, &in_front);
+        line.range(run, &run_begin, &run_end);
+        uint32_t in_front;
+        sequence = line.sequence_at(p, run_end - 1, &in_front);
         const Sequence s = sequence_of(p, sequence, false);
-        index = static_cast<int>(divide(unit - in_front, s.units));
-        begin = in_front + static_cast<long long>(index) * s.units;
+        index = static_cast<int>((run_end - 1 - in_front) / static_cast<uint32_t>(s.units));
+        begin = in_front + index * s.units;
         last = line.run_of(begin + s.units - 1);
-        if (begin < line.begin(run)) return;
+        if (begin < run_begin) return;
     }
     if (last == run) return;
     const int head = index / p.row_tiles, first_row = (index - head * p.row_tiles) * kRowTile;

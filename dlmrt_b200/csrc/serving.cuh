@@ -24,7 +24,7 @@ constexpr int kRowTile = 16;   // rows of an item: the M of its matrix instructi
 constexpr int kUnitShift = 6, kTileKeys = 1 << kUnitShift;  // keys of a step, and of the units that items are cut into
 
 struct alignas(64) AttendDev {
-    CUtensorMap tm_k, tm_v;  // (head_dim, page size, heads, pages), boxes of up to 128 bytes x min(page size, kTileKeys) slots
+    CUtensorMap tm_k, tm_v;  // (128 bytes, page size, column blocks, heads, pages); a box: min(page size, kTileKeys) whole slots
     DlmAttend a;
     float* partial;    // [cta][2][rows_cap][head_dim] unnormalised outputs of items that lie in several CTAs' runs, or null
     float* stats;      // the same without head_dim, 2: running maximum (base 2) and sum
@@ -35,7 +35,7 @@ struct alignas(64) AttendDev {
     int rows_cap;      // rows of a tile that exist: min(kRowTile, rows)
     int items;         // of one sequence: key heads * row tiles
     int unit_shift;    // log2 of the keys of a unit: kUnitKeys, or more than there are where items are not split
-    int least_units;   // of a run
+    int least_shift;   // log2 of the units of a run of a short line
     int resident;      // CTAs that the GPU holds
     int grid;          // runs that there are at most
     int by_item;       // the join has a block for each item, not for each run
@@ -44,19 +44,17 @@ struct alignas(64) AttendDev {
 
 // How a line of `total` units is cut into runs: `waves` waves of `across` runs each. The first wave takes half of the line, the
 // second a quarter and so on, the last what is left: CTAs take runs in order as they get done, and what they take last is
-// short. A run has at least `least` units (the line's last one excepted), and no wave is shorter than two units a run.
+// short. No wave is shorter than two units a run; a line of less than that has runs of about 2^least_shift units.
 struct Cut {
     int across, waves;
 };
 constexpr int kMostWaves = 5;
 
-__host__ __device__ inline Cut attend_cut(long long total, int resident, int least) {
+__host__ __device__ inline Cut attend_cut(uint32_t total, int resident, int least_shift) {
     Cut c{resident, 1};
-    while (c.waves < kMostWaves && (total >> c.waves) >= 2ll * resident) ++c.waves;
-    if (c.waves == 1) {
-        const long long most = (total + least - 1) / least;
-        if (most < c.across) c.across = most < 1 ? 1 : static_cast<int>(most);
-    }
+    while (c.waves < kMostWaves && (total >> c.waves) >= 2u * static_cast<uint32_t>(resident)) ++c.waves;
+    const uint32_t most = (total + (1u << least_shift) - 1) >> least_shift;
+    if (c.waves == 1 && most < static_cast<uint32_t>(resident)) c.across = most < 1 ? 1 : static_cast<int>(most);
     return c;
 }
 
