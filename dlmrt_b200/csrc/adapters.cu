@@ -5,11 +5,12 @@
 // Bound by reading the adapters' matrices once (rank * (k + n) * 2 bytes each) and, for the small sizes of a block of
 // rows, by the chain of latencies between the two products. One launch does both: a cluster of eight CTAs takes up to 16
 // rows of one adapter (the M of an mma.sync). Its CTAs split k for x A^T, add their FP32 partial sums through each other's
-// shared memory in rank order (so the value never depends on timing), and split n for the second product.
+// shared memory in rank order (so the value never depends on timing), and split n for the second product, whose first
+// operands are on their way before the exchange.
 //
-// Which rows form a cluster is read off `ids` by the cluster itself: cluster c leads if row c is the 1st, 17th, 33rd ...
-// row of its adapter, and then takes the next rows of that adapter, up to 16; otherwise it has nothing to do. No sort, no
-// host round trip, any order of ids.
+// Which rows form a cluster is read off `ids` by the cluster itself: a row leads if it is the 1st, 17th, 33rd ... of its
+// adapter, and cluster c takes the c-th leader's adapter and that row's next fellows, up to 16. No sort, no host round trip,
+// any order of ids. There are at most count + m / 16 leaders.
 #include <cooperative_groups.h>
 
 #include "mma.cuh"
@@ -19,78 +20,111 @@ namespace dlm {
 
 namespace {
 
-constexpr int kAdapterThreads = 256;
-constexpr int kAdapterWarps = kAdapterThreads / 32;
 constexpr int kAdapterCtas = 8;
 constexpr int kAdapterRows = 16;
-constexpr int kMaxRank = 128;
+constexpr int kMostRows = 256;
 
+constexpr int kWarps = 8, kThreads = kWarps * 32;  // a thread for each row that a call may have
+static_assert(kThreads == kMostRows, "a thread looks at one row's id");
+
+// kTiles: n8 tiles of the first product's output, rank / 8 rounded up. CTAs of an SM: rank 16 with 48 adapters is 408 CTAs,
+// in one wave at three an SM (12 us) but three waves at one (22 us, with 16 warps each).
+template <int kTiles>
+constexpr int adapter_ctas() {
+    return kTiles <= 2 ? 3 : kTiles <= 8 ? 2 : 1;
+}
+
+template <int kTiles>
 struct AdapterSmem {
-    float part[kAdapterWarps][kAdapterRows][kMaxRank];
-    float sum[kAdapterRows][kMaxRank];                     // this CTA's share of x A^T, read by the cluster
-    uint32_t high[kAdapterRows][kMaxRank / 2 + 4];         // x A^T times the scale, BF16 pairs
-    uint32_t low[kAdapterRows][kMaxRank / 2 + 4];          // what those leave over, BF16 pairs
+    float part[kWarps][kAdapterRows][kTiles * 8 + 4];
+    float sum[kAdapterRows][kTiles * 8];                    // this CTA's share of x A^T, read by the cluster
+    uint32_t high[kAdapterRows][kTiles * 4 + 4];            // x A^T times the scale, BF16 pairs
+    uint32_t low[kAdapterRows][kTiles * 4 + 4];             // what those leave over, BF16 pairs
+    int4 ids[kMostRows / 4];
     int rows[kAdapterRows];
-    uint32_t match[kAdapterWarps];
+    uint32_t leads[kMostRows / 32];
+    int lead, lead_before;
 };
 
 }  // namespace
 
-// kTiles: n8 tiles of the first product's output, rank / 8 rounded up.
 template <int kTiles>
-__global__ void __launch_bounds__(kAdapterThreads) adapters_kernel(const __grid_constant__ DlmAdapters p) {
+__global__ void __launch_bounds__(kThreads, adapter_ctas<kTiles>()) adapters_kernel(const __grid_constant__ DlmAdapters p) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) uint8_t raw[];
-    AdapterSmem& sm = *reinterpret_cast<AdapterSmem*>(raw);
+    AdapterSmem<kTiles>& sm = *reinterpret_cast<AdapterSmem<kTiles>*>(raw);
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int cta = static_cast<int>(blockIdx.x), lead = static_cast<int>(blockIdx.y);
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lead_id = p.ids[lead];
+    const int cta = static_cast<int>(blockIdx.x), which = static_cast<int>(blockIdx.y), clusters = static_cast<int>(gridDim.y);
     const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(p.base);
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
-    if (lead_id < 0 || lead_id >= p.count) {  // uniform over the cluster
-        if (lead_id >= p.count && cta == 0 && tid == 0) report_index(p.status, lead, kIndexAdapter, lead_id);
-        if (base != out) {
-            for (int c = cta * kAdapterThreads + tid; c < p.n / 8; c += kAdapterCtas * kAdapterThreads)
-                *reinterpret_cast<uint4*>(out + lead * p.ldo + c * 8) = *reinterpret_cast<const uint4*>(base + lead * p.ldb + c * 8);
-        }
-        return;
-    }
-    // Rows of this adapter: how many are in front of `lead`, and the 16 from it on.
-    {
-        const bool same = tid < p.m && p.ids[tid] == lead_id;
-        const uint32_t bits = __ballot_sync(0xFFFFFFFFu, same);
-        if (lane == 0) sm.match[warp] = bits;
-        if (tid < kAdapterRows) sm.rows[tid] = -1;
-        __syncthreads();
-        int before_me = __popc(bits & ((1u << lane) - 1)), before_lead = 0;
-#pragma unroll
-        for (int w = 0; w < kAdapterWarps; ++w) {
-            if (w < warp) before_me += __popc(sm.match[w]);
-            if (w < lead / 32) before_lead += __popc(sm.match[w]);
-            if (w == lead / 32) before_lead += __popc(sm.match[w] & ((1u << (lead & 31)) - 1));
-        }
-        if (before_lead % kAdapterRows) return;  // another cluster has this row; uniform over the cluster
-        const int at = before_me - before_lead;
-        if (same && at >= 0 && at < kAdapterRows) sm.rows[at] = tid;
-        __syncthreads();
-    }
-    const int row0 = sm.rows[g], row1 = sm.rows[g + 8];
     const int rank = p.rank;
+    int* ids = reinterpret_cast<int*>(sm.ids);
+    if (tid < kAdapterRows) sm.rows[tid] = -1;
+    if (tid == 0) sm.lead = -1;
+    pdl_wait();
+    pdl_launch_dependents();
+    int id = -1;
+    if (tid < p.m) {
+        id = p.ids[tid];
+        if (id >= p.count) {
+            if (cta == 0 && which == 0) report_index(p.status, tid, kIndexAdapter, id);
+            id = -1;
+        }
+    }
+    ids[tid] = id;
+    __syncthreads();
+    // Rows of the same adapter in front of this thread's row; the leaders among all rows.
+    int before = 0;
+    for (int w = 0; w < warp; ++w) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int4 other = sm.ids[w * 8 + i];
+            before += (other.x == id) + (other.y == id) + (other.z == id) + (other.w == id);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int4 other = sm.ids[warp * 8 + i];
+        before += (other.x == id && 4 * i < lane) + (other.y == id && 4 * i + 1 < lane) + (other.z == id && 4 * i + 2 < lane) +
+                  (other.w == id && 4 * i + 3 < lane);
+    }
+    const bool leads = id >= 0 && before % kAdapterRows == 0;
+    const uint32_t leaders = __ballot_sync(0xFFFFFFFFu, leads);
+    if (lane == 0) sm.leads[warp] = leaders;
+    // Rows without an adapter: out = base, shared out among the clusters.
+    if (base != out) {
+        for (int row = which; row < p.m; row += clusters) {
+            if (ids[row] >= 0) continue;
+            for (int c = cta * kThreads + tid; c < p.n / 8; c += kAdapterCtas * kThreads)
+                *reinterpret_cast<uint4*>(out + row * p.ldo + c * 8) = *reinterpret_cast<const uint4*>(base + row * p.ldb + c * 8);
+        }
+    }
+    __syncthreads();
+    if (leads) {
+        int place = __popc(leaders & ((1u << lane) - 1));  // leaders in front of this row
+        for (int w = 0; w < warp; ++w) place += __popc(sm.leads[w]);
+        if (place == which) sm.lead = tid, sm.lead_before = before;
+    }
+    __syncthreads();
+    const int lead = sm.lead;
+    if (lead < 0) return;  // fewer leaders than clusters; uniform over the cluster
+    const int adapter = ids[lead], at = before - sm.lead_before;
+    if (id == adapter && at >= 0 && at < kAdapterRows) sm.rows[at] = tid;
+    __syncthreads();
+    const int row0 = sm.rows[g], row1 = sm.rows[g + 8];
 
     // -- x A^T over this CTA's part of k: units of 32, a lane's 16 bytes are two k16 steps' operands -----------------
     {
         const __nv_bfloat16* x0 = static_cast<const __nv_bfloat16*>(p.x) + (row0 < 0 ? 0 : row0) * p.ldx;
         const __nv_bfloat16* x1 = static_cast<const __nv_bfloat16*>(p.x) + (row1 < 0 ? 0 : row1) * p.ldx;
-        const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + static_cast<size_t>(lead_id) * rank * p.k;
+        const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a) + static_cast<size_t>(adapter) * rank * p.k;
         const int units = (p.k + 31) / 32;
         const int u0 = units * cta / kAdapterCtas, u1 = units * (cta + 1) / kAdapterCtas;
         float acc[kTiles][4] = {};
         const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
-        for (int u = u0 + warp; u < u1; u += kAdapterWarps) {
+#pragma unroll(kTiles <= 4 ? 4 : 2)
+        for (int u = u0 + warp; u < u1; u += kWarps) {
             const int at = u * 32 + t * 8;
             const bool in = at < p.k;
             const uint4 r0 = in && row0 >= 0 ? *reinterpret_cast<const uint4*>(x0 + at) : zero;
@@ -112,26 +146,50 @@ __global__ void __launch_bounds__(kAdapterThreads) adapters_kernel(const __grid_
             *reinterpret_cast<float2*>(&sm.part[warp][g + 8][i * 8 + 2 * t]) = make_float2(acc[i][2], acc[i][3]);
         }
     }
+    // -- the second product's operands: groups of 32 columns. Tile j's column c stands for column 8 (c / 2) + 2 j + c % 2 of
+    // the group, so that a lane's results of four tiles are eight neighbouring columns: 16 bytes of the output row.
+    constexpr int kSteps = (kTiles + 1) / 2;  // k16 steps; a lane's 8 bytes of B are one step's operand
+    const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.b) + static_cast<size_t>(adapter) * p.n * rank;
+    const int groups = (p.n + 31) / 32;
+    uint2 w[kSteps][4];
+    uint4 old[2];
+    auto fetch = [&](int group) {
+        const int column0 = group * 32 + 8 * (g / 2) + (g & 1);  // of tile 0
+        const bool col_in = group * 32 + 8 * (g / 2) < p.n;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const bool in = col_in && s * 16 + t * 4 < rank;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[s][j] = in ? *reinterpret_cast<const uint2*>(b + static_cast<size_t>(column0 + 2 * j) * rank + s * 16 + t * 4) : make_uint2(0, 0);
+        }
+        const int column = group * 32 + 8 * t;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        old[0] = column < p.n && row0 >= 0 ? *reinterpret_cast<const uint4*>(base + row0 * p.ldb + column) : zero;
+        old[1] = column < p.n && row1 >= 0 ? *reinterpret_cast<const uint4*>(base + row1 * p.ldb + column) : zero;
+    };
+    int group = cta + warp * kAdapterCtas;  // neighbouring groups in different CTAs: all have work where groups are few
+    if (group < groups) fetch(group);
     __syncthreads();
-    for (int i = tid; i < kAdapterRows * kTiles * 8; i += kAdapterThreads) {
+    for (int i = tid; i < kAdapterRows * kTiles * 8; i += kThreads) {
         const int r = i / (kTiles * 8), c = i - r * (kTiles * 8);
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kAdapterWarps; ++w) v += sm.part[w][r][c];
+        for (int from = 0; from < kWarps; ++from) v += sm.part[from][r][c];
         sm.sum[r][c] = v;
     }
     cluster.sync();
     // -- the cluster's sum, scaled, as BF16 pairs of high and low part (16 bits of mantissa between them) ------------
     {
-        const float scale = p.scales[lead_id];
-        for (int i = tid; i < kAdapterRows * kTiles * 4; i += kAdapterThreads) {
+        const float scale = p.scales[adapter];
+        for (int i = tid; i < kAdapterRows * kTiles * 4; i += kThreads) {
             const int r = i / (kTiles * 4), c = (i - r * (kTiles * 4)) * 2;
-            float2 v = make_float2(0.f, 0.f);
+            float2 s[kAdapterCtas], v = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kAdapterCtas; ++w) {
-                const float2 s = *reinterpret_cast<const float2*>(cluster.map_shared_rank(&sm.sum[r][c], w));
-                v.x += s.x, v.y += s.y;
-            }
+            for (int from = 0; from < kAdapterCtas; ++from)
+                s[from] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(&sm.sum[r][c], from));
+#pragma unroll
+            for (int from = 0; from < kAdapterCtas; ++from) v.x += s[from].x, v.y += s[from].y;
             v.x *= scale, v.y *= scale;
             const uint32_t high = narrow2<__nv_bfloat16>(v.x, v.y);
             const float2 h = widen2<__nv_bfloat16>(high);
@@ -139,12 +197,8 @@ __global__ void __launch_bounds__(kAdapterThreads) adapters_kernel(const __grid_
             sm.low[r][c / 2] = narrow2<__nv_bfloat16>(v.x - h.x, v.y - h.y);
         }
     }
-    cluster.sync();  // also: no CTA leaves while another still reads its sums
-
-    // -- the second product over this CTA's part of n ----------------------------------------------------------------
-    // Groups of 32 columns. Tile j's column c stands for column 8 (c / 2) + 2 j + c % 2 of the group, so that a lane's
-    // results of four tiles are eight neighbouring columns: 16 bytes of the output row.
-    constexpr int kSteps = (kTiles + 1) / 2;  // k16 steps; a lane's 8 bytes of B are one step's operand
+    auto read_all = cluster.barrier_arrive();  // no CTA leaves while another still reads its sums
+    __syncthreads();
     uint32_t high[kSteps][4], low[kSteps][4];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -155,47 +209,44 @@ __global__ void __launch_bounds__(kAdapterThreads) adapters_kernel(const __grid_
         low[s][0] = in ? sm.low[g][at] : 0, low[s][1] = in ? sm.low[g + 8][at] : 0;
         low[s][2] = in ? sm.low[g][at + 1] : 0, low[s][3] = in ? sm.low[g + 8][at + 1] : 0;
     }
-    const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.b) + static_cast<size_t>(lead_id) * p.n * rank;
-    const int groups = (p.n + 31) / 32;
-    for (int group = cta * kAdapterWarps + warp; group < groups; group += kAdapterCtas * kAdapterWarps) {
+    while (group < groups) {
         float acc[4][4] = {};
-        const int column0 = group * 32 + 8 * (g / 2) + (g & 1);  // of tile 0
-        const bool col_in = group * 32 + 8 * (g / 2) < p.n;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const bool in = col_in && s * 16 + t * 4 < rank;
-            uint2 w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[j] = in ? *reinterpret_cast<const uint2*>(b + static_cast<size_t>(column0 + 2 * j) * rank + s * 16 + t * 4) : make_uint2(0, 0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                mma_16816<__nv_bfloat16>(acc[j], high[s], w[j].x, w[j].y);
-                mma_16816<__nv_bfloat16>(acc[j], low[s], w[j].x, w[j].y);
+                mma_16816<__nv_bfloat16>(acc[j], high[s], w[s][j].x, w[s][j].y);
+                mma_16816<__nv_bfloat16>(acc[j], low[s], w[s][j].x, w[s][j].y);
             }
         }
         const int column = group * 32 + 8 * t;
+        const uint4 before_add[2] = {old[0], old[1]};
+        group += kAdapterCtas * kWarps;
+        if (group < groups) fetch(group);
         if (column < p.n) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int row = half ? row1 : row0;
                 if (row < 0) continue;
-                const uint4 old = *reinterpret_cast<const uint4*>(base + row * p.ldb + column);
                 float v[kVec] = {};
-                add_bf16x8(v, old);
+                add_bf16x8(v, before_add[half]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[2 * j] += acc[j][2 * half], v[2 * j + 1] += acc[j][2 * half + 1];
                 *reinterpret_cast<uint4*>(out + row * p.ldo + column) = pack_bf16x8(v);
             }
         }
     }
+    cluster.barrier_wait(std::move(read_all));
 }
 
 int launch_adapters(const DlmAdapters& p, const LaunchOpts& o) {
     void* args[] = {const_cast<DlmAdapters*>(&p)};
     auto run = [&](auto tiles) {
-        return launch_kernel<adapters_kernel<decltype(tiles)::value>>(dim3(kAdapterCtas, p.m), dim3(kAdapterThreads),
-                                                                      static_cast<int>(sizeof(AdapterSmem)), args, o, kAdapterCtas);
+        constexpr int kTiles = decltype(tiles)::value;
+        const int leaders = p.count + p.m / kAdapterRows;
+        return launch_kernel<adapters_kernel<kTiles>>(dim3(kAdapterCtas, leaders < p.m ? leaders : p.m),
+                                                      dim3(kThreads),
+                                                      static_cast<int>(sizeof(AdapterSmem<kTiles>)), args, o, kAdapterCtas);
     };
     const int tiles = p.rank / 8;
     if (tiles <= 1) return run(std::integral_constant<int, 1>{});

@@ -4,9 +4,12 @@
 //   y = x * rsqrt(mean(x^2) + eps) * weight          over a head, where a weight is given
 //   (a, b) -> (a cos - b sin, b cos + a sin)          on the first `rotated` elements, pairs i, i + rotated / 2 or 2i, 2i + 1
 //
-// Everything is FP32 between the load and the one rounding at the store. A head row is spread over head_dim / 8 lanes, 16
-// bytes each: the partner of a rotated element sits in another lane of the same group (one shuffle per element) or, for
-// neighbouring pairs, in the same lane.
+// Everything is FP32 between the load and the one rounding at the store. A block takes one token. A head row is spread over
+// head_dim / 8 lanes, 16 bytes each: the partner of a rotated element sits in another lane of the same group (one shuffle per
+// element) or, for neighbouring pairs, in the same lane, and a lane's cosines and sines are the same for all heads. Bound by
+// HBM for prompts: each lane has up to four heads' loads on the way at once, before the token's position and slot are known,
+// and registers are held to five blocks an SM (8189 tokens of 32 head rows of 256: 98 us with one row a lane, 65 with four at
+// three blocks an SM, 54 at five).
 #include "../../include/dlmrt_b200.h"
 #include "mma.cuh"
 #include "serving.cuh"
@@ -15,7 +18,8 @@ namespace dlm {
 
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendMostThreads = 256;
+constexpr int kHeadsAtOnce = 4;  // head rows that a lane has on the way
 
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& raw, float (&v)[8]) {
@@ -42,127 +46,135 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 }  // namespace
 
 template <typename T, int D, bool kCodes>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ DlmAppend p, int page_shift) {
-    constexpr int kLanes = D / 8;                       // lanes of one head row
-    constexpr int kRows = kAppendThreads / kLanes;      // head rows of a block
-    const int lane = static_cast<int>(threadIdx.x) % kLanes;
+__global__ void __launch_bounds__(kAppendMostThreads, kCodes ? 4 : 5) append_kernel(const __grid_constant__ DlmAppend p, int page_shift) {
+    constexpr int kLanes = D / 8;  // lanes of one head row
+    const int lane = static_cast<int>(threadIdx.x) % kLanes, group = static_cast<int>(threadIdx.x) / kLanes;
+    const int groups = static_cast<int>(blockDim.x) / kLanes;
     const int q_heads = p.q != nullptr ? p.q_heads : 0, heads = p.cache.heads;
-    const int per_token = q_heads + 2 * heads;
-    const long long item = static_cast<long long>(blockIdx.x) * kRows + static_cast<int>(threadIdx.x) / kLanes;
-    const long long token = item / per_token;
-    const int which = static_cast<int>(item - token * per_token);
-    const bool is_q = which < q_heads, is_v = which >= q_heads + heads;
-    const int head = is_q ? which : is_v ? which - q_heads - heads : which - q_heads;
+    const int rows = q_heads + 2 * heads;  // queries, keys, values
+    const long long token = blockIdx.x;
     pdl_wait();
     pdl_launch_dependents();
-    bool live = token < p.n;
-    int pos = 0;
-    long long slot = -1;
-    if (live) {
-        slot = p.slots[token];
-        if (p.rotated) pos = p.positions[token];
+    const long long slot = p.slots[token];
+    const int pos = p.rotated ? p.positions[token] : 0;
+    const T* q = static_cast<const T*>(p.q) + token * p.q_strides[0] + lane * 8;
+    const T* k = static_cast<const T*>(p.k) + token * p.k_strides[0] + lane * 8;
+    const T* v = static_cast<const T*>(p.v) + token * p.v_strides[0] + lane * 8;
+    auto load = [&](int row) {
+        const T* src = row < q_heads           ? q + row * p.q_strides[1]
+                       : row < q_heads + heads ? k + (row - q_heads) * p.k_strides[1]
+                                               : v + (row - q_heads - heads) * p.v_strides[1];
+        return *reinterpret_cast<const uint4*>(src);
+    };
+    // The same number of passes for every group: all lanes of a warp take part in the shuffles.
+    for (int base = group; base - group < rows; base += groups * kHeadsAtOnce) {
+        uint4 raw[kHeadsAtOnce];
+#pragma unroll
+        for (int i = 0; i < kHeadsAtOnce; ++i) {
+            const int row = base + i * groups;
+            raw[i] = row < rows ? load(row) : make_uint4(0, 0, 0, 0);
+        }
         const bool bad_slot = slot >= static_cast<long long>(p.cache.pages) << page_shift;
         const bool bad_pos = p.rotated && (pos < 0 || pos >= p.table_rows);
-        if (bad_slot || bad_pos) {
-            if (which == 0 && lane == 0)
+        if (bad_slot || bad_pos) {  // nothing of this token is written
+            if (threadIdx.x == 0)
                 report_index(p.cache.status, static_cast<int>(token), bad_slot ? kIndexSlot : kIndexPosition,
                              bad_slot ? static_cast<int>(slot >> page_shift) : pos);
-            live = false;
+            return;
         }
-        if (slot < 0 && !is_q) live = false;
-    }
-    float v[8] = {};
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (live) {
-        const T* src = is_q ? static_cast<const T*>(p.q) + token * p.q_strides[0] + head * p.q_strides[1]
-                     : is_v ? static_cast<const T*>(p.v) + token * p.v_strides[0] + head * p.v_strides[1]
-                            : static_cast<const T*>(p.k) + token * p.k_strides[0] + head * p.k_strides[1];
-        raw = *reinterpret_cast<const uint4*>(src + lane * 8);
-        unpack8<T>(raw, v);
-    }
-    // The rows of one warp may be queries, keys and values: every lane takes part in the shuffles, whoever uses them.
-    const T* norm = static_cast<const T*>(is_v ? nullptr : is_q ? p.q_norm : p.k_norm);
-    if (p.q_norm != nullptr || p.k_norm != nullptr) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += v[i] * v[i];
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (norm != nullptr) {
-            const float r = rsqrtf(sum * (1.f / D) + p.eps);
-            float w[8];
-            unpack8<T>(*reinterpret_cast<const uint4*>(norm + lane * 8), w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i];
-        }
-    }
-    if (p.rotated) {
-        const int half = p.rotated / 2;
-        const bool turned = live && !is_v && lane * 8 < p.rotated;
-        const float* row = p.table + static_cast<long long>(turned ? pos : 0) * p.rotated;
-        if (p.interleaved) {
-            if (turned) {
-                const float4 c = *reinterpret_cast<const float4*>(row + lane * 4);
-                const float4 s = *reinterpret_cast<const float4*>(row + half + lane * 4);
-                const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = v[2 * i], b = v[2 * i + 1];
-                    v[2 * i] = a * cs[i] - b * sn[i];
-                    v[2 * i + 1] = b * cs[i] + a * sn[i];
-                }
-            }
-        } else {
-            const int step = half / 8;  // lanes between a pair's elements
-            const bool first = lane < step;
-            const int base = (static_cast<int>(threadIdx.x) & 31) - lane;
-            const int from = base + (lane * 8 < p.rotated ? (first ? lane + step : lane - step) : lane);
-            float other[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xFFFFFFFFu, v[i], from);
-            if (turned) {
+        // This lane's cosines and sines; partner: the lane that holds the other halves of its pairs.
+        float cs[8], sn[8];
+        const int half = p.rotated / 2, step = half / 8;
+        const bool turned = lane * 8 < p.rotated, first = lane < step;
+        const int partner = (static_cast<int>(threadIdx.x) & 31) + (!turned || p.interleaved ? 0 : first ? step : -step);
+        if (turned) {
+            const float* row = p.table + static_cast<long long>(pos) * p.rotated;
+            if (p.interleaved) {
+                *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(row + lane * 4);
+                *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(row + half + lane * 4);
+            } else {
                 const float* at = row + (first ? lane : lane - step) * 8;
-                float cs[8], sn[8];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     *reinterpret_cast<float4*>(cs + 4 * i) = *reinterpret_cast<const float4*>(at + 4 * i);
                     *reinterpret_cast<float4*>(sn + 4 * i) = *reinterpret_cast<const float4*>(at + half + 4 * i);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = first ? v[i] * cs[i] - other[i] * sn[i] : v[i] * cs[i] + other[i] * sn[i];
+                for (int i = 0; i < 8; ++i) sn[i] = first ? -sn[i] : sn[i];  // x * cos + partner * sn, for both halves
             }
         }
-    }
-    if (!live) return;
-    const bool as_is = norm == nullptr && (is_v || !p.rotated);  // a copy keeps its bits, those of a NaN among them
-    if (is_q) {
-        T* dst = static_cast<T*>(p.q_out) + token * p.out_strides[0] + head * p.out_strides[1];
-        *reinterpret_cast<uint4*>(dst + lane * 8) = as_is ? raw : pack8<T>(v);
-        return;
-    }
-    const int64_t* st = is_v ? p.cache.v_strides : p.cache.k_strides;
-    const long long page = slot >> page_shift, within = slot & ((1ll << page_shift) - 1);
-    const long long at = page * st[0] + head * st[1] + within * st[2] + lane * 8;
-    void* pool = is_v ? p.cache.values : p.cache.keys;
-    if constexpr (kCodes) {
-        const float scale = (is_v ? p.cache.v_scale : p.cache.k_scale)[head];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] / scale;
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at) =
-            make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
-    } else {
-        *reinterpret_cast<uint4*>(static_cast<T*>(pool) + at) = as_is ? raw : pack8<T>(v);
+        for (int i = 0; i < kHeadsAtOnce; ++i) {
+            const int row = base + i * groups;
+            const bool is_q = row < q_heads, is_v = row >= q_heads + heads;
+            const int head = is_q ? row : is_v ? row - q_heads - heads : row - q_heads;
+            const T* norm = static_cast<const T*>(is_v ? nullptr : is_q ? p.q_norm : p.k_norm);
+            float x[8];
+            unpack8<T>(raw[i], x);
+            if (p.q_norm != nullptr || p.k_norm != nullptr) {
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
+#pragma unroll
+                for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+                if (norm != nullptr) {
+                    const float r = rsqrtf(sum * (1.f / D) + p.eps);
+                    float w[8];
+                    unpack8<T>(*reinterpret_cast<const uint4*>(norm + lane * 8), w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = x[j] * r * w[j];
+                }
+            }
+            if (p.rotated && p.interleaved) {
+                if (turned && !is_v) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float a = x[2 * j], b = x[2 * j + 1];
+                        x[2 * j] = a * cs[j] - b * sn[j];
+                        x[2 * j + 1] = b * cs[j] + a * sn[j];
+                    }
+                }
+            } else if (p.rotated) {
+                float other[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(0xFFFFFFFFu, x[j], partner);
+                if (turned && !is_v) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = x[j] * cs[j] + other[j] * sn[j];
+                }
+            }
+            if (row >= rows || (slot < 0 && !is_q)) continue;
+            const bool as_is = norm == nullptr && (is_v || !p.rotated);  // a copy keeps its bits, those of a NaN among them
+            if (is_q) {
+                T* dst = static_cast<T*>(p.q_out) + token * p.out_strides[0] + head * p.out_strides[1] + lane * 8;
+                *reinterpret_cast<uint4*>(dst) = as_is ? raw[i] : pack8<T>(x);
+                continue;
+            }
+            const int64_t* st = is_v ? p.cache.v_strides : p.cache.k_strides;
+            const long long page = slot >> page_shift, within = slot & ((1ll << page_shift) - 1);
+            const long long at = page * st[0] + head * st[1] + within * st[2] + lane * 8;
+            void* pool = is_v ? p.cache.values : p.cache.keys;
+            if constexpr (kCodes) {
+                const float scale = (is_v ? p.cache.v_scale : p.cache.k_scale)[head];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = x[j] / scale;
+                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + at) =
+                    make_uint2(e4m3x4(x[0], x[1], x[2], x[3]), e4m3x4(x[4], x[5], x[6], x[7]));
+            } else {
+                *reinterpret_cast<uint4*>(static_cast<T*>(pool) + at) = as_is ? raw[i] : pack8<T>(x);
+            }
+        }
     }
 }
 
 template <typename T, int D>
 static int launch_append_d(const DlmAppend& p, int page_shift, const LaunchOpts& o) {
-    const long long items = static_cast<long long>(p.n) * ((p.q != nullptr ? p.q_heads : 0) + 2 * p.cache.heads);
-    constexpr int kRows = kAppendThreads / (D / 8);
+    const int rows = (p.q != nullptr ? p.q_heads : 0) + 2 * p.cache.heads;
+    const int lanes = (rows + kHeadsAtOnce - 1) / kHeadsAtOnce * (D / 8);
+    const int threads = lanes >= kAppendMostThreads ? kAppendMostThreads : (lanes + 31) / 32 * 32;
     void* args[] = {const_cast<DlmAppend*>(&p), &page_shift};
-    const dim3 grid(static_cast<unsigned>((items + kRows - 1) / kRows));
-    return p.cache.type == DLM_E4M3 ? launch_kernel<append_kernel<T, D, true>>(grid, dim3(kAppendThreads), 0, args, o)
-                                    : launch_kernel<append_kernel<T, D, false>>(grid, dim3(kAppendThreads), 0, args, o);
+    return p.cache.type == DLM_E4M3 ? launch_kernel<append_kernel<T, D, true>>(dim3(p.n), dim3(threads), 0, args, o)
+                                    : launch_kernel<append_kernel<T, D, false>>(dim3(p.n), dim3(threads), 0, args, o);
 }
 
 int launch_append(const DlmAppend& p, int page_shift, const LaunchOpts& o) {

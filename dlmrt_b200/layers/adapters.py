@@ -42,6 +42,7 @@ class Adapters:
         d.a, d.b, d.scales, d.status = a.data_ptr(), b.data_ptr(), scales.data_ptr(), self.status.data_ptr()
         d.n, d.k, d.rank, d.count, d.pdl = self.n, self.k, self.rank, self.count, 1
         self._plans = {}  # everything of a call's arguments but addresses -> its checked descriptor without these
+        self._last = (None, None)  # the one used last, compared before the others are looked through
         _lib.lib()
 
     def check(self):
@@ -54,12 +55,15 @@ class Adapters:
         a row without adapter."""
         key = (x.shape, x.stride(), x.dtype, x.device, ids.shape, ids.stride(), ids.dtype, ids.device, base.shape, base.stride(),
                base.dtype, base.device, None if out is None else (out.shape, out.stride(), out.dtype, out.device))
-        plan = self._plans.get(key)
-        if plan is None:
-            plan = self._plan(x, ids, base, out)
-            if len(self._plans) >= _MOST_PLANS:
-                self._plans.clear()
-            self._plans[key] = plan
+        last, plan = self._last
+        if key != last:
+            plan = self._plans.get(key)
+            if plan is None:
+                plan = self._plan(x, ids, base, out)
+                if len(self._plans) >= _MOST_PLANS:
+                    self._plans.clear()
+                self._plans[key] = plan
+            self._last = key, plan
         if out is None:
             out = torch.empty_like(base, memory_format=torch.contiguous_format)
         d = DlmAdapters.from_buffer_copy(plan)
