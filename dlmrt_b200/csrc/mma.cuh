@@ -29,6 +29,16 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
     }
 }
 
+// The same of E4M3: D[16, 8] += A[16, 32] * B[32, 8]; a0 holds A[g][4t .. 4t + 3], a1 row g + 8, a2 columns + 16, a3 both; b0
+// holds B[4t .. 4t + 3][g], b1 rows + 16.
+__device__ __forceinline__ void mma_16832_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t smem) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -58,6 +68,14 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
     return h2;
 }
 
+// Four values as E4M3 codes, the first in the low byte: to nearest, at most the largest code in magnitude, NaN stays NaN.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
+}
+
 template <typename T>
 __device__ __forceinline__ float2 widen2(uint32_t v) {
     if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
@@ -78,7 +96,8 @@ __device__ __forceinline__ float exp2_approx(float x) {  // relative error about
 }
 
 
-// Launches `Kernel`; its limit of dynamic shared memory is raised once per device, to `smem` (the same at every call).
+// Launches `Kernel`; where it takes more dynamic shared memory than any kernel may, its limit is raised once per device, to
+// `smem` (then the same at every call).
 template <auto Kernel>
 int launch_kernel(dim3 grid, dim3 block, int smem, void** args, const LaunchOpts& o, int cluster = 1) {
     const void* kernel = reinterpret_cast<const void*>(Kernel);
@@ -102,7 +121,7 @@ int launch_kernel(dim3 grid, dim3 block, int smem, void** args, const LaunchOpts
     config.attrs = attrs;
     config.numAttrs = static_cast<unsigned>(n);
     cudaError_t err = cudaSuccess;
-    if (smem > 0) {
+    if (smem > 40 * 1024) {
         static bool raised[64] = {};
         int dev = 0;
         err = cudaGetDevice(&dev);

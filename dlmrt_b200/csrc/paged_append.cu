@@ -36,13 +36,6 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
     return make_uint4(narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3]), narrow2<T>(v[4], v[5]), narrow2<T>(v[6], v[7]));
 }
 
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {  // saturating, NaN stays NaN
-    uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-    return static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
-}
-
 }  // namespace
 
 template <typename T, int D, bool kCodes>

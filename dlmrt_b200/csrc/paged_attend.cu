@@ -254,6 +254,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     constexpr int kSteps = D / 16;       // k16 steps of q . k
     constexpr int kOut = D / 8;          // n8 tiles of the output
     constexpr int kElem = kCodes ? 1 : 2;
+    // BF16 queries of FP8 keys: a query is the sum of two E4M3 values, exactly, and keys need not be widened.
+    constexpr bool kTwoCodes = kCodes && std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full[kStages], empty[kStages], work_full[kWorkSlots], work_empty[kWorkSlots], answered;
@@ -298,15 +300,16 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             }
             if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
         };
-        // Where the next step is: a run, an item in it, a step of 64 keys in that. Its pages are looked up a step ahead of its
-        // use, across items and runs: lane j asks for the page of box j.
+        // Where the next step is: a run, an item in it, a step of 64 keys in that. Pages are looked up a step ahead of their
+        // use, across items and runs, 32 entries of the table at once: lane j holds entry `window` + j.
         uint32_t unit = 0, last_unit = 0;
-        int sequence = 0, index = 0, first = 0, units = 0, lo = 0, tile = 0, page = INT_MIN;
+        int sequence = 0, index = 0, first = 0, units = 0, lo = 0, tile = 0, window = 0, pages = 0;
         Sequence s{};
         Work work{};
-        auto look_up = [&]() {
-            const int key = work.start + tile * kTileKeys + lane * box_keys;
-            page = lane < boxes && key < work.end ? p.a.page_table[sequence * p.a.table_stride + (key >> p.page_shift)] : INT_MIN;
+        auto look_up = [&](int from) {
+            window = from;
+            const int entry = from + lane;
+            pages = entry << p.page_shift < work.end ? p.a.page_table[sequence * p.a.table_stride + entry] : INT_MIN;
         };
         auto begin_item = [&]() {
             units = min(static_cast<int>(last_unit - unit), s.units - first);
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             work.end = first + units == s.units ? hi : min(hi, s.base + ((first + units) << p.unit_shift));
             work.tiles = work.end > work.start ? (work.end - work.start + kTileKeys - 1) / kTileKeys : 0;
             tile = 0;
-            look_up();
+            if (work.tiles > 0) look_up(work.start >> p.page_shift);
         };
         auto begin_run = [&]() -> bool {
             if (run < 0 || run >= line.runs) return false;
@@ -341,7 +344,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         };
         auto advance = [&]() -> bool {
             if (++tile < work.tiles) {
-                look_up();
+                const int entry = (work.start + tile * kTileKeys) >> p.page_shift;
+                if (entry >= window + 32) look_up(entry);
                 return true;
             }
             unit += units;
@@ -364,18 +368,22 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         while (more) {
             const Work now = work;
             const int now_tile = tile, now_lo = lo;
-            int now_page = page;
+            const int now_pages = pages, now_window = window;
             more = advance();
             if (now_tile == 0) announce(now);
             if (now.tiles == 0) continue;
             const int key0 = now.start + now_tile * kTileKeys;
-            const bool in_pool = static_cast<uint32_t>(now_page) < static_cast<uint32_t>(p.a.cache.pages);
+            // Lane j: the page of box j, INT_MIN where no key of the box is in the run.
+            const int entry = ((key0 + lane * box_keys) >> p.page_shift) - now_window;
+            int page = __shfl_sync(0xFFFFFFFFu, now_pages, entry & 31);
+            const bool in_pool = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.a.cache.pages);
             uint64_t present = ~0ull;
             if (!__all_sync(0xFFFFFFFFu, in_pool || lane >= boxes) || now.end - key0 < kTileKeys) {
-                if (!in_pool && now_page != INT_MIN && key0 + (lane + 1) * box_keys > now_lo)
-                    report_index(p.a.cache.status, now.sequence, kIndexPage, now_page);
-                const uint32_t there = __ballot_sync(0xFFFFFFFFu, in_pool);
-                if (!in_pool) now_page = p.a.cache.pages;  // past the pool's end: the box is filled with zeros
+                if (lane >= boxes || key0 + lane * box_keys >= now.end) page = INT_MIN;
+                else if (!in_pool && key0 + (lane + 1) * box_keys > now_lo)
+                    report_index(p.a.cache.status, now.sequence, kIndexPage, page);
+                const uint32_t there = __ballot_sync(0xFFFFFFFFu, in_pool && page != INT_MIN);
+                if (!in_pool || page == INT_MIN) page = p.a.cache.pages;  // past the pool's end: the box is filled with zeros
                 const uint64_t box_bits = box_keys == 64 ? ~0ull : (1ull << box_keys) - 1;
                 present = 0;
                 for (int j = 0; j < boxes; ++j)
@@ -395,7 +403,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 else mbar_expect_tx(bar, 2 * S::kBytes);
             }
             for (int j = 0; j < boxes; ++j) {
-                const int from = __shfl_sync(0xFFFFFFFFu, now_page, j);
+                const int from = __shfl_sync(0xFFFFFFFFu, page, j);
                 const int at = (key0 + j * box_keys) & slot_mask, box = j * box_keys * S::kPieces * 16;
                 if (leader && !failed) {
                     tma_load_5d(to + box, &p.tm_k, bar, 0, at, 0, now.head, from, kEvictNormal);
@@ -455,8 +463,10 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     }
     float scale0 = p.a.scale * kLog2e, scale1 = scale0;
     if constexpr (kCodes) {
-        // A BF16 row may not fit a half: it is scaled by the power of two that brings its largest element below 2 (exact,
-        // but for elements 2^-14 of the largest, whose error is at most 2^-25 of it), and the scores are scaled back.
+        // Rows are scaled by the power of two that brings their largest element below 2 (BF16 need not fit a half; exact, but
+        // for elements 2^-14 of the largest, whose error is at most 2^-25 of it) or below 256, and the scores scaled back.
+        // A BF16 element's eight bits are then four in a high code and four in a low one, which counts a sixteenth (exact
+        // again, but for elements 2^-13 of the largest, whose error is at most 2^-21 of it).
         const float key_scale = p.a.cache.k_scale[head];
         scale0 *= key_scale, scale1 *= key_scale;
         float top0 = 0.f, top1 = 0.f;
@@ -477,17 +487,39 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         // 2^-e and 2^e for the exponent e of the largest element, kept where both are normal numbers.
         const int e0 = min(max(static_cast<int>(__float_as_uint(top0) >> 23) - 127, -100), 126);
         const int e1 = min(max(static_cast<int>(__float_as_uint(top1) >> 23) - 127, -100), 126);
-        const float down0 = __uint_as_float(static_cast<uint32_t>(127 - e0) << 23);
-        const float down1 = __uint_as_float(static_cast<uint32_t>(127 - e1) << 23);
-        scale0 *= __uint_as_float(static_cast<uint32_t>(127 + e0) << 23);
-        scale1 *= __uint_as_float(static_cast<uint32_t>(127 + e1) << 23);
+        constexpr int kUp = kTwoCodes ? 7 : 0;
+        const float down0 = __uint_as_float(static_cast<uint32_t>(127 + kUp - e0) << 23);
+        const float down1 = __uint_as_float(static_cast<uint32_t>(127 + kUp - e1) << 23);
+        scale0 *= __uint_as_float(static_cast<uint32_t>(127 - kUp + e0) << 23);
+        scale1 *= __uint_as_float(static_cast<uint32_t>(127 - kUp + e1) << 23);
+        if constexpr (kTwoCodes) {
+            if (!isfinite(top0)) scale0 = NAN;  // a code would be the largest one instead
+            if (!isfinite(top1)) scale1 = NAN;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < kSteps; s += 2) {  // q[s]: the A operand of a k32 step of high codes, q[s + 1]: of low codes
+                uint32_t high[4], low[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 a = widen2<T>(q[s][i]);
-                const float down = i & 1 ? down1 : down0;
-                q[s][i] = narrow2<__half>(a.x * down, a.y * down);
+                for (int i = 0; i < 4; ++i) {  // rows g, g + 8; 16 elements further on
+                    const int from = s + i / 2;
+                    const float down = i & 1 ? down1 : down0;
+                    const float2 a = widen2<T>(q[from][i & 1]), b = widen2<T>(q[from][2 + (i & 1)]);
+                    const float x[4] = {a.x * down, a.y * down, b.x * down, b.y * down};
+                    high[i] = e4m3x4(x[0], x[1], x[2], x[3]);
+                    const float2 h0 = widen2<__half>(e4m3x2_to_f16x2(high[i] & 0xFFFFu)), h1 = widen2<__half>(e4m3x2_to_f16x2(high[i] >> 16));
+                    low[i] = e4m3x4((x[0] - h0.x) * 16.f, (x[1] - h0.y) * 16.f, (x[2] - h1.x) * 16.f, (x[3] - h1.y) * 16.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[s][i] = high[i], q[s + 1][i] = low[i];
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 a = widen2<T>(q[s][i]);
+                    const float down = i & 1 ? down1 : down0;
+                    q[s][i] = narrow2<__half>(a.x * down, a.y * down);
+                }
             }
         }
     }
@@ -550,13 +582,21 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 query_step(k, a0);
                 query_step(k + 1, a1);
                 ldmatrix_x4(b, stage_k32 + rows_of_stage.at(r, k + (lane >> 4)));
-                mma_16816<M>(s[0], a0, e4m3x2_to_f16x2(b[0] & 0xFFFFu), e4m3x2_to_f16x2(b[0] >> 16));
-                mma_16816<M>(s[1], a0, e4m3x2_to_f16x2(b[1] & 0xFFFFu), e4m3x2_to_f16x2(b[1] >> 16));
-                mma_16816<M>(more_s[0], a1, e4m3x2_to_f16x2(b[2] & 0xFFFFu), e4m3x2_to_f16x2(b[2] >> 16));
-                mma_16816<M>(more_s[1], a1, e4m3x2_to_f16x2(b[3] & 0xFFFFu), e4m3x2_to_f16x2(b[3] >> 16));
+                if constexpr (kTwoCodes) {
+                    mma_16832_e4m3(s[0], a0, b[0], b[2]);
+                    mma_16832_e4m3(s[1], a0, b[1], b[3]);
+                    mma_16832_e4m3(more_s[0], a1, b[0], b[2]);
+                    mma_16832_e4m3(more_s[1], a1, b[1], b[3]);
+                } else {
+                    mma_16816<M>(s[0], a0, e4m3x2_to_f16x2(b[0] & 0xFFFFu), e4m3x2_to_f16x2(b[0] >> 16));
+                    mma_16816<M>(s[1], a0, e4m3x2_to_f16x2(b[1] & 0xFFFFu), e4m3x2_to_f16x2(b[1] >> 16));
+                    mma_16816<M>(more_s[0], a1, e4m3x2_to_f16x2(b[2] & 0xFFFFu), e4m3x2_to_f16x2(b[2] >> 16));
+                    mma_16816<M>(more_s[1], a1, e4m3x2_to_f16x2(b[3] & 0xFFFFu), e4m3x2_to_f16x2(b[3] >> 16));
+                }
             }
+            constexpr float kMore = kTwoCodes ? 1.f / 16 : 1.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i], s[1][i] += more_s[1][i];
+            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i] * kMore, s[1][i] += more_s[1][i] * kMore;
         }
         const bool by_row = key0 < all_from || key0 + kWarpKeys > all_to;  // rows see different keys of this tile
 #pragma unroll
@@ -742,17 +782,16 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
 
 // Joins the partial results of an item that lies in several runs: item blockIdx.x, or (with more items than runs) the one that
 // begins in run blockIdx.x and goes on. For each of its rows, out = sum_c exp2(m_c - m) o_c / sum_c exp2(m_c - m) l_c. The rows
-// are shared by gridDim.y blocks; in a block D / 4 threads take a row, and those that are left over further partial results
-// of the same rows.
+// are shared by gridDim.y blocks and their elements by gridDim.z; in a block every thread has four elements of a row, and
+// threads that are left over take further partial results of the same rows.
 constexpr int kJoinMostThreads = 1024;
 constexpr int kJoinAhead = 4;  // partial results that a thread has on the way at once
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_constant__ AttendDev p) {
-    constexpr int kAcross = D / 4;
-    __shared__ float4 sums[kJoinMostThreads / kAcross][kAcross];
-    __shared__ float2 stats[kJoinMostThreads / kAcross];
-    const int lines = blockDim.x / kAcross;
+    extern __shared__ float4 sums[];  // [lines][across], then stats[lines]
+    float2* stats = reinterpret_cast<float2*>(sums + blockDim.x);
+    const int across = D / 4 / gridDim.z, lines = blockDim.x / across;  // threads along a row, and how often
     // The lengths are older than the kernel in front, whose blocks waited for them before this one could start.
     const Line line(p, false);
     int sequence, index, run, last;
@@ -781,7 +820,7 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
     const int per_block = (p.rows_cap + gridDim.y - 1) / gridDim.y;
     const int row_begin = blockIdx.y * per_block, row_end = min(min(row_begin + per_block, p.rows_cap), p.rows - first_row);
     const int deep = max(1, lines / per_block);  // threads along the partial results of a row
-    const int x = threadIdx.x % kAcross, at = threadIdx.x / kAcross, y = at / per_block;
+    const int at = threadIdx.x / across, x = threadIdx.x - at * across + blockIdx.z * across, y = at / per_block;
     const float value_scale = p.a.cache.type == DLM_E4M3 ? p.a.cache.v_scale[head] : 1.f;
     for (int r0 = row_begin; r0 < row_end; r0 += deep == 1 ? lines : per_block) {
         const int r = r0 + (deep == 1 ? at : at % per_block);
@@ -817,20 +856,21 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
                 }
             }
         }
-        if (deep > 1) {  // the same for every thread of the block
-            sums[at][x] = sum;
-            if (x == 0) stats[at] = make_float2(top, l);
+        // The lines of a row are added two by two (the same loop for every thread of the block).
+        for (int n = deep; n > 1; n = (n + 1) / 2) {
+            const int far = (n + 1) / 2;
+            if (takes_part && y >= far && y < n) {
+                sums[threadIdx.x] = sum;
+                if (threadIdx.x == at * across) stats[at] = make_float2(top, l);
+            }
             __syncthreads();
-            if (takes_part && y == 0) {
-                for (int i = 1; i < deep; ++i) top = fmaxf(top, stats[at + i * per_block].x);
-                sum = make_float4(0.f, 0.f, 0.f, 0.f), l = 0.f;
-                for (int i = 0; i < deep; ++i) {
-                    const float2 ml = stats[at + i * per_block];
-                    const float4 v = sums[at + i * per_block][x];
-                    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
-                    l += ml.y * f;
-                    sum.x += v.x * f, sum.y += v.y * f, sum.z += v.z * f, sum.w += v.w * f;
-                }
+            if (takes_part && y + far < n) {
+                const float2 ml = stats[at + far * per_block];
+                const float4 v = sums[threadIdx.x + far * per_block * across];
+                const float m = fmaxf(top, ml.x);
+                const float f = top == -INFINITY ? 0.f : exp2_approx(top - m), h = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - m);
+                top = m, l = l * f + ml.y * h;
+                sum.x = sum.x * f + v.x * h, sum.y = sum.y * f + v.y * h, sum.z = sum.z * f + v.z * h, sum.w = sum.w * f + v.w * h;
             }
             __syncthreads();
         }
@@ -845,16 +885,18 @@ static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
     const int rc = launch_kernel<attend_kernel<T, D, kCodes>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes>::kBytes,
                                                               args, o);
     if (rc != 0 || p.partial == nullptr) return rc;
-    // With fewer items than runs an item may have hundreds of partial results: large blocks, one for each row. Otherwise it has
-    // two or three, and most blocks only find out that there is nothing to join (0.5 us; 9000 blocks took 25).
+    // With fewer items than runs an item may have hundreds of partial results: large blocks, one for a quarter of each row (293
+    // partial results of a row: 7 us in blocks of a whole row, all of it latency). Otherwise it has two or three, and most blocks
+    // only find out that there is nothing to join (0.5 us; 9000 blocks took 25).
     const long long items = static_cast<long long>(p.a.batch) * p.items;
     const LaunchOpts dependent{o.stream, true, false};  // always a dependent launch of the kernel above
-    if (p.by_item) {
-        const int rows = p.sms * 2 / items < 1 ? 1 : static_cast<int>(p.sms * 2 / items);
-        return launch_kernel<join_kernel<T, D>>(dim3(static_cast<unsigned>(items), rows < p.rows_cap ? rows : p.rows_cap),
-                                                dim3(p.grid >= 16 * items ? kJoinMostThreads : 256), 0, args, dependent);
-    }
-    return launch_kernel<join_kernel<T, D>>(dim3(p.grid), dim3(256), 0, args, dependent);
+    auto join = [&](unsigned blocks, int rows, int splits, int threads) {
+        return launch_kernel<join_kernel<T, D>>(dim3(blocks, rows < 1 ? 1 : rows < p.rows_cap ? rows : p.rows_cap, splits), dim3(threads),
+                                                threads * 16 + threads * splits / (D / 4) * 8, args, dependent);
+    };
+    if (!p.by_item) return join(static_cast<unsigned>(p.grid), 1, 1, 256);
+    const int rows = static_cast<int>(p.sms * 2 / items);
+    return p.grid > 32 * items ? join(static_cast<unsigned>(items), rows, 4, kJoinMostThreads) : join(static_cast<unsigned>(items), rows, 1, 256);
 }
 
 // Calls f with the type and the sizes of a call as compile-time constants.
