@@ -254,8 +254,6 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     constexpr int kSteps = D / 16;       // k16 steps of q . k
     constexpr int kOut = D / 8;          // n8 tiles of the output
     constexpr int kElem = kCodes ? 1 : 2;
-    // BF16 queries of FP8 keys: a query is the sum of two E4M3 values, exactly, and keys need not be widened.
-    constexpr bool kTwoCodes = kCodes && std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full[kStages], empty[kStages], work_full[kWorkSlots], work_empty[kWorkSlots], answered;
@@ -463,10 +461,9 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     }
     float scale0 = p.a.scale * kLog2e, scale1 = scale0;
     if constexpr (kCodes) {
-        // Rows are scaled by the power of two that brings their largest element below 2 (BF16 need not fit a half; exact, but
-        // for elements 2^-14 of the largest, whose error is at most 2^-25 of it) or below 256, and the scores scaled back.
-        // A BF16 element's eight bits are then four in a high code and four in a low one, which counts a sixteenth (exact
-        // again, but for elements 2^-13 of the largest, whose error is at most 2^-21 of it).
+        // A BF16 row may not fit a half: it is scaled by the power of two that brings its largest element below 2 (exact,
+        // but for elements 2^-14 of the largest, whose error is at most 2^-25 of it), and the scores are scaled back. (A query
+        // as the sum of two E4M3 values, and FP8 products: 170 us against 110 for 24 sequences of 12000 keys, heads of 256.)
         const float key_scale = p.a.cache.k_scale[head];
         scale0 *= key_scale, scale1 *= key_scale;
         float top0 = 0.f, top1 = 0.f;
@@ -487,43 +484,20 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         // 2^-e and 2^e for the exponent e of the largest element, kept where both are normal numbers.
         const int e0 = min(max(static_cast<int>(__float_as_uint(top0) >> 23) - 127, -100), 126);
         const int e1 = min(max(static_cast<int>(__float_as_uint(top1) >> 23) - 127, -100), 126);
-        constexpr int kUp = kTwoCodes ? 7 : 0;
-        const float down0 = __uint_as_float(static_cast<uint32_t>(127 + kUp - e0) << 23);
-        const float down1 = __uint_as_float(static_cast<uint32_t>(127 + kUp - e1) << 23);
-        scale0 *= __uint_as_float(static_cast<uint32_t>(127 - kUp + e0) << 23);
-        scale1 *= __uint_as_float(static_cast<uint32_t>(127 - kUp + e1) << 23);
-        if constexpr (kTwoCodes) {
-            if (!isfinite(top0)) scale0 = NAN;  // a code would be the largest one instead
-            if (!isfinite(top1)) scale1 = NAN;
+        const float down0 = __uint_as_float(static_cast<uint32_t>(127 - e0) << 23);
+        const float down1 = __uint_as_float(static_cast<uint32_t>(127 - e1) << 23);
+        scale0 *= __uint_as_float(static_cast<uint32_t>(127 + e0) << 23);
+        scale1 *= __uint_as_float(static_cast<uint32_t>(127 + e1) << 23);
 #pragma unroll
-            for (int s = 0; s < kSteps; s += 2) {  // q[s]: the A operand of a k32 step of high codes, q[s + 1]: of low codes
-                uint32_t high[4], low[4];
+        for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {  // rows g, g + 8; 16 elements further on
-                    const int from = s + i / 2;
-                    const float down = i & 1 ? down1 : down0;
-                    const float2 a = widen2<T>(q[from][i & 1]), b = widen2<T>(q[from][2 + (i & 1)]);
-                    const float x[4] = {a.x * down, a.y * down, b.x * down, b.y * down};
-                    high[i] = e4m3x4(x[0], x[1], x[2], x[3]);
-                    const float2 h0 = widen2<__half>(e4m3x2_to_f16x2(high[i] & 0xFFFFu)), h1 = widen2<__half>(e4m3x2_to_f16x2(high[i] >> 16));
-                    low[i] = e4m3x4((x[0] - h0.x) * 16.f, (x[1] - h0.y) * 16.f, (x[2] - h1.x) * 16.f, (x[3] - h1.y) * 16.f);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) q[s][i] = high[i], q[s + 1][i] = low[i];
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 a = widen2<T>(q[s][i]);
-                    const float down = i & 1 ? down1 : down0;
-                    q[s][i] = narrow2<__half>(a.x * down, a.y * down);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const float2 a = widen2<T>(q[s][i]);
+                const float down = i & 1 ? down1 : down0;
+                q[s][i] = narrow2<__half>(a.x * down, a.y * down);
             }
         }
     }
-
     const uint32_t* shared_q = nullptr;
     if constexpr (Shared::kQueriesInShared) {
         uint32_t* to = reinterpret_cast<uint32_t*>(smem + Shared::kRing);
@@ -582,21 +556,13 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 query_step(k, a0);
                 query_step(k + 1, a1);
                 ldmatrix_x4(b, stage_k32 + rows_of_stage.at(r, k + (lane >> 4)));
-                if constexpr (kTwoCodes) {
-                    mma_16832_e4m3(s[0], a0, b[0], b[2]);
-                    mma_16832_e4m3(s[1], a0, b[1], b[3]);
-                    mma_16832_e4m3(more_s[0], a1, b[0], b[2]);
-                    mma_16832_e4m3(more_s[1], a1, b[1], b[3]);
-                } else {
-                    mma_16816<M>(s[0], a0, e4m3x2_to_f16x2(b[0] & 0xFFFFu), e4m3x2_to_f16x2(b[0] >> 16));
-                    mma_16816<M>(s[1], a0, e4m3x2_to_f16x2(b[1] & 0xFFFFu), e4m3x2_to_f16x2(b[1] >> 16));
-                    mma_16816<M>(more_s[0], a1, e4m3x2_to_f16x2(b[2] & 0xFFFFu), e4m3x2_to_f16x2(b[2] >> 16));
-                    mma_16816<M>(more_s[1], a1, e4m3x2_to_f16x2(b[3] & 0xFFFFu), e4m3x2_to_f16x2(b[3] >> 16));
-                }
+                mma_16816<M>(s[0], a0, e4m3x2_to_f16x2(b[0] & 0xFFFFu), e4m3x2_to_f16x2(b[0] >> 16));
+                mma_16816<M>(s[1], a0, e4m3x2_to_f16x2(b[1] & 0xFFFFu), e4m3x2_to_f16x2(b[1] >> 16));
+                mma_16816<M>(more_s[0], a1, e4m3x2_to_f16x2(b[2] & 0xFFFFu), e4m3x2_to_f16x2(b[2] >> 16));
+                mma_16816<M>(more_s[1], a1, e4m3x2_to_f16x2(b[3] & 0xFFFFu), e4m3x2_to_f16x2(b[3] >> 16));
             }
-            constexpr float kMore = kTwoCodes ? 1.f / 16 : 1.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i] * kMore, s[1][i] += more_s[1][i] * kMore;
+            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i], s[1][i] += more_s[1][i];
         }
         const bool by_row = key0 < all_from || key0 + kWarpKeys > all_to;  // rows see different keys of this tile
 #pragma unroll
