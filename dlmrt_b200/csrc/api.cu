@@ -806,7 +806,7 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
 
 // Everything about an attention call that its device pointers do not decide.
 static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
-    constexpr int kWholeKeys = 512;
+    constexpr int kWholeKeys = 512, kBlocksAbove = 32;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
@@ -817,8 +817,10 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     if (a->cache.type != DLM_E4M3 && a->cache.type != a->type) return DLM_ERR_SHAPE;
     d->group = a->q_heads / a->cache.heads;
     d->rows = a->tokens * d->group;
-    d->row_tiles = (d->rows + kRowTile - 1) / kRowTile;
-    d->rows_cap = d->rows < kRowTile ? d->rows : kRowTile;
+    d->blocks = a->cache.type != DLM_E4M3 && d->rows > kBlocksAbove;
+    d->tile_rows = d->blocks ? kBlockRows : kRowTile;
+    d->row_tiles = (d->rows + d->tile_rows - 1) / d->tile_rows;
+    d->rows_cap = d->rows < d->tile_rows ? d->rows : d->tile_rows;
     if (static_cast<long long>(a->cache.heads) * d->row_tiles > 1 << 20) return DLM_ERR_SHAPE;
     d->items = a->cache.heads * d->row_tiles;
     long long span = keys;  // from the first key that some token sees, aligned down, to the last
@@ -828,18 +830,19 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->unit_shift = whole ? 31 : kUnitShift;
     d->least_shift = whole ? 0 : 1;
     d->sms = sms;
-    d->resident = sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
+    d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
+    d->most_waves = d->blocks ? 1 : 5;
     const long long units = whole ? 1 : (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
     if (units * a->batch * d->items > INT32_MAX) return DLM_ERR_SHAPE;
-    const Cut cut = attend_cut(static_cast<uint32_t>(units * a->batch * d->items), d->resident, d->least_shift);
+    const Cut cut = attend_cut(static_cast<uint32_t>(units * a->batch * d->items), d->resident, d->least_shift, d->most_waves);
     d->grid = cut.across * cut.waves;
     d->by_item = static_cast<long long>(a->batch) * d->items < d->grid;
     return DLM_OK;
 }
 
 // The pool as TMA reads it for the attention kernel: whole slots of one head and page, up to kTileKeys at once, in column
-// blocks of 128 bytes (the width of the swizzle) or of a head's 64.
-static int make_map_pages(CUtensorMap* map, const void* base, const DlmPages& c, const int64_t* strides) {
+// blocks of 128 bytes (the width of the swizzle) or of a head's 64; or, `apart`, one such block of them.
+static int make_map_pages(CUtensorMap* map, const void* base, const DlmPages& c, const int64_t* strides, bool apart) {
     EncodeTiled fn = encode_tiled();
     if (fn == nullptr) return DLM_ERR_CUDA;
     const int size = c.type == DLM_E4M3 ? 1 : 2, row_bytes = c.head_dim * size, block_bytes = row_bytes < 128 ? row_bytes : 128;
@@ -851,7 +854,7 @@ static int make_map_pages(CUtensorMap* map, const void* base, const DlmPages& c,
                                  bytes(strides[0], c.pages)};
     const cuuint32_t box[5] = {static_cast<cuuint32_t>(block_bytes / size),
                                static_cast<cuuint32_t>(c.page_size < kTileKeys ? c.page_size : kTileKeys),
-                               static_cast<cuuint32_t>(row_bytes / block_bytes), 1, 1};
+                               static_cast<cuuint32_t>(apart ? 1 : row_bytes / block_bytes), 1, 1};
     const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
     const CUresult r = fn(map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, const_cast<void*>(base),
                           dims, steps, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -902,8 +905,8 @@ int dlm_paged_attend(const DlmAttend* a, dlm_stream_t stream) {
         d.partial = static_cast<float*>(a->workspace);
         d.stats = d.partial + need / 4 / (a->cache.head_dim + 2) * a->cache.head_dim;
     }
-    rc = make_map_pages(&d.tm_k, a->cache.keys, a->cache, a->cache.k_strides);
-    if (rc == DLM_OK) rc = make_map_pages(&d.tm_v, a->cache.values, a->cache, a->cache.v_strides);
+    rc = make_map_pages(&d.tm_k, a->cache.keys, a->cache, a->cache.k_strides, d.blocks);
+    if (rc == DLM_OK) rc = make_map_pages(&d.tm_v, a->cache.values, a->cache, a->cache.v_strides, d.blocks);
     if (rc != DLM_OK) return rc;
     return launch_attend(d, {static_cast<cudaStream_t>(stream), a->pdl != 0, false});
 }

@@ -1,0 +1,335 @@
+// What both attention kernels over the paged cache share (paged_attend.cu, paged_blocks.cu): how the work is dealt out, the
+// producer that requests keys and values, and how a row is finished.
+//
+// An item is one sequence, key head and row tile. The keys of all items are lined up in units of 64 keys and cut into runs,
+// whatever the lengths of the sequences. The first runs go to as many CTAs as the GPU holds; a CTA that is done takes over
+// the run of a CTA that was not launched yet (cluster launch control). Runs get shorter towards the line's end, because SMs do
+// not read equally fast: with one run for each CTA the slowest came in 30 % behind the others. Requests go on across items and
+// runs. An item that lies in several runs leaves a partial result in each, which join_kernel adds up in their order: the
+// result does not depend on which CTA took which run.
+#pragma once
+
+#include <climits>
+
+#include "mma.cuh"
+#include "serving.cuh"
+
+namespace dlm {
+
+constexpr int kWorkSlots = 4;  // items that may be announced ahead
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A sequence's keys: how many, the position of its first new token, where its units begin, and how many an item of it has.
+struct Sequence {
+    int length, first_pos, base, units;
+};
+
+__device__ __forceinline__ Sequence sequence_of(const AttendDev& p, int index, bool tell) {
+    Sequence s;
+    const long long room = static_cast<long long>(p.a.table_pages) << p.page_shift;
+    const int length = p.a.lengths[index];
+    s.length = length < 0 ? 0 : length > room ? static_cast<int>(room) : length;
+    if (tell && s.length != length) report_index(p.a.cache.status, index, kIndexLength, length);
+    s.first_pos = s.length - p.a.tokens;
+    s.base = (p.a.window > 0 ? max(0, s.first_pos - p.a.window + 1) : 0) & ~(kTileKeys - 1);
+    s.units = max(1, static_cast<int>((static_cast<uint32_t>(s.length - s.base) + (1u << p.unit_shift) - 1) >> p.unit_shift));
+    return s;
+}
+// Keys that a token sees: [seen_from, seen_to).
+__device__ __forceinline__ int seen_from(const AttendDev& p, int first_pos, int token) {
+    return p.a.window > 0 ? max(0, first_pos + token - p.a.window + 1) : 0;
+}
+__device__ __forceinline__ int seen_to(const AttendDev& p, int first_pos, int length, int token) {
+    return p.a.causal ? min(length, first_pos + token + 1) : length;
+}
+
+// The token that a row (query head of the group, token) belongs to.
+__device__ __forceinline__ int token_of(const AttendDev& p, int row) { return p.a.tokens == 1 ? 0 : row / p.group; }
+
+// The line of units and its runs (see attend_cut). Every warp that needs it works it out for itself: a lane looks at a range
+// of the sequences. The host has seen to it that there are fewer than 2^31 units.
+struct Line {
+    uint32_t total;
+    Cut cut;
+    int runs;
+    int first, last;    // this lane's sequences
+    uint32_t before;    // units in front of them
+    uint32_t mine;      // units of them
+
+    __device__ __forceinline__ Line(const AttendDev& p, bool tell) {
+        const int lane = threadIdx.x & 31;
+        const int per = (p.a.batch + 31) >> 5;
+        first = min(lane * per, p.a.batch), last = min(first + per, p.a.batch);
+        mine = 0;
+        for (int i = first; i < last; ++i) mine += sequence_of(p, i, tell).units;
+        mine *= p.items;
+        before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, before, o);
+            if (lane >= o) before += up;
+        }
+        total = __shfl_sync(0xFFFFFFFFu, before, 31);
+        before -= mine;
+        cut = attend_cut(total, p.resident, p.least_shift, p.most_waves);
+        runs = cut.across * cut.waves;
+    }
+    __device__ __forceinline__ uint32_t wave_begin(int wave) const { return wave < cut.waves ? total - (total >> wave) : total; }
+    // The units [begin, end) of a run: a wave's are dealt out evenly, rounded down, and no run is empty.
+    __device__ __forceinline__ void range(int run, uint32_t* begin, uint32_t* end) const {
+        const uint32_t across = cut.across, wave = static_cast<uint32_t>(run) / across, i = run - wave * across;
+        const uint32_t from = wave_begin(wave), units = wave_begin(wave + 1) - from, each = units / across, over = units - each * across;
+        *begin = from + each * i + over * i / across;
+        *end = from + each * (i + 1) + over * (i + 1) / across;
+    }
+    __device__ __forceinline__ int run_of(uint32_t unit) const {
+        int wave = 0;
+        while (wave + 1 < cut.waves && unit >= wave_begin(wave + 1)) ++wave;
+        const uint32_t from = wave_begin(wave);
+        return wave * cut.across +
+               static_cast<int>((static_cast<unsigned long long>(unit - from + 1) * cut.across - 1) / (wave_begin(wave + 1) - from));
+    }
+    // The units in front of a sequence. All lanes of the warp.
+    __device__ __forceinline__ uint32_t in_front_of(const AttendDev& p, int sequence) const {
+        const int per = (p.a.batch + 31) >> 5, holder = sequence / per;
+        uint32_t front = __shfl_sync(0xFFFFFFFFu, before, holder);
+        for (int i = holder * per; i < sequence; ++i) front += static_cast<uint32_t>(sequence_of(p, i, false).units) * p.items;
+        return front;
+    }
+    // The sequence that holds a unit, and the units in front of that sequence. All lanes of the warp.
+    __device__ __forceinline__ int sequence_at(const AttendDev& p, uint32_t unit, uint32_t* in_front) const {
+        int sequence = first;
+        uint32_t front = before;
+        const bool here = unit >= before && unit < before + mine;
+        if (here) {
+            for (; sequence < last - 1; ++sequence) {
+                const uint32_t units = static_cast<uint32_t>(sequence_of(p, sequence, false).units) * p.items;
+                if (unit < front + units) break;
+                front += units;
+            }
+        }
+        const uint32_t holder = __ballot_sync(0xFFFFFFFFu, here);
+        const int from = holder ? __ffs(holder) - 1 : 0;
+        *in_front = __shfl_sync(0xFFFFFFFFu, front, from);
+        return __shfl_sync(0xFFFFFFFFu, sequence, from);
+    }
+};
+
+// What those who compute have to know of an item in a run.
+struct Work {
+    int sequence, head, row_tile;  // head -1: there is no more work
+    int length, first_pos;
+    int start, end, tiles;         // keys of this run, steps of 64 of them
+    int whole;                     // all keys of the item are in this run
+    int piece;                     // otherwise: index of its partial result
+};
+
+// The rings between the producer and the warps that compute: stages of keys and values, and announced items.
+template <int kStages>
+struct alignas(16) Pipes {
+    uint4 answer;
+    uint64_t full[kStages], empty[kStages], present[kStages];  // present: bit j says that the stage's key j is there
+    uint64_t work_full[kWorkSlots], work_empty[kWorkSlots], answered;
+    Work works[kWorkSlots];
+
+    // One thread; `readers` arrive for every stage that they are done with, `listeners` for every item.
+    __device__ __forceinline__ void init(int readers, int listeners) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], readers);
+        for (int i = 0; i < kWorkSlots; ++i) mbar_init(&work_full[i], 1), mbar_init(&work_empty[i], listeners);
+        mbar_init(&answered, 1);
+        fence_barrier_init();
+    }
+};
+
+// Asks for the block index of a CTA that was not launched yet, which then never will be: 16 bytes that arrive on `bar`.
+__device__ __forceinline__ void ask_for_cta(uint4* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The block index of an answer, or -1 where every CTA has been launched.
+__device__ __forceinline__ int cta_of(const uint4* answer) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n"
+        ".reg .b128 a;\n"
+        ".reg .pred p;\n"
+        ".reg .b32 y, z, w;\n"
+        "ld.shared.b128 a, [%2];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
+        "selp.u32 %1, 1, 0, p;\n"
+        "mov.u32 %0, 0;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, a;\n"
+        "}\n"
+        : "=&r"(x), "=&r"(got)
+        : "r"(smem_u32(answer))
+        : "memory");
+    return got ? static_cast<int>(x) : -1;
+}
+
+
+// A wait that runs out is reported; what follows is computed from whatever is there, and nothing more is requested.
+__device__ __forceinline__ void stalled(const AttendDev& p, int who, int at) {
+    report(p.a.cache.status, kErrTimeout, who, kPhasePipeline, at);
+}
+
+// The producer: a whole warp. A stage of the ring is kPieces * 16 bytes for each of 64 keys, then the same for values. Boxes
+// are a page's slots, at most 64; kApart: of one column block of 128 bytes each, so that a block's 64 rows follow one another.
+template <int kStages, int kPieces, bool kApart>
+__device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes<kStages>& pipes, long long deadline, bool leader) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kBytes = kTileKeys * kPieces * 16;
+    constexpr int kBlocks = kApart ? (kPieces + 7) / 8 : 1;  // boxes along a row
+    const Line line(p, blockIdx.x == 0);
+    const int box_keys = min(kTileKeys, 1 << p.page_shift), boxes = kTileKeys / box_keys;
+    const int slot_mask = (1 << p.page_shift) - 1;
+    int stage = 0, slot = 0, run = blockIdx.x;
+    uint32_t parity = 1, slot_parity = 1, answer_parity = 0;  // the first lap of a ring waits for nothing
+    bool failed = false;
+    auto announce = [&](const Work& work) {
+        if (!mbar_wait_warp(&pipes.work_empty[slot], slot_parity, deadline) && !failed) {
+            failed = true;
+            if (leader) stalled(p, 0, run);
+        }
+        if (leader) {
+            pipes.works[slot] = work;
+            mbar_arrive(&pipes.work_full[slot]);
+        }
+        if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
+    };
+    // Where the next step is: a run, an item in it, a step of 64 keys in that. Pages are looked up a step ahead of their
+    // use, across items and runs, 32 entries of the table at once: lane j holds entry `window` + j.
+    uint32_t unit = 0, last_unit = 0;
+    int sequence = 0, index = 0, first = 0, units = 0, lo = 0, tile = 0, window = 0, pages = 0;
+    Sequence s{};
+    Work work{};
+    auto look_up = [&](int from) {
+        window = from;
+        const int entry = from + lane;
+        pages = entry << p.page_shift < work.end ? p.a.page_table[sequence * p.a.table_stride + entry] : INT_MIN;
+    };
+    auto begin_item = [&]() {
+        units = min(static_cast<int>(last_unit - unit), s.units - first);
+        work.sequence = sequence, work.length = s.length, work.first_pos = s.first_pos;
+        work.head = p.row_tiles == 1 ? index : index / p.row_tiles, work.row_tile = index - work.head * p.row_tiles;
+        const int first_row = work.row_tile * p.tile_rows, last_row = min(first_row + p.tile_rows, p.rows) - 1;
+        lo = seen_from(p, s.first_pos, token_of(p, first_row));
+        const int hi = seen_to(p, s.first_pos, s.length, token_of(p, last_row));
+        work.whole = units == s.units;
+        work.piece = run * 2 + (first == 0);  // a run has at most one that began before it and one that goes on
+        work.start = max(s.base + (first << p.unit_shift), lo & ~(kTileKeys - 1));  // first is 0 if units are whole items
+        work.end = first + units == s.units ? hi : min(hi, s.base + ((first + units) << p.unit_shift));
+        work.tiles = work.end > work.start ? (work.end - work.start + kTileKeys - 1) / kTileKeys : 0;
+        tile = 0;
+        if (work.tiles > 0) look_up(work.start >> p.page_shift);
+    };
+    auto begin_run = [&]() -> bool {
+        if (run < 0 || run >= line.runs) return false;
+        if (leader) {
+            fence_proxy_async();  // the last answer has been read
+            mbar_expect_tx(&pipes.answered, sizeof(pipes.answer));
+            ask_for_cta(&pipes.answer, &pipes.answered);
+        }
+        line.range(run, &unit, &last_unit);
+        uint32_t in_front;
+        sequence = line.sequence_at(p, unit, &in_front);
+        s = sequence_of(p, sequence, false);
+        index = static_cast<int>((unit - in_front) / static_cast<uint32_t>(s.units));  // key head * row tiles + row tile
+        first = static_cast<int>(unit - in_front) - index * s.units;
+        begin_item();
+        return true;
+    };
+    auto advance = [&]() -> bool {
+        if (++tile < work.tiles) {
+            const int entry = (work.start + tile * kTileKeys) >> p.page_shift;
+            if (entry >= window + 32) look_up(entry);
+            return true;
+        }
+        unit += units;
+        if (unit < last_unit) {
+            first = 0;
+            if (++index == p.items) index = 0, s = sequence_of(p, ++sequence, false);
+            begin_item();
+            return true;
+        }
+        if (!mbar_wait_warp(&pipes.answered, answer_parity, deadline)) {
+            if (leader) stalled(p, 2, run);
+            return false;
+        }
+        answer_parity ^= 1;
+        run = cta_of(&pipes.answer);
+        __syncwarp();
+        return begin_run();
+    };
+    bool more = begin_run();
+    while (more) {
+        const Work now = work;
+        const int now_tile = tile, now_lo = lo;
+        const int now_pages = pages, now_window = window;
+        more = advance();
+        if (now_tile == 0) announce(now);
+        if (now.tiles == 0) continue;
+        const int key0 = now.start + now_tile * kTileKeys;
+        // Lane j: the page of box j, INT_MIN where no key of the box is in the run.
+        const int entry = ((key0 + lane * box_keys) >> p.page_shift) - now_window;
+        int page = __shfl_sync(0xFFFFFFFFu, now_pages, entry & 31);
+        const bool in_pool = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.a.cache.pages);
+        uint64_t present = ~0ull;
+        if (!__all_sync(0xFFFFFFFFu, in_pool || lane >= boxes) || now.end - key0 < kTileKeys) {
+            if (lane >= boxes || key0 + lane * box_keys >= now.end) page = INT_MIN;
+            else if (!in_pool && key0 + (lane + 1) * box_keys > now_lo)
+                report_index(p.a.cache.status, now.sequence, kIndexPage, page);
+            const uint32_t there = __ballot_sync(0xFFFFFFFFu, in_pool && page != INT_MIN);
+            if (!in_pool || page == INT_MIN) page = p.a.cache.pages;  // past the pool's end: the box is filled with zeros
+            const uint64_t box_bits = box_keys == 64 ? ~0ull : (1ull << box_keys) - 1;
+            present = 0;
+            for (int j = 0; j < boxes; ++j)
+                if (there >> j & 1) present |= box_bits << (j * box_keys);
+            if (now.end - key0 < kTileKeys) present &= (1ull << (now.end - key0)) - 1;
+        }
+        if (!mbar_wait(&pipes.empty[stage], parity, deadline) && !failed) {
+            failed = true;
+            if (leader) stalled(p, 1, now_tile);
+        }
+        __syncwarp();
+        uint8_t* to = ring + stage * 2 * kBytes;
+        uint64_t* bar = &pipes.full[stage];
+        if (leader) {
+            pipes.present[stage] = present;
+            if (failed) mbar_arrive(bar);
+            else mbar_expect_tx(bar, 2 * kBytes);
+        }
+        for (int j = 0; j < boxes; ++j) {
+            const int from = __shfl_sync(0xFFFFFFFFu, page, j);
+            const int at = (key0 + j * box_keys) & slot_mask;
+            const int box = j * box_keys * (kApart ? 128 : kPieces * 16);
+            if (leader && !failed) {
+#pragma unroll
+                for (int c = 0; c < kBlocks; ++c) {
+                    tma_load_5d(to + c * kTileKeys * 128 + box, &p.tm_k, bar, 0, at, c, now.head, from, kEvictNormal);
+                    tma_load_5d(to + kBytes + c * kTileKeys * 128 + box, &p.tm_v, bar, 0, at, c, now.head, from, kEvictNormal);
+                }
+            }
+        }
+        if (++stage == kStages) stage = 0, parity ^= 1;
+    }
+    Work none;
+    none.head = -1;
+    announce(none);
+}
+
+// Four elements of a finished row: the sum over its keys, divided by the sum of their weights.
+template <typename T>
+__device__ __forceinline__ void finish_row(const AttendDev& p, int sequence, int head, int row, int d, const float4& sum,
+                                           float top, float l, float value_scale) {
+    const float inv = l == 0.f ? 0.f : value_scale / l;
+    const int token = token_of(p, row), query_head = head * p.group + row - token * p.group;
+    T* out = static_cast<T*>(p.a.out) + sequence * p.a.out_strides[0] + token * p.a.out_strides[1] +
+             query_head * p.a.out_strides[2] + d;
+    *reinterpret_cast<uint2*>(out) = make_uint2(narrow2<T>(sum.x * inv, sum.y * inv), narrow2<T>(sum.z * inv, sum.w * inv));
+    if (p.a.lse != nullptr && d == 0)
+        p.a.lse[(static_cast<size_t>(sequence) * p.a.tokens + token) * p.a.q_heads + query_head] =
+            l == 0.f ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
+}
+
+}  // namespace dlm

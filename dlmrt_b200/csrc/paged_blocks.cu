@@ -1,0 +1,404 @@
+// Attention over the paged cache for blocks of tokens: more rows share a key head's keys than a warp's tile holds (a block of
+// 32 tokens of four query heads each is 128), so that a step's arithmetic is worth a 128-row tile in tensor memory.
+//
+//   warps 0-3  a row of the tile each thread: Q into shared memory, then for every step of 64 keys the row of scores out of
+//              tensor memory, mask, maximum, weights exp2(s - m) back into tensor memory over the scores, and their sum.
+//   warp 4     the producer (paged_attend.cuh).
+//   warp 5     issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory, V as it
+//              lies, its 64 keys down the rows). S has two buffers: the next step's scores are computed under this one's
+//              softmax.
+//
+// m is the running maximum when O was last rescaled: O, which lives in tensor memory, is multiplied by exp2(m - m') only when
+// some row's maximum has grown by more than 8 (a factor of 256, which the weights and their FP32 sum have room for).
+//
+// One CTA an SM; shared memory holds 3 to 6 steps of 64 keys. A step is 2 * 128 * 64 * head_dim multiply-adds (512 cycles of the
+// tensor pipe at 128) and 64 exponentials for each of 128 threads, which is what bounds it once keys come fast enough.
+#include "paged_attend.cuh"
+
+namespace dlm {
+
+namespace {
+
+constexpr int kSoftmaxThreads = 128;
+constexpr int kBlockThreads = 192;
+constexpr int kProducerWarp = 4, kIssuerWarp = 5;
+constexpr float kRescaleAbove = 8.f;
+
+template <int D>
+struct BlockSmem {
+    static constexpr int kStages = D == 256 ? 2 : D == 128 ? 4 : 6;
+    static constexpr int kBytes = kTileKeys * D * 2;          // keys, or values, of a stage
+    static constexpr int kRing = kStages * 2 * kBytes;
+    static constexpr int kQueries = kBlockRows * D * 2;
+    static constexpr int kAll = kRing + kQueries + 1024;      // the ring begins at a multiple of 1024
+    static constexpr uint32_t kColumns = D == 256 ? 512 : 256;  // of tensor memory: O, then two S of 64
+};
+
+// Instruction descriptor of kind::f16, see umma_idesc_bf16: T is BF16 or FP16, B is K-major, or MN-major where `b_mn`.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
+    const uint32_t format = std::is_same<T, __half>::value ? 0 : 1;
+    return (1u << 4) | (format << 7) | (format << 10) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Descriptor of an MN-major operand under the 128-byte swizzle: rows of 64 elements along N, 8 k's a group of 1024 bytes;
+// `blocks` bytes from one 64 elements of N to the next.
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t smem, uint32_t blocks) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem & 0x3FFFF) >> 4);
+    d |= static_cast<uint64_t>(blocks >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+// D[tmem] += A[tmem] * B[smem], A being 128 rows of 16 k's in 8 columns of 16-bit pairs.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, 1, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// All-ones in the 16-bit halves of a word that are infinite or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+    return __vcmpeq2(w & kExponent, kExponent);
+}
+
+}  // namespace
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_constant__ AttendDev p) {
+    using Shared = BlockSmem<D>;
+    constexpr int kStages = Shared::kStages, kBytes = Shared::kBytes;
+    constexpr int kBlockBytes = kTileKeys * 128;  // 64 keys of a column block of 64 elements
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* queries = smem + Shared::kRing;
+    __shared__ Pipes<kStages> pipes;
+    // queries written; scores computed (two buffers); weights written; a step's values consumed; a side step of the warps 0-3
+    __shared__ uint64_t q_full, s_full[2], p_full[2], pv_done, aside;
+    __shared__ uint32_t tmem_base;
+
+    const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    const bool leader = elect_one();
+    if (warp == kProducerWarp && leader) {
+        pipes.init(1, kSoftmaxThreads / 32 + 1);
+        mbar_init(&q_full, kSoftmaxThreads);
+        for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kSoftmaxThreads);
+        mbar_init(&pv_done, 1);
+        mbar_init(&aside, kSoftmaxThreads);
+        fence_barrier_init();
+        tma_prefetch_descriptor(&p.tm_k);
+        tma_prefetch_descriptor(&p.tm_v);
+    }
+    if (warp == kIssuerWarp) tmem_alloc(&tmem_base, Shared::kColumns);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = uniform(tmem_base);
+    const uint32_t tmem_s = tmem + D;  // S of step n: + (n & 1) * 64; its weights take the first 32 of these columns
+    const long long deadline = globaltimer() + kDefaultTimeoutNs;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    if (warp == kProducerWarp) {
+        produce<kStages, D / 8, true>(p, smem, pipes, deadline, leader);
+    } else if (warp == kIssuerWarp) {
+        // -- the issuer: a whole warp on uniform values, one lane issuing ------------------------------------------------
+        constexpr uint32_t kIdescS = idesc_f16<T>(kBlockRows, kTileKeys, false), kIdescO = idesc_f16<T>(kBlockRows, D, true);
+        const uint64_t q_desc = umma_desc_k128(queries);
+        int stage = 0, slot = 0, next_stage = 0;
+        uint32_t parity = 0, slot_parity = 0, q_parity = 0, step = 0;
+        auto wait = [&](uint64_t* bar, uint32_t phase, int who, int at) {
+            if (!mbar_wait_warp(bar, phase, deadline) && leader) stalled(p, who, at);
+            tcgen05_fence_after();
+        };
+        while (true) {
+            const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
+            if (!announced) {
+                if (leader) stalled(p, 5, slot);
+                break;
+            }
+            const int head = pipes.works[slot].head, tiles = pipes.works[slot].tiles;
+            __syncwarp();
+            if (leader) mbar_arrive(&pipes.work_empty[slot]);
+            if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
+            if (head < 0) break;
+            wait(&q_full, q_parity, 6, tiles);
+            q_parity ^= 1;
+            auto scores = [&](uint32_t n) {  // of step n, whose keys are the next stage's
+                wait(&pipes.full[next_stage], parity, 7, n);
+                const uint32_t keys = smem_u32(smem) + next_stage * 2 * kBytes;
+                const uint64_t k_desc = (q_desc & 0xFFFFFFFF00000000ull) | (umma_desc_k128(smem) & 0xFFFF0000u) | ((keys & 0x3FFFF) >> 4);
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_bf16(tmem_s + (n & 1) * 64, q_desc + (k / 4) * (kBlockRows * 128 >> 4) + (k % 4) * 2,
+                                  k_desc + (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, kIdescS, k != 0);
+                    umma_commit(&s_full[n & 1]);
+                }
+                if (++next_stage == kStages) next_stage = 0, parity ^= 1;
+            };
+            if (tiles > 0) scores(step);
+            for (int tile = 0; tile < tiles; ++tile, ++step) {
+                if (tile + 1 < tiles) {
+                    // The other buffer held the weights of the step before, which have to have been consumed.
+                    if (tile > 0) wait(&pv_done, (step - 1) & 1, 8, tile);
+                    scores(step + 1);
+                }
+                wait(&p_full[step & 1], step >> 1 & 1, 9, tile);
+                const uint32_t values = smem_u32(smem) + stage * 2 * kBytes + kBytes;
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < kTileKeys / 16; ++k)
+                        umma_f16_ts(tmem, tmem_s + (step & 1) * 64 + k * 8, umma_desc_mn128(values + k * 2048, kBlockBytes), kIdescO);
+                    umma_commit(&pipes.empty[stage]);
+                    umma_commit(&pv_done);
+                }
+                if (++stage == kStages) stage = 0;
+            }
+        }
+    } else {
+        // -- a row of the tile each thread -----------------------------------------------------------------------------
+        const int r = threadIdx.x;
+        const uint32_t mine = static_cast<uint32_t>(warp * 32) << 16;  // this warp's lanes of tensor memory
+        const float scale = p.a.scale * kLog2e;
+        int stage = 0, slot = 0;
+        uint32_t slot_parity = 0, step = 0, aside_parity = 0;
+        auto wait = [&](uint64_t* bar, uint32_t phase, int who, int at) {
+            if (!mbar_wait(bar, phase, deadline)) stalled(p, who, at);
+            __syncwarp();
+            tcgen05_fence_after();
+        };
+        while (true) {
+            const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
+            if (!announced) {
+                if (leader) stalled(p, 10, slot);
+                break;
+            }
+            const Work item = pipes.works[slot];
+            __syncwarp();
+            if (leader) mbar_arrive(&pipes.work_empty[slot]);
+            if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
+            if (item.head < 0) break;
+            const int first_row = item.row_tile * kBlockRows, row = first_row + r, last_row = min(first_row + kBlockRows, p.rows) - 1;
+            const int token = token_of(p, min(row, last_row));
+            const int from = seen_from(p, item.first_pos, token), to = seen_to(p, item.first_pos, item.length, token);
+            const int all_from = seen_from(p, item.first_pos, token_of(p, last_row));                     // from here on every row sees
+            const int all_to = seen_to(p, item.first_pos, item.length, token_of(p, first_row));         // the keys, up to here
+            {   // Q, swizzled as TMA would; the products that read the last item's are done
+                const T* q = static_cast<const T*>(p.a.q) + item.sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
+                             static_cast<long long>(item.head * p.group + min(row, last_row) - token * p.group) * p.a.q_strides[2];
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    const uint4 v = row <= last_row ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(queries + (c / 8) * (kBlockRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16) = v;
+                }
+                fence_proxy_async();
+                mbar_arrive(&q_full);
+            }
+            {
+                uint32_t zero[32] = {};
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) tmem_store_32(tmem + mine + c * 32, zero);
+                tmem_store_wait();
+            }
+            float m = -INFINITY, l = 0.f;
+            for (int tile = 0; tile < item.tiles; ++tile, ++step) {
+                const uint32_t s_at = tmem_s + mine + (step & 1) * 64;
+                uint32_t raw[64];
+                wait(&s_full[step & 1], step >> 1 & 1, 11, tile);
+                tmem_load_32(s_at, raw);
+                tmem_load_32(s_at + 32, raw + 32);
+                tmem_load_wait();
+                float (&s)[64] = reinterpret_cast<float(&)[64]>(raw);
+                const int key0 = item.start + tile * kTileKeys;
+                const uint64_t present = pipes.present[stage];
+                const bool by_row = key0 < all_from || key0 + kTileKeys > all_to;  // rows see different keys of this step
+                const bool edge = by_row || present != ~0ull;
+#pragma unroll
+                for (int j = 0; j < 64; ++j) s[j] *= scale;
+                if (edge) {
+                    const int lo = from - key0, hi = to - key0;
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (j < lo || j >= hi || !(present >> j & 1)) s[j] = -INFINITY;
+                }
+                float top4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int j = 4; j < 64; ++j) top4[j & 3] = fmaxf(top4[j & 3], s[j]);
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                if (__any_sync(0xFFFFFFFFu, top > m + kRescaleAbove || (m == -INFINITY && top > m))) {
+                    const float n = fmaxf(m, top);
+                    const float f = m == n ? 1.f : exp2_approx(m - n);  // 0 where nothing was there
+                    l *= f, m = n;
+                    if (tile > 0) {
+                        wait(&pv_done, (step - 1) & 1, 12, tile);
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_load_32(tmem + mine + c * 32, o);
+                            tmem_load_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_store_32(tmem + mine + c * 32, o);
+                        }
+                    }
+                }
+                const float sub = m == -INFINITY ? 0.f : m;
+                float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t weights[32];
+#pragma unroll
+                for (int j = 0; j < 64; j += 2) {
+                    s[j] = exp2_approx(s[j] - sub), s[j + 1] = exp2_approx(s[j + 1] - sub);
+                    sum4[j & 3] += s[j], sum4[(j + 1) & 3] += s[j + 1];
+                    weights[j / 2] = narrow2<T>(s[j], s[j + 1]);
+                }
+                l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+                tmem_store_32(s_at, weights);
+                if (edge) {
+                    // Values that are not finite, in keys that some rows see and others do not, or that are not there: 0 * inf
+                    // would reach the result. Their keys are found by every warp for itself.
+                    uint8_t* values = smem + stage * 2 * kBytes + kBytes;
+                    auto piece = [&](int key, int c) {  // 16 bytes of a key's row
+                        return reinterpret_cast<uint4*>(values + (c / 8) * kBlockBytes + key * 128 + ((c % 8) ^ (key & 7)) * 16);
+                    };
+                    uint64_t bad = 0;
+#pragma unroll 1
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = lane + 32 * i;
+                        bool any = false;
+                        if (by_row || !(present >> key & 1)) {
+                            for (int c = 0; c < D / 8; ++c) {
+                                const uint4 v = *piece(key, c);
+                                any |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
+                            }
+                        }
+                        bad |= static_cast<uint64_t>(__ballot_sync(0xFFFFFFFFu, any)) << (32 * i);
+                    }
+                    if (bad != 0) {  // the same in all four warps
+                        uint64_t weightless = 0;  // keys whose weight is zero here: 0 * inf is NaN
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) weightless |= static_cast<uint64_t>(s[j] == 0.f) << j;
+                        if (tile > 0) wait(&pv_done, (step - 1) & 1, 13, tile);
+#pragma unroll 1
+                        for (uint64_t left = bad; left != 0; left &= left - 1) {
+                            const int key = __ffsll(static_cast<long long>(left)) - 1;
+                            const bool see = key0 + key >= from && key0 + key < to && (present >> key & 1);
+#pragma unroll 1
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_load_32(tmem + mine + c * 32, o);
+                                tmem_load_wait();
+#pragma unroll
+                                for (int j = 0; j < 32; j += 2) {
+                                    const uint32_t w = reinterpret_cast<const uint32_t*>(piece(key, c * 4 + j / 8))[j / 2 % 4];
+                                    const float2 v = widen2<T>(w);
+                                    const float none = weightless >> key & 1 ? NAN : 1.f;
+                                    if (see && !isfinite(v.x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + v.x * none);
+                                    if (see && !isfinite(v.y)) o[j + 1] = __float_as_uint(__uint_as_float(o[j + 1]) + v.y * none);
+                                }
+                                tmem_store_32(tmem + mine + c * 32, o);
+                            }
+                            tmem_store_wait();
+                        }
+                        mbar_arrive(&aside);  // everybody has read them
+                        wait(&aside, aside_parity, 14, tile);
+                        aside_parity ^= 1;
+                        for (uint64_t left = bad; left != 0; left &= left - 1) {
+                            const int key = __ffsll(static_cast<long long>(left)) - 1;
+                            if ((key & 3) != warp) continue;
+                            for (int c = lane; c < D / 8; c += 32) {
+                                uint4 v = *piece(key, c);
+                                v.x &= ~not_finite<T>(v.x), v.y &= ~not_finite<T>(v.y), v.z &= ~not_finite<T>(v.z), v.w &= ~not_finite<T>(v.w);
+                                *piece(key, c) = v;
+                            }
+                        }
+                        fence_proxy_async();
+                    }
+                }
+                tmem_store_wait();
+                tcgen05_fence_before();
+                mbar_arrive(&p_full[step & 1]);
+                if (++stage == kStages) stage = 0;
+            }
+            // -- the row's result ---------------------------------------------------------------------------------------
+            if (item.tiles > 0) wait(&pv_done, (step - 1) & 1, 15, item.tiles);
+            const int piece = item.piece * p.rows_cap + r;
+            if (!item.whole && row <= last_row) *reinterpret_cast<float2*>(p.stats + piece * 2) = make_float2(m, l);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_load_32(tmem + mine + c * 32, o);
+                tmem_load_wait();
+                const float (&v)[32] = reinterpret_cast<const float(&)[32]>(o);
+                if (row <= last_row && item.whole) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        finish_row<T>(p, item.sequence, item.head, row, c * 32 + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]), m, l, 1.f);
+                } else if (row <= last_row) {
+                    float4* out = reinterpret_cast<float4*>(p.partial + static_cast<size_t>(piece) * D + c * 32);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) out[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                }
+                __syncwarp();
+            }
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == kIssuerWarp) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem, Shared::kColumns);
+    }
+}
+
+int launch_blocks(const AttendDev& p, const LaunchOpts& o) {
+    void* args[] = {const_cast<AttendDev*>(&p)};
+    auto run = [&](auto t, auto dim) {
+        constexpr int kDim = decltype(dim)::value;
+        return launch_kernel<blocks_kernel<decltype(t), kDim>>(dim3(p.grid), dim3(kBlockThreads), BlockSmem<kDim>::kAll, args, o);
+    };
+    auto by_dim = [&](auto t) {
+        switch (p.a.cache.head_dim) {
+            case 64: return run(t, std::integral_constant<int, 64>{});
+            case 128: return run(t, std::integral_constant<int, 128>{});
+            default: return run(t, std::integral_constant<int, 256>{});
+        }
+    };
+    return p.a.type == DLM_F16 ? by_dim(__half{}) : by_dim(__nv_bfloat16{});
+}
+
+}  // namespace dlm

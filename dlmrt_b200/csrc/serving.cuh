@@ -20,7 +20,8 @@ __device__ __forceinline__ void report_index(int* status, int row, int kind, int
     }
 }
 
-constexpr int kRowTile = 16;   // rows of an item: the M of its matrix instructions
+constexpr int kRowTile = 16;     // rows of an item: the M of its matrix instructions
+constexpr int kBlockRows = 128;  // the same in the kernel for blocks of tokens
 constexpr int kUnitShift = 6, kTileKeys = 1 << kUnitShift;  // keys of a step, and of the units that items are cut into
 
 struct alignas(64) AttendDev {
@@ -31,11 +32,14 @@ struct alignas(64) AttendDev {
     int page_shift;
     int group;         // query heads of a key head
     int rows;          // tokens * group rows share a key head's keys
-    int row_tiles;     // of kRowTile rows
-    int rows_cap;      // rows of a tile that exist: min(kRowTile, rows)
+    int tile_rows;     // rows of an item: kRowTile, or kBlockRows in the kernel for blocks of tokens
+    int row_tiles;     // of tile_rows rows
+    int rows_cap;      // rows of a tile that exist: min(tile_rows, rows)
+    int blocks;        // the kernel for blocks of tokens takes this call
     int items;         // of one sequence: key heads * row tiles
     int unit_shift;    // log2 of the keys of a unit: kUnitKeys, or more than there are where items are not split
     int least_shift;   // log2 of the units of a run of a short line
+    int most_waves;
     int resident;      // CTAs that the GPU holds
     int grid;          // runs that there are at most
     int by_item;       // the join has a block for each item, not for each run
@@ -48,11 +52,9 @@ struct alignas(64) AttendDev {
 struct Cut {
     int across, waves;
 };
-constexpr int kMostWaves = 5;
-
-__host__ __device__ inline Cut attend_cut(uint32_t total, int resident, int least_shift) {
+__host__ __device__ inline Cut attend_cut(uint32_t total, int resident, int least_shift, int most_waves) {
     Cut c{resident, 1};
-    while (c.waves < kMostWaves && (total >> c.waves) >= 2u * static_cast<uint32_t>(resident)) ++c.waves;
+    while (c.waves < most_waves && (total >> c.waves) >= 2u * static_cast<uint32_t>(resident)) ++c.waves;
     const uint32_t most = (total + (1u << least_shift) - 1) >> least_shift;
     if (c.waves == 1 && most < static_cast<uint32_t>(resident)) c.across = most < 1 ? 1 : static_cast<int>(most);
     return c;
@@ -60,6 +62,7 @@ __host__ __device__ inline Cut attend_cut(uint32_t total, int resident, int leas
 
 int launch_append(const DlmAppend& p, int page_shift, const LaunchOpts& o);
 int launch_attend(const AttendDev& p, const LaunchOpts& o);
+int launch_blocks(const AttendDev& p, const LaunchOpts& o);  // its first half, without the join
 int attend_ctas_per_sm(int type, int cache_type, int head_dim);
 int launch_adapters(const DlmAdapters& p, const LaunchOpts& o);
 
