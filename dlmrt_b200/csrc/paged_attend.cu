@@ -450,10 +450,10 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     }
 }
 
-// Joins the partial results of an item that lies in several runs: item blockIdx.x, or (with more items than runs) the one that
-// begins in run blockIdx.x and goes on. For each of its rows, out = sum_c exp2(m_c - m) o_c / sum_c exp2(m_c - m) l_c. The rows
-// are shared by gridDim.y blocks and their elements by gridDim.z; in a block every thread has four elements of a row, and
-// threads that are left over take further partial results of the same rows.
+// Joins the partial results of an item that lies in several runs (see SplitItem): for each of its rows,
+// out = sum_c exp2(m_c - m) o_c / sum_c exp2(m_c - m) l_c. The rows are shared by gridDim.y blocks and their elements by
+// gridDim.z; in a block every thread has four elements of a row, and threads that are left over take further partial results
+// of the same rows.
 constexpr int kJoinMostThreads = 1024;
 constexpr int kJoinAhead = 4;  // partial results that a thread has on the way at once
 
@@ -462,29 +462,9 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
     extern __shared__ float4 sums[];  // [lines][across], then stats[lines]
     float2* stats = reinterpret_cast<float2*>(sums + blockDim.x);
     const int across = D / 4 / gridDim.z, lines = blockDim.x / across;  // threads along a row, and how often
-    // The lengths are older than the kernel in front, whose blocks waited for them before this one could start.
-    const Line line(p, false);
-    int sequence, index, run, last;
-    uint32_t begin, run_begin, run_end;
-    if (p.by_item) {
-        sequence = blockIdx.x / p.items, index = blockIdx.x - sequence * p.items;
-        const Sequence s = sequence_of(p, sequence, false);
-        begin = line.in_front_of(p, sequence) + index * s.units;
-        run = line.run_of(begin), last = line.run_of(begin + s.units - 1);
-    } else {
-        run = blockIdx.x;
-        if (run + 1 >= line.runs) return;
-        line.range(run, &run_begin, &run_end);
-        uint32_t in_front;
-        sequence = line.sequence_at(p, run_end - 1, &in_front);
-        const Sequence s = sequence_of(p, sequence, false);
-        index = static_cast<int>((run_end - 1 - in_front) / static_cast<uint32_t>(s.units));
-        begin = in_front + index * s.units;
-        last = line.run_of(begin + s.units - 1);
-        if (begin < run_begin) return;
-    }
-    if (last == run) return;
-    const int head = index / p.row_tiles, first_row = (index - head * p.row_tiles) * p.tile_rows;
+    const SplitItem item(p, blockIdx.x);
+    if (!item.split) return;
+    const int run = item.run, last = item.last, head = item.head, first_row = item.row_tile * kRowTile;
     pdl_wait();
     pdl_launch_dependents();
     const int per_block = (p.rows_cap + gridDim.y - 1) / gridDim.y;
@@ -545,16 +525,14 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
             __syncthreads();
         }
         if (takes_part && (deep == 1 || y == 0))
-            finish_row<T>(p, sequence, head, first_row + r, x * 4, sum, top, l, value_scale);
+            finish_row<T>(p, item.sequence, head, first_row + r, x * 4, sum, top, l, value_scale);
     }
 }
 
 template <typename T, int D, bool kCodes>
 static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
     void* args[] = {const_cast<AttendDev*>(&p)};
-    const int rc = p.blocks ? launch_blocks(p, o)
-                            : launch_kernel<attend_kernel<T, D, kCodes>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes>::kBytes,
-                                                                         args, o);
+    const int rc = launch_kernel<attend_kernel<T, D, kCodes>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes>::kBytes, args, o);
     if (rc != 0 || p.partial == nullptr) return rc;
     // With fewer items than runs an item may have hundreds of partial results: large blocks, one for a quarter of each row (293
     // partial results of a row: 7 us in blocks of a whole row, all of it latency). Otherwise it has two or three, and most blocks
@@ -585,6 +563,7 @@ static int by_type(int type, int cache_type, int head_dim, F f) {
 }
 
 int launch_attend(const AttendDev& p, const LaunchOpts& o) {
+    if (p.blocks) return launch_blocks(p, o);
     return by_type(p.a.type, p.a.cache.type, p.a.cache.head_dim, [&](auto t, auto dim, auto codes) {
         return launch_attend_t<decltype(t), decltype(dim)::value, decltype(codes)::value>(p, o);
     });

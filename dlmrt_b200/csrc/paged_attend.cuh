@@ -318,6 +318,38 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
     announce(none);
 }
 
+// What a block of a join looks at: an item that lies in several runs. Block `b` has item b, or (with more items than runs) the
+// item that begins in run b and goes on. All threads; lengths are older than the kernel in front, whose blocks waited for them
+// before a dependent launch could start, so this need not wait.
+struct SplitItem {
+    bool split;
+    int sequence, head, row_tile, run, last;  // its runs are [run, last]
+
+    __device__ __forceinline__ SplitItem(const AttendDev& p, int b) : split(false) {
+        const Line line(p, false);
+        int index;
+        if (p.by_item) {
+            sequence = b / p.items, index = b - sequence * p.items;
+            const Sequence s = sequence_of(p, sequence, false);
+            const uint32_t begin = line.in_front_of(p, sequence) + index * s.units;
+            run = line.run_of(begin), last = line.run_of(begin + s.units - 1);
+            split = last != run;
+        } else {
+            run = b;
+            if (run + 1 >= line.runs) return;
+            uint32_t run_begin, run_end, in_front;
+            line.range(run, &run_begin, &run_end);
+            sequence = line.sequence_at(p, run_end - 1, &in_front);
+            const Sequence s = sequence_of(p, sequence, false);
+            index = static_cast<int>((run_end - 1 - in_front) / static_cast<uint32_t>(s.units));
+            const uint32_t begin = in_front + index * s.units;
+            last = line.run_of(begin + s.units - 1);
+            split = begin >= run_begin && last != run;
+        }
+        head = index / p.row_tiles, row_tile = index - head * p.row_tiles;
+    }
+};
+
 // Four elements of a finished row: the sum over its keys, divided by the sum of their weights.
 template <typename T>
 __device__ __forceinline__ void finish_row(const AttendDev& p, int sequence, int head, int row, int d, const float4& sum,

@@ -89,6 +89,25 @@ __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* r)
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 16-byte piece `c` of row `r` of a tile of 128 rows, in column blocks of 128 bytes under the 128-byte swizzle.
+__device__ __forceinline__ uint4* tile_piece(uint8_t* tile, int r, int c) {
+    return reinterpret_cast<uint4*>(tile + (c / 8) * (kBlockRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16);
+}
+
+// The address of row `row` of a [sequence, token, head, D] tensor, in lane order: every lane passes its own row's, and reads
+// rows in turn, D / 8 lanes of 16 bytes each.
+template <int D, typename F>
+__device__ __forceinline__ void by_rows(const void* mine, F f) {
+    constexpr int kAcross = D / 8, kAtOnce = 32 / kAcross;
+    const int lane = threadIdx.x & 31;
+    const unsigned long long at = reinterpret_cast<unsigned long long>(mine);
+#pragma unroll
+    for (int i = 0; i < 32 / kAtOnce; ++i) {
+        const int r = i * kAtOnce + lane / kAcross;
+        f(i, r, lane % kAcross, reinterpret_cast<uint8_t*>(__shfl_sync(0xFFFFFFFFu, at, r)));
+    }
+}
+
 // All-ones in the 16-bit halves of a word that are infinite or NaN.
 template <typename T>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
@@ -218,14 +237,16 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
             const int from = seen_from(p, item.first_pos, token), to = seen_to(p, item.first_pos, item.length, token);
             const int all_from = seen_from(p, item.first_pos, token_of(p, last_row));                     // from here on every row sees
             const int all_to = seen_to(p, item.first_pos, item.length, token_of(p, first_row));         // the keys, up to here
-            {   // Q, swizzled as TMA would; the products that read the last item's are done
+            const int query_head = item.head * p.group + min(row, last_row) - token * p.group;
+            {   // Q, swizzled as TMA would, a warp its own 32 rows; the products that read the last item's are done
                 const T* q = static_cast<const T*>(p.a.q) + item.sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
-                             static_cast<long long>(item.head * p.group + min(row, last_row) - token * p.group) * p.a.q_strides[2];
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const uint4 v = row <= last_row ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(queries + (c / 8) * (kBlockRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16) = v;
-                }
+                             query_head * p.a.q_strides[2];
+                constexpr int kReads = D / 8;
+                uint4 v[kReads];
+                by_rows<D>(row <= last_row ? q : nullptr, [&](int i, int, int c, const uint8_t* at) {
+                    v[i] = at != nullptr ? reinterpret_cast<const uint4*>(at)[c] : make_uint4(0, 0, 0, 0);
+                });
+                by_rows<D>(nullptr, [&](int i, int at, int c, const uint8_t*) { *tile_piece(queries, warp * 32 + at, c) = v[i]; });
                 fence_proxy_async();
                 mbar_arrive(&q_full);
             }
@@ -356,23 +377,42 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
             }
             // -- the row's result ---------------------------------------------------------------------------------------
             if (item.tiles > 0) wait(&pv_done, (step - 1) & 1, 15, item.tiles);
-            const int piece = item.piece * p.rows_cap + r;
-            if (!item.whole && row <= last_row) *reinterpret_cast<float2*>(p.stats + piece * 2) = make_float2(m, l);
+            // Parts of a row go out with rows side by side, [element / 4][row], a finished row by way of the tile of queries, whose
+            // products are done: a thread's own row would be 32 lanes' stores far apart (5 us an item instead of 1.5).
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (row <= last_row) {
+                if (!item.whole)
+                    *reinterpret_cast<float2*>(p.stats + (static_cast<size_t>(item.piece) * p.rows_cap + r) * 2) = make_float2(m, l);
+                else if (p.a.lse != nullptr)
+                    p.a.lse[(static_cast<size_t>(item.sequence) * p.a.tokens + token) * p.a.q_heads + query_head] =
+                        l == 0.f ? -INFINITY : (m + log2f(l)) * (1.f / kLog2e);
+            }
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
                 tmem_load_32(tmem + mine + c * 32, o);
                 tmem_load_wait();
                 const float (&v)[32] = reinterpret_cast<const float(&)[32]>(o);
-                if (row <= last_row && item.whole) {
+                if (item.whole) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        finish_row<T>(p, item.sequence, item.head, row, c * 32 + j, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]), m, l, 1.f);
+                    for (int j = 0; j < 4; ++j)
+                        *tile_piece(queries, r, c * 4 + j) =
+                            make_uint4(narrow2<T>(v[8 * j] * inv, v[8 * j + 1] * inv), narrow2<T>(v[8 * j + 2] * inv, v[8 * j + 3] * inv),
+                                       narrow2<T>(v[8 * j + 4] * inv, v[8 * j + 5] * inv), narrow2<T>(v[8 * j + 6] * inv, v[8 * j + 7] * inv));
                 } else if (row <= last_row) {
-                    float4* out = reinterpret_cast<float4*>(p.partial + static_cast<size_t>(piece) * D + c * 32);
+                    float4* out = reinterpret_cast<float4*>(p.partial) + static_cast<size_t>(item.piece) * p.rows_cap * (D / 4) + r;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) out[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    for (int j = 0; j < 8; ++j)
+                        out[static_cast<size_t>(c * 8 + j) * p.rows_cap] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 }
+            }
+            if (item.whole) {
+                __syncwarp();
+                T* out = static_cast<T*>(p.a.out) + item.sequence * p.a.out_strides[0] + token * p.a.out_strides[1] +
+                         query_head * p.a.out_strides[2];
+                by_rows<D>(row <= last_row ? out : nullptr, [&](int, int at, int c, uint8_t* to) {
+                    if (to != nullptr) reinterpret_cast<uint4*>(to)[c] = *tile_piece(queries, warp * 32 + at, c);
+                });
                 __syncwarp();
             }
         }
@@ -385,11 +425,85 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
     }
 }
 
+// Joins the partial results of an item that lies in several runs (see SplitItem): 32 rows a block, a row each lane, the elements
+// of a row shared among the warps. Finished rows go out by way of shared memory.
+constexpr int kJoinRows = 32, kJoinWarps = 8;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_blocks_kernel(const __grid_constant__ AttendDev p) {
+    constexpr int kMine = D / 4 / kJoinWarps;             // float4s of a row that a thread has
+    constexpr int kAhead = D == 64 ? 8 : D == 128 ? 4 : 2;  // partial results on the way at once
+    __shared__ __align__(16) uint8_t rows[kJoinRows][D * 2 + 16];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const SplitItem item(p, blockIdx.x);
+    if (!item.split) return;
+    const int r = blockIdx.y * kJoinRows + lane, row = item.row_tile * kBlockRows + r;
+    const bool there = r < p.rows_cap && row < p.rows;
+    pdl_wait();
+    pdl_launch_dependents();
+    float4 sum[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, l = 0.f;
+    if (there) {
+        for (int c0 = item.run; c0 <= item.last; c0 += kAhead) {
+            float2 ml[kAhead];
+            float4 v[kAhead][kMine];
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                const int c = c0 + a;
+                ml[a] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) v[a][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c > item.last) continue;
+                const size_t piece = static_cast<size_t>(c * 2 + (c == item.run));
+                ml[a] = __ldcg(reinterpret_cast<const float2*>(p.stats) + piece * p.rows_cap + r);
+#pragma unroll
+                for (int i = 0; i < kMine; ++i)
+                    v[a][i] = __ldcg(reinterpret_cast<const float4*>(p.partial) + (piece * (D / 4) + warp + i * kJoinWarps) * p.rows_cap + r);
+            }
+            float n = top;
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) n = fmaxf(n, ml[a].x);
+            const float keep = top == -INFINITY ? 0.f : exp2_approx(top - n);
+            l *= keep, top = n;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) sum[i].x *= keep, sum[i].y *= keep, sum[i].z *= keep, sum[i].w *= keep;
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                const float f = ml[a].x == -INFINITY ? 0.f : exp2_approx(ml[a].x - n);
+                l += ml[a].y * f;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i)
+                    sum[i].x += v[a][i].x * f, sum[i].y += v[a][i].y * f, sum[i].z += v[a][i].z * f, sum[i].w += v[a][i].w * f;
+            }
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int token = token_of(p, min(row, p.rows - 1)), query_head = item.head * p.group + min(row, p.rows - 1) - token * p.group;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        *reinterpret_cast<uint2*>(&rows[lane][(warp + i * kJoinWarps) * 8]) =
+            make_uint2(narrow2<T>(sum[i].x * inv, sum[i].y * inv), narrow2<T>(sum[i].z * inv, sum[i].w * inv));
+    if (there && warp == 0 && p.a.lse != nullptr)
+        p.a.lse[(static_cast<size_t>(item.sequence) * p.a.tokens + token) * p.a.q_heads + query_head] =
+            l == 0.f ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
+    __syncthreads();
+    T* out = static_cast<T*>(p.a.out) + item.sequence * p.a.out_strides[0] + token * p.a.out_strides[1] + query_head * p.a.out_strides[2];
+    by_rows<D>(there ? out : nullptr, [&](int i, int at, int c, uint8_t* to) {
+        if (to != nullptr && i % kJoinWarps == warp) reinterpret_cast<uint4*>(to)[c] = *reinterpret_cast<const uint4*>(&rows[at][c * 16]);
+    });
+}
+
 int launch_blocks(const AttendDev& p, const LaunchOpts& o) {
     void* args[] = {const_cast<AttendDev*>(&p)};
     auto run = [&](auto t, auto dim) {
+        using T = decltype(t);
         constexpr int kDim = decltype(dim)::value;
-        return launch_kernel<blocks_kernel<decltype(t), kDim>>(dim3(p.grid), dim3(kBlockThreads), BlockSmem<kDim>::kAll, args, o);
+        const int rc = launch_kernel<blocks_kernel<T, kDim>>(dim3(p.grid), dim3(kBlockThreads), BlockSmem<kDim>::kAll, args, o);
+        if (rc != 0 || p.partial == nullptr) return rc;
+        return launch_kernel<join_blocks_kernel<T, kDim>>(dim3(p.by_item ? p.a.batch * p.items : p.grid, (p.rows_cap + kJoinRows - 1) / kJoinRows),
+                                                          dim3(kJoinWarps * 32), 0, args, {o.stream, true, false});
     };
     auto by_dim = [&](auto t) {
         switch (p.a.cache.head_dim) {

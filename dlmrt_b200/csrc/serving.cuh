@@ -27,7 +27,8 @@ constexpr int kUnitShift = 6, kTileKeys = 1 << kUnitShift;  // keys of a step, a
 struct alignas(64) AttendDev {
     CUtensorMap tm_k, tm_v;  // (128 bytes, page size, column blocks, heads, pages); a box: min(page size, kTileKeys) whole slots
     DlmAttend a;
-    float* partial;    // [cta][2][rows_cap][head_dim] unnormalised outputs of items that lie in several CTAs' runs, or null
+    float* partial;    // [run][2][rows_cap][head_dim] unnormalised outputs of items that lie in several runs, or null; in the
+                       // kernel for blocks of tokens [run][2][head_dim / 4][rows_cap][4]
     float* stats;      // the same without head_dim, 2: running maximum (base 2) and sum
     int page_shift;
     int group;         // query heads of a key head
@@ -62,7 +63,7 @@ __host__ __device__ inline Cut attend_cut(uint32_t total, int resident, int leas
 
 int launch_append(const DlmAppend& p, int page_shift, const LaunchOpts& o);
 int launch_attend(const AttendDev& p, const LaunchOpts& o);
-int launch_blocks(const AttendDev& p, const LaunchOpts& o);  // its first half, without the join
+int launch_blocks(const AttendDev& p, const LaunchOpts& o);
 int attend_ctas_per_sm(int type, int cache_type, int head_dim);
 int launch_adapters(const DlmAdapters& p, const LaunchOpts& o);
 
