@@ -463,10 +463,11 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
     float2* stats = reinterpret_cast<float2*>(sums + blockDim.x);
     const int across = D / 4 / gridDim.z, lines = blockDim.x / across;  // threads along a row, and how often
     const SplitItem item(p, blockIdx.x);
-    if (!item.split) return;
     const int run = item.run, last = item.last, head = item.head, first_row = item.row_tile * kRowTile;
+    // Every block waits, those without work too: this kernel's end stands for the end of the one in front.
     pdl_wait();
     pdl_launch_dependents();
+    if (!item.split) return;
     const int per_block = (p.rows_cap + gridDim.y - 1) / gridDim.y;
     const int row_begin = blockIdx.y * per_block, row_end = min(min(row_begin + per_block, p.rows_cap), p.rows - first_row);
     const int deep = max(1, lines / per_block);  // threads along the partial results of a row

@@ -325,7 +325,7 @@ struct SplitItem {
     bool split;
     int sequence, head, row_tile, run, last;  // its runs are [run, last]
 
-    __device__ __forceinline__ SplitItem(const AttendDev& p, int b) : split(false) {
+    __device__ __forceinline__ SplitItem(const AttendDev& p, int b) : split(false), sequence(0), head(0), row_tile(0), run(b), last(b) {
         const Line line(p, false);
         int index;
         if (p.by_item) {

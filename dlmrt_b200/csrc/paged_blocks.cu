@@ -1,27 +1,30 @@
 // Attention over the paged cache for blocks of tokens: more rows share a key head's keys than a warp's tile holds (a block of
 // 32 tokens of four query heads each is 128), so that a step's arithmetic is worth a 128-row tile in tensor memory.
 //
-//   warps 0-3  a row of the tile each thread: Q into shared memory, then for every step of 64 keys the row of scores out of
-//              tensor memory, mask, maximum, weights exp2(s - m) back into tensor memory over the scores, and their sum.
-//   warp 4     the producer (paged_attend.cuh).
-//   warp 5     issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory, V as it
+//   warps 0-7  two threads for each row of the tile, 32 of a step's 64 keys and half of the output's elements each: Q into
+//              shared memory, then for every step the scores out of tensor memory, mask, maximum (the two exchange theirs),
+//              weights exp2(s - m) back into tensor memory over the scores, and their sum.
+//   warp 8     the producer (paged_attend.cuh).
+//   warp 9     issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory, V as it
 //              lies, its 64 keys down the rows). S has two buffers: the next step's scores are computed under this one's
 //              softmax.
 //
 // m is the running maximum when O was last rescaled: O, which lives in tensor memory, is multiplied by exp2(m - m') only when
 // some row's maximum has grown by more than 8 (a factor of 256, which the weights and their FP32 sum have room for).
 //
-// One CTA an SM; shared memory holds 3 to 6 steps of 64 keys. A step is 2 * 128 * 64 * head_dim multiply-adds (512 cycles of the
-// tensor pipe at 128) and 64 exponentials for each of 128 threads, which is what bounds it once keys come fast enough.
+// One CTA an SM; shared memory holds 2 to 6 steps of 64 keys. A step is 2 * 128 * 64 * head_dim multiply-adds (512 cycles of the
+// tensor pipe at 128) and 8192 exponentials (512 cycles). With one thread a row it took 1300 cycles, as long as its 32 KB take
+// from HBM, and nothing was left to catch up with what an item's beginning and end cost.
 #include "paged_attend.cuh"
 
 namespace dlm {
 
 namespace {
 
-constexpr int kSoftmaxThreads = 128;
-constexpr int kBlockThreads = 192;
-constexpr int kProducerWarp = 4, kIssuerWarp = 5;
+constexpr int kSoftmaxThreads = 256;
+constexpr int kBlockThreads = 320;
+constexpr int kProducerWarp = 8, kIssuerWarp = 9;
+constexpr int kHalfKeys = kTileKeys / 2;
 constexpr float kRescaleAbove = 8.f;
 
 template <int D>
@@ -77,6 +80,14 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -89,21 +100,39 @@ __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* r)
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The two warps that share 32 rows meet.
+__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
+
+__device__ __forceinline__ bool pair_any(int quarter, bool vote) {
+    int any;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.s32 p, %1, 0;\n"
+        "barrier.cta.red.or.pred q, %2, 64, p;\n"
+        "selp.s32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(any)
+        : "r"(static_cast<int>(vote)), "r"(quarter + 1)
+        : "memory");
+    return any != 0;
+}
+
 // 16-byte piece `c` of row `r` of a tile of 128 rows, in column blocks of 128 bytes under the 128-byte swizzle.
 __device__ __forceinline__ uint4* tile_piece(uint8_t* tile, int r, int c) {
     return reinterpret_cast<uint4*>(tile + (c / 8) * (kBlockRows * 128) + r * 128 + ((c % 8) ^ (r & 7)) * 16);
 }
 
-// The address of row `row` of a [sequence, token, head, D] tensor, in lane order: every lane passes its own row's, and reads
-// rows in turn, D / 8 lanes of 16 bytes each.
-template <int D, typename F>
-__device__ __forceinline__ void by_rows(const void* mine, F f) {
-    constexpr int kAcross = D / 8, kAtOnce = 32 / kAcross;
+// Goes through 32 rows of D 16-bit elements, D / 8 lanes of 16 bytes each: every lane passes the address of its own row. One of
+// kWays warps that share the rows takes `part`. f(turn, row, piece, address).
+template <int D, int kWays, typename F>
+__device__ __forceinline__ void by_rows(const void* mine, int part, F f) {
+    constexpr int kAcross = D / 8, kAtOnce = 32 / kAcross, kTurns = 32 / kAtOnce / kWays;
     const int lane = threadIdx.x & 31;
     const unsigned long long at = reinterpret_cast<unsigned long long>(mine);
 #pragma unroll
-    for (int i = 0; i < 32 / kAtOnce; ++i) {
-        const int r = i * kAtOnce + lane / kAcross;
+    for (int i = 0; i < kTurns; ++i) {
+        const int r = (i * kWays + part) * kAtOnce + lane / kAcross;
         f(i, r, lane % kAcross, reinterpret_cast<uint8_t*>(__shfl_sync(0xFFFFFFFFu, at, r)));
     }
 }
@@ -126,17 +155,20 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* queries = smem + Shared::kRing;
     __shared__ Pipes<kStages> pipes;
-    // queries written; scores computed (two buffers); weights written; a step's values consumed; a side step of the warps 0-3
-    __shared__ uint64_t q_full, s_full[2], p_full[2], pv_done, aside;
+    // Queries written; scores computed, weights written, values consumed, of even and of odd steps; a side step of the warps 0-7.
+    // Two barriers each, because a wait can only tell a phase from the one before it: when a step's values are waited for, those
+    // of the step before may still be on their way.
+    __shared__ uint64_t q_full, s_full[2], p_full[2], pv_done[2], aside;
     __shared__ uint32_t tmem_base;
+    __shared__ float tops[2][2][kBlockRows], sums[2][kBlockRows];  // of a row's halves: maxima of a step (two in turn), sums
+    __shared__ uint32_t zeros[2][kBlockRows];
 
     const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const bool leader = elect_one();
     if (warp == kProducerWarp && leader) {
         pipes.init(1, kSoftmaxThreads / 32 + 1);
         mbar_init(&q_full, kSoftmaxThreads);
-        for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kSoftmaxThreads);
-        mbar_init(&pv_done, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kSoftmaxThreads), mbar_init(&pv_done[i], 1);
         mbar_init(&aside, kSoftmaxThreads);
         fence_barrier_init();
         tma_prefetch_descriptor(&p.tm_k);
@@ -175,6 +207,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
             if (leader) mbar_arrive(&pipes.work_empty[slot]);
             if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
             if (head < 0) break;
+            if (tiles == 0) continue;  // nothing to compute, and no queries were brought
             wait(&q_full, q_parity, 6, tiles);
             q_parity ^= 1;
             auto scores = [&](uint32_t n) {  // of step n, whose keys are the next stage's
@@ -190,11 +223,11 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                 }
                 if (++next_stage == kStages) next_stage = 0, parity ^= 1;
             };
-            if (tiles > 0) scores(step);
+            scores(step);
             for (int tile = 0; tile < tiles; ++tile, ++step) {
                 if (tile + 1 < tiles) {
                     // The other buffer held the weights of the step before, which have to have been consumed.
-                    if (tile > 0) wait(&pv_done, (step - 1) & 1, 8, tile);
+                    if (tile > 0) wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 8, tile);
                     scores(step + 1);
                 }
                 wait(&p_full[step & 1], step >> 1 & 1, 9, tile);
@@ -204,15 +237,17 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                     for (int k = 0; k < kTileKeys / 16; ++k)
                         umma_f16_ts(tmem, tmem_s + (step & 1) * 64 + k * 8, umma_desc_mn128(values + k * 2048, kBlockBytes), kIdescO);
                     umma_commit(&pipes.empty[stage]);
-                    umma_commit(&pv_done);
+                    umma_commit(&pv_done[step & 1]);
                 }
                 if (++stage == kStages) stage = 0;
             }
         }
     } else {
-        // -- a row of the tile each thread -----------------------------------------------------------------------------
-        const int r = threadIdx.x;
-        const uint32_t mine = static_cast<uint32_t>(warp * 32) << 16;  // this warp's lanes of tensor memory
+        // -- half a row of the tile each thread --------------------------------------------------------------------------
+        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
+        const uint32_t mine = static_cast<uint32_t>(quarter * 32) << 16;  // this warp's lanes of tensor memory
+        constexpr int kChunks = D / 64;                                   // of 32 elements of the output, from chunk0 on
+        const int chunk0 = half * kChunks;
         const float scale = p.a.scale * kLog2e;
         int stage = 0, slot = 0;
         uint32_t slot_parity = 0, step = 0, aside_parity = 0;
@@ -223,10 +258,8 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
         };
         while (true) {
             const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
-            if (!announced) {
-                if (leader) stalled(p, 10, slot);
-                break;
-            }
+            if (!announced && leader) stalled(p, 10, slot);
+            if (pair_any(quarter, !announced)) break;  // neither may wait for the other any more
             const Work item = pipes.works[slot];
             __syncwarp();
             if (leader) mbar_arrive(&pipes.work_empty[slot]);
@@ -238,77 +271,80 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
             const int all_from = seen_from(p, item.first_pos, token_of(p, last_row));                     // from here on every row sees
             const int all_to = seen_to(p, item.first_pos, item.length, token_of(p, first_row));         // the keys, up to here
             const int query_head = item.head * p.group + min(row, last_row) - token * p.group;
-            {   // Q, swizzled as TMA would, a warp its own 32 rows; the products that read the last item's are done
+            if (item.tiles > 0) {  // Q, swizzled as TMA would, a warp every other of its rows; the products that read the last item's are done
                 const T* q = static_cast<const T*>(p.a.q) + item.sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
                              query_head * p.a.q_strides[2];
-                constexpr int kReads = D / 8;
-                uint4 v[kReads];
-                by_rows<D>(row <= last_row ? q : nullptr, [&](int i, int, int c, const uint8_t* at) {
+                uint4 v[D / 16];
+                by_rows<D, 2>(row <= last_row ? q : nullptr, half, [&](int i, int, int c, const uint8_t* at) {
                     v[i] = at != nullptr ? reinterpret_cast<const uint4*>(at)[c] : make_uint4(0, 0, 0, 0);
                 });
-                by_rows<D>(nullptr, [&](int i, int at, int c, const uint8_t*) { *tile_piece(queries, warp * 32 + at, c) = v[i]; });
+                by_rows<D, 2>(nullptr, half, [&](int i, int at, int c, const uint8_t*) { *tile_piece(queries, quarter * 32 + at, c) = v[i]; });
                 fence_proxy_async();
                 mbar_arrive(&q_full);
             }
             {
                 uint32_t zero[32] = {};
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) tmem_store_32(tmem + mine + c * 32, zero);
+                for (int c = 0; c < kChunks; ++c) tmem_store_32(tmem + mine + (chunk0 + c) * 32, zero);
                 tmem_store_wait();
             }
             float m = -INFINITY, l = 0.f;
             for (int tile = 0; tile < item.tiles; ++tile, ++step) {
                 const uint32_t s_at = tmem_s + mine + (step & 1) * 64;
-                uint32_t raw[64];
+                uint32_t raw[kHalfKeys];
                 wait(&s_full[step & 1], step >> 1 & 1, 11, tile);
-                tmem_load_32(s_at, raw);
-                tmem_load_32(s_at + 32, raw + 32);
+                tmem_load_32(s_at + half * kHalfKeys, raw);
                 tmem_load_wait();
-                float (&s)[64] = reinterpret_cast<float(&)[64]>(raw);
+                float (&s)[kHalfKeys] = reinterpret_cast<float(&)[kHalfKeys]>(raw);
                 const int key0 = item.start + tile * kTileKeys;
                 const uint64_t present = pipes.present[stage];
                 const bool by_row = key0 < all_from || key0 + kTileKeys > all_to;  // rows see different keys of this step
                 const bool edge = by_row || present != ~0ull;
 #pragma unroll
-                for (int j = 0; j < 64; ++j) s[j] *= scale;
+                for (int j = 0; j < kHalfKeys; ++j) s[j] *= scale;
                 if (edge) {
-                    const int lo = from - key0, hi = to - key0;
+                    const int first_key = key0 + half * kHalfKeys;
+                    const int lo = from - first_key, hi = to - first_key;
+                    const uint32_t there = static_cast<uint32_t>(present >> (half * kHalfKeys));
 #pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (j < lo || j >= hi || !(present >> j & 1)) s[j] = -INFINITY;
+                    for (int j = 0; j < kHalfKeys; ++j)
+                        if (j < lo || j >= hi || !(there >> j & 1)) s[j] = -INFINITY;
                 }
                 float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int j = 4; j < 64; ++j) top4[j & 3] = fmaxf(top4[j & 3], s[j]);
-                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                for (int j = 4; j < kHalfKeys; ++j) top4[j & 3] = fmaxf(top4[j & 3], s[j]);
+                float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                tops[step & 1][half][r] = top;
+                pair_sync(quarter);  // also: both have their scores, which the weights overwrite
+                top = fmaxf(top, tops[step & 1][half ^ 1][r]);
                 if (__any_sync(0xFFFFFFFFu, top > m + kRescaleAbove || (m == -INFINITY && top > m))) {
                     const float n = fmaxf(m, top);
                     const float f = m == n ? 1.f : exp2_approx(m - n);  // 0 where nothing was there
                     l *= f, m = n;
                     if (tile > 0) {
-                        wait(&pv_done, (step - 1) & 1, 12, tile);
+                        wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 12, tile);
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
+                        for (int c = 0; c < kChunks; ++c) {
                             uint32_t o[32];
-                            tmem_load_32(tmem + mine + c * 32, o);
+                            tmem_load_32(tmem + mine + (chunk0 + c) * 32, o);
                             tmem_load_wait();
 #pragma unroll
                             for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tmem_store_32(tmem + mine + c * 32, o);
+                            tmem_store_32(tmem + mine + (chunk0 + c) * 32, o);
                         }
                     }
                 }
                 const float sub = m == -INFINITY ? 0.f : m;
                 float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t weights[32];
+                uint32_t weights[kHalfKeys / 2];
 #pragma unroll
-                for (int j = 0; j < 64; j += 2) {
+                for (int j = 0; j < kHalfKeys; j += 2) {
                     s[j] = exp2_approx(s[j] - sub), s[j + 1] = exp2_approx(s[j + 1] - sub);
                     sum4[j & 3] += s[j], sum4[(j + 1) & 3] += s[j + 1];
                     weights[j / 2] = narrow2<T>(s[j], s[j + 1]);
                 }
                 l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-                tmem_store_32(s_at, weights);
+                tmem_store_16(s_at + half * (kHalfKeys / 2), weights);
                 if (edge) {
                     // Values that are not finite, in keys that some rows see and others do not, or that are not there: 0 * inf
                     // would reach the result. Their keys are found by every warp for itself.
@@ -329,17 +365,20 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                         }
                         bad |= static_cast<uint64_t>(__ballot_sync(0xFFFFFFFFu, any)) << (32 * i);
                     }
-                    if (bad != 0) {  // the same in all four warps
-                        uint64_t weightless = 0;  // keys whose weight is zero here: 0 * inf is NaN
+                    if (bad != 0) {  // the same in all eight warps
+                        uint32_t none_of_half = 0;  // keys whose weight is zero here: 0 * inf is NaN
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) weightless |= static_cast<uint64_t>(s[j] == 0.f) << j;
-                        if (tile > 0) wait(&pv_done, (step - 1) & 1, 13, tile);
+                        for (int j = 0; j < kHalfKeys; ++j) none_of_half |= static_cast<uint32_t>(s[j] == 0.f) << j;
+                        zeros[half][r] = none_of_half;
+                        pair_sync(quarter);
+                        const uint64_t weightless = static_cast<uint64_t>(zeros[1][r]) << 32 | zeros[0][r];
+                        if (tile > 0) wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 13, tile);
 #pragma unroll 1
                         for (uint64_t left = bad; left != 0; left &= left - 1) {
                             const int key = __ffsll(static_cast<long long>(left)) - 1;
                             const bool see = key0 + key >= from && key0 + key < to && (present >> key & 1);
 #pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
+                            for (int c = chunk0; c < chunk0 + kChunks; ++c) {
                                 uint32_t o[32];
                                 tmem_load_32(tmem + mine + c * 32, o);
                                 tmem_load_wait();
@@ -360,7 +399,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                         aside_parity ^= 1;
                         for (uint64_t left = bad; left != 0; left &= left - 1) {
                             const int key = __ffsll(static_cast<long long>(left)) - 1;
-                            if ((key & 3) != warp) continue;
+                            if ((key & 7) != warp) continue;
                             for (int c = lane; c < D / 8; c += 32) {
                                 uint4 v = *piece(key, c);
                                 v.x &= ~not_finite<T>(v.x), v.y &= ~not_finite<T>(v.y), v.z &= ~not_finite<T>(v.z), v.w &= ~not_finite<T>(v.w);
@@ -376,11 +415,14 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                 if (++stage == kStages) stage = 0;
             }
             // -- the row's result ---------------------------------------------------------------------------------------
-            if (item.tiles > 0) wait(&pv_done, (step - 1) & 1, 15, item.tiles);
+            if (item.tiles > 0) wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 15, item.tiles);
             // Parts of a row go out with rows side by side, [element / 4][row], a finished row by way of the tile of queries, whose
             // products are done: a thread's own row would be 32 lanes' stores far apart (5 us an item instead of 1.5).
+            sums[half][r] = l;
+            pair_sync(quarter);
+            l = sums[0][r] + sums[1][r];
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (row <= last_row) {
+            if (row <= last_row && half == 0) {
                 if (!item.whole)
                     *reinterpret_cast<float2*>(p.stats + (static_cast<size_t>(item.piece) * p.rows_cap + r) * 2) = make_float2(m, l);
                 else if (p.a.lse != nullptr)
@@ -388,7 +430,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                         l == 0.f ? -INFINITY : (m + log2f(l)) * (1.f / kLog2e);
             }
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = chunk0; c < chunk0 + kChunks; ++c) {
                 uint32_t o[32];
                 tmem_load_32(tmem + mine + c * 32, o);
                 tmem_load_wait();
@@ -407,14 +449,14 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                 }
             }
             if (item.whole) {
-                __syncwarp();
+                pair_sync(quarter);
                 T* out = static_cast<T*>(p.a.out) + item.sequence * p.a.out_strides[0] + token * p.a.out_strides[1] +
                          query_head * p.a.out_strides[2];
-                by_rows<D>(row <= last_row ? out : nullptr, [&](int, int at, int c, uint8_t* to) {
-                    if (to != nullptr) reinterpret_cast<uint4*>(to)[c] = *tile_piece(queries, warp * 32 + at, c);
+                by_rows<D, 2>(row <= last_row ? out : nullptr, half, [&](int, int at, int c, uint8_t* to) {
+                    if (to != nullptr) reinterpret_cast<uint4*>(to)[c] = *tile_piece(queries, quarter * 32 + at, c);
                 });
-                __syncwarp();
             }
+            pair_sync(quarter);  // the next item's queries and sums take the place of these
         }
     }
     tcgen05_fence_before();
@@ -436,11 +478,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_blocks_kernel(const __gr
     __shared__ __align__(16) uint8_t rows[kJoinRows][D * 2 + 16];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const SplitItem item(p, blockIdx.x);
-    if (!item.split) return;
     const int r = blockIdx.y * kJoinRows + lane, row = item.row_tile * kBlockRows + r;
     const bool there = r < p.rows_cap && row < p.rows;
+    // Every block waits, those without work too: this kernel's end stands for the end of the one in front.
     pdl_wait();
     pdl_launch_dependents();
+    if (!item.split) return;
     float4 sum[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -490,8 +533,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_blocks_kernel(const __gr
             l == 0.f ? -INFINITY : (top + log2f(l)) * (1.f / kLog2e);
     __syncthreads();
     T* out = static_cast<T*>(p.a.out) + item.sequence * p.a.out_strides[0] + token * p.a.out_strides[1] + query_head * p.a.out_strides[2];
-    by_rows<D>(there ? out : nullptr, [&](int i, int at, int c, uint8_t* to) {
-        if (to != nullptr && i % kJoinWarps == warp) reinterpret_cast<uint4*>(to)[c] = *reinterpret_cast<const uint4*>(&rows[at][c * 16]);
+    by_rows<D, kJoinWarps>(there ? out : nullptr, warp, [&](int, int at, int c, uint8_t* to) {
+        if (to != nullptr) reinterpret_cast<uint4*>(to)[c] = *reinterpret_cast<const uint4*>(&rows[at][c * 16]);
     });
 }
 

@@ -94,6 +94,22 @@ def test_the_same_bits_and_graphs():
     assert torch.equal(outs[0], first) and torch.equal(outs[1], want)
 
 
+@pytest.mark.parametrize("t, hq, hk, d", [(1, 8, 2, 128), (40, 2, 1, 64), (64, 8, 2, 128), (70, 4, 2, 256)])
+def test_calls_in_turn_do_not_see_each_others_scratch(t, hq, hk, d):
+    """Two calls on other inputs in turn, whose scratch torch's allocator puts in the same place: a result that was joined too
+    early would be the other call's."""
+    kv, q, table, lengths = setup([900, 300, t, 2000, 640], t, hq, hk, d, 16, BF16, BF16)
+    other = (q.flip(0) * -1).contiguous()
+    want = {}
+    for x in (q, other):
+        out, bound, _ = su.attend(x[:, :1], kv.keys, kv.values, None, None, table, lengths.tolist(), d ** -0.5)
+        want[x is q] = kv.attend(x, table, lengths).clone()
+        su.assert_within(want[x is q][:, :1], out, bound)
+    for _ in range(60):
+        assert torch.equal(kv.attend(q, table, lengths), want[True])
+        assert torch.equal(kv.attend(other, table, lengths), want[False])
+
+
 def test_strided_queries_in_place():
     kv, q, table, lengths = setup([100, 70], 40, 4, 2, 64, 16, BF16, BF16)
     want = kv.attend(q, table, lengths)
