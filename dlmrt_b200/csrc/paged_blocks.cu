@@ -1,40 +1,42 @@
 // Attention over the paged cache for blocks of tokens: more rows share a key head's keys than a warp's tile holds (a block of
 // 32 tokens of four query heads each is 128), so that a step's arithmetic is worth a 128-row tile in tensor memory.
 //
-//   warps 0-7  two threads for each row of the tile, 32 of a step's 64 keys and half of the output's elements each: Q into
-//              shared memory, then for every step the scores out of tensor memory, mask, maximum (the two exchange theirs),
-//              weights exp2(s - m) back into tensor memory over the scores, and their sum.
-//   warp 8     the producer (paged_attend.cuh).
-//   warp 9     issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory, V as it
-//              lies, its 64 keys down the rows). S has two buffers: the next step's scores are computed under this one's
-//              softmax.
+//   softmax    groups of four warps, a row of the tile each thread: Q into shared memory, then for every step of 64 keys the row
+//              of scores out of tensor memory, mask, maximum, weights exp2(s - m) back into tensor memory over the scores, and
+//              their sum. Two groups take steps in turn, each with its own maximum, sum and O, and put them together at an
+//              item's end (heads of 256 leave tensor memory for one).
+//   producer   a warp, see paged_attend.cuh.
+//   issuer     a warp that issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory,
+//              V as it lies, its 64 keys down the rows). Each group has two buffers of S: its next step's scores are computed
+//              under this one's softmax.
 //
 // m is the running maximum when O was last rescaled: O, which lives in tensor memory, is multiplied by exp2(m - m') only when
 // some row's maximum has grown by more than 8 (a factor of 256, which the weights and their FP32 sum have room for).
 //
-// One CTA an SM; shared memory holds 2 to 6 steps of 64 keys. A step is 2 * 128 * 64 * head_dim multiply-adds (512 cycles of the
-// tensor pipe at 128) and 8192 exponentials (512 cycles). With one thread a row it took 1300 cycles, as long as its 32 KB take
-// from HBM, and nothing was left to catch up with what an item's beginning and end cost.
+// One CTA an SM; shared memory holds 2 to 8 steps of 64 keys. A step is 2 * 128 * 64 * head_dim multiply-adds (512 cycles of the
+// tensor pipe at 128) and 8192 exponentials (512 cycles). A group takes 1300 cycles for a step, most of it latency, which is as
+// long as a step's 32 KB take from HBM: with one group nothing is left to catch up with what an item's beginning and end cost.
 #include "paged_attend.cuh"
 
 namespace dlm {
 
 namespace {
 
-constexpr int kSoftmaxThreads = 256;
-constexpr int kBlockThreads = 320;
-constexpr int kProducerWarp = 8, kIssuerWarp = 9;
-constexpr int kHalfKeys = kTileKeys / 2;
+constexpr int kGroupThreads = 128;
 constexpr float kRescaleAbove = 8.f;
 
 template <int D>
-struct BlockSmem {
-    static constexpr int kStages = D == 256 ? 2 : D == 128 ? 4 : 6;
+struct BlockShape {
+    static constexpr int kGroups = D == 256 ? 1 : 2;
+    static constexpr int kBuffers = 2 * kGroups;              // of S
+    static constexpr int kProducerWarp = 4 * kGroups, kIssuerWarp = kProducerWarp + 1;
+    static constexpr int kThreads = kGroups * kGroupThreads + 64;
+    static constexpr int kStages = D == 256 ? 2 : D == 128 ? 5 : 8;
     static constexpr int kBytes = kTileKeys * D * 2;          // keys, or values, of a stage
     static constexpr int kRing = kStages * 2 * kBytes;
     static constexpr int kQueries = kBlockRows * D * 2;
     static constexpr int kAll = kRing + kQueries + 1024;      // the ring begins at a multiple of 1024
-    static constexpr uint32_t kColumns = D == 256 ? 512 : 256;  // of tensor memory: O, then two S of 64
+    static constexpr uint32_t kColumns = 512;                 // of tensor memory: an O of each group, then the buffers of S
 };
 
 // Instruction descriptor of kind::f16, see umma_idesc_bf16: T is BF16 or FP16, B is K-major, or MN-major where `b_mn`.
@@ -80,14 +82,6 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
 __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -100,20 +94,28 @@ __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* r)
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// The two warps that share 32 rows meet.
-__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
-
-__device__ __forceinline__ bool pair_any(int quarter, bool vote) {
+// The warps that share 32 rows, one of each group, meet.
+template <int kGroups>
+__device__ __forceinline__ void rows_sync(int quarter) {
+    if constexpr (kGroups > 1) {
+        tcgen05_fence_before();
+        asm volatile("bar.sync %0, %1;" ::"r"(quarter + 1), "n"(kGroups * 32) : "memory");
+        tcgen05_fence_after();
+    }
+}
+template <int kGroups>
+__device__ __forceinline__ bool rows_any(int quarter, bool vote) {
+    if constexpr (kGroups == 1) return __any_sync(0xFFFFFFFFu, vote);
     int any;
     asm volatile(
         "{\n"
         ".reg .pred p, q;\n"
         "setp.ne.s32 p, %1, 0;\n"
-        "barrier.cta.red.or.pred q, %2, 64, p;\n"
+        "barrier.cta.red.or.pred q, %2, %3, p;\n"
         "selp.s32 %0, 1, 0, q;\n"
         "}\n"
         : "=r"(any)
-        : "r"(static_cast<int>(vote)), "r"(quarter + 1)
+        : "r"(static_cast<int>(vote)), "r"(quarter + 1), "n"(kGroups * 32)
         : "memory");
     return any != 0;
 }
@@ -147,53 +149,53 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 }  // namespace
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_constant__ AttendDev p) {
-    using Shared = BlockSmem<D>;
-    constexpr int kStages = Shared::kStages, kBytes = Shared::kBytes;
+__global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(const __grid_constant__ AttendDev p) {
+    using Shape = BlockShape<D>;
+    constexpr int kStages = Shape::kStages, kBytes = Shape::kBytes, kGroups = Shape::kGroups, kBuffers = Shape::kBuffers;
     constexpr int kBlockBytes = kTileKeys * 128;  // 64 keys of a column block of 64 elements
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* queries = smem + Shared::kRing;
+    uint8_t* queries = smem + Shape::kRing;
     __shared__ Pipes<kStages> pipes;
-    // Queries written; scores computed, weights written, values consumed, of even and of odd steps; a side step of the warps 0-7.
-    // Two barriers each, because a wait can only tell a phase from the one before it: when a step's values are waited for, those
-    // of the step before may still be on their way.
-    __shared__ uint64_t q_full, s_full[2], p_full[2], pv_done[2], aside;
+    // Queries written; of the step that a buffer of S is for: scores computed, weights written, values consumed; a side step of
+    // a group. A wait can only tell a phase from the one before it, which here is kBuffers steps back.
+    __shared__ uint64_t q_full, s_full[kBuffers], p_full[kBuffers], pv_done[kBuffers], aside[kGroups];
     __shared__ uint32_t tmem_base;
-    __shared__ float tops[2][2][kBlockRows], sums[2][kBlockRows];  // of a row's halves: maxima of a step (two in turn), sums
-    __shared__ uint32_t zeros[2][kBlockRows];
+    __shared__ float2 group_stats[kGroups][kBlockRows];  // maximum and sum of a group's steps
 
     const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const bool leader = elect_one();
-    if (warp == kProducerWarp && leader) {
-        pipes.init(1, kSoftmaxThreads / 32 + 1);
-        mbar_init(&q_full, kSoftmaxThreads);
-        for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kSoftmaxThreads), mbar_init(&pv_done[i], 1);
-        mbar_init(&aside, kSoftmaxThreads);
+    if (warp == Shape::kProducerWarp && leader) {
+        pipes.init(1, kGroups * 4 + 1);
+        mbar_init(&q_full, kGroups * kGroupThreads);
+        for (int i = 0; i < kBuffers; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kGroupThreads), mbar_init(&pv_done[i], 1);
+        for (int i = 0; i < kGroups; ++i) mbar_init(&aside[i], kGroupThreads);
         fence_barrier_init();
         tma_prefetch_descriptor(&p.tm_k);
         tma_prefetch_descriptor(&p.tm_v);
     }
-    if (warp == kIssuerWarp) tmem_alloc(&tmem_base, Shared::kColumns);
+    if (warp == Shape::kIssuerWarp) tmem_alloc(&tmem_base, Shape::kColumns);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem = uniform(tmem_base);
-    const uint32_t tmem_s = tmem + D;  // S of step n: + (n & 1) * 64; its weights take the first 32 of these columns
+    const uint32_t tmem_s = tmem + kGroups * D;  // S of step n: + (n % kBuffers) * 64; its weights take the first 32 of these
+    auto buffer = [](uint32_t step) { return step % kBuffers; };
+    auto phase = [](uint32_t step) { return step / kBuffers & 1; };
     const long long deadline = globaltimer() + kDefaultTimeoutNs;
     pdl_wait();
     pdl_launch_dependents();
 
-    if (warp == kProducerWarp) {
+    if (warp == Shape::kProducerWarp) {
         produce<kStages, D / 8, true>(p, smem, pipes, deadline, leader);
-    } else if (warp == kIssuerWarp) {
+    } else if (warp == Shape::kIssuerWarp) {
         // -- the issuer: a whole warp on uniform values, one lane issuing ------------------------------------------------
         constexpr uint32_t kIdescS = idesc_f16<T>(kBlockRows, kTileKeys, false), kIdescO = idesc_f16<T>(kBlockRows, D, true);
         const uint64_t q_desc = umma_desc_k128(queries);
         int stage = 0, slot = 0, next_stage = 0;
         uint32_t parity = 0, slot_parity = 0, q_parity = 0, step = 0;
-        auto wait = [&](uint64_t* bar, uint32_t phase, int who, int at) {
-            if (!mbar_wait_warp(bar, phase, deadline) && leader) stalled(p, who, at);
+        auto wait = [&](uint64_t* bar, uint32_t bar_phase, int who, int at) {
+            if (!mbar_wait_warp(bar, bar_phase, deadline) && leader) stalled(p, who, at);
             tcgen05_fence_after();
         };
         while (true) {
@@ -217,49 +219,50 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                 if (leader) {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        umma_bf16(tmem_s + (n & 1) * 64, q_desc + (k / 4) * (kBlockRows * 128 >> 4) + (k % 4) * 2,
+                        umma_bf16(tmem_s + buffer(n) * 64, q_desc + (k / 4) * (kBlockRows * 128 >> 4) + (k % 4) * 2,
                                   k_desc + (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, kIdescS, k != 0);
-                    umma_commit(&s_full[n & 1]);
+                    umma_commit(&s_full[buffer(n)]);
                 }
                 if (++next_stage == kStages) next_stage = 0, parity ^= 1;
             };
-            scores(step);
+            for (int ahead = 0; ahead < kGroups && ahead < tiles; ++ahead) scores(step + ahead);
             for (int tile = 0; tile < tiles; ++tile, ++step) {
-                if (tile + 1 < tiles) {
-                    // The other buffer held the weights of the step before, which have to have been consumed.
-                    if (tile > 0) wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 8, tile);
-                    scores(step + 1);
+                if (tile + kGroups < tiles) {
+                    // The buffer held the weights of the group's step before, which have to have been consumed.
+                    const uint32_t next = step + kGroups;
+                    if (tile >= kGroups) wait(&pv_done[buffer(next - kBuffers)], phase(next - kBuffers), 8, tile);
+                    scores(next);
                 }
-                wait(&p_full[step & 1], step >> 1 & 1, 9, tile);
+                wait(&p_full[buffer(step)], phase(step), 9, tile);
                 const uint32_t values = smem_u32(smem) + stage * 2 * kBytes + kBytes;
                 if (leader) {
 #pragma unroll
                     for (int k = 0; k < kTileKeys / 16; ++k)
-                        umma_f16_ts(tmem, tmem_s + (step & 1) * 64 + k * 8, umma_desc_mn128(values + k * 2048, kBlockBytes), kIdescO);
+                        umma_f16_ts(tmem + step % kGroups * D, tmem_s + buffer(step) * 64 + k * 8, umma_desc_mn128(values + k * 2048, kBlockBytes),
+                                    kIdescO);
                     umma_commit(&pipes.empty[stage]);
-                    umma_commit(&pv_done[step & 1]);
+                    umma_commit(&pv_done[buffer(step)]);
                 }
                 if (++stage == kStages) stage = 0;
             }
         }
     } else {
-        // -- half a row of the tile each thread --------------------------------------------------------------------------
-        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
+        // -- a row of the tile each thread, every kGroups-th step ------------------------------------------------------------
+        const int quarter = warp & 3, group = warp >> 2, r = quarter * 32 + lane;
         const uint32_t mine = static_cast<uint32_t>(quarter * 32) << 16;  // this warp's lanes of tensor memory
-        constexpr int kChunks = D / 64;                                   // of 32 elements of the output, from chunk0 on
-        const int chunk0 = half * kChunks;
+        const uint32_t tmem_o = tmem + mine + group * D;
         const float scale = p.a.scale * kLog2e;
         int stage = 0, slot = 0;
         uint32_t slot_parity = 0, step = 0, aside_parity = 0;
-        auto wait = [&](uint64_t* bar, uint32_t phase, int who, int at) {
-            if (!mbar_wait(bar, phase, deadline)) stalled(p, who, at);
+        auto wait = [&](uint64_t* bar, uint32_t bar_phase, int who, int at) {
+            if (!mbar_wait(bar, bar_phase, deadline)) stalled(p, who, at);
             __syncwarp();
             tcgen05_fence_after();
         };
         while (true) {
             const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
             if (!announced && leader) stalled(p, 10, slot);
-            if (pair_any(quarter, !announced)) break;  // neither may wait for the other any more
+            if (rows_any<kGroups>(quarter, !announced)) break;  // neither may wait for the other any more
             const Work item = pipes.works[slot];
             __syncwarp();
             if (leader) mbar_arrive(&pipes.work_empty[slot]);
@@ -271,80 +274,81 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
             const int all_from = seen_from(p, item.first_pos, token_of(p, last_row));                     // from here on every row sees
             const int all_to = seen_to(p, item.first_pos, item.length, token_of(p, first_row));         // the keys, up to here
             const int query_head = item.head * p.group + min(row, last_row) - token * p.group;
-            if (item.tiles > 0) {  // Q, swizzled as TMA would, a warp every other of its rows; the products that read the last item's are done
+            if (item.tiles > 0) {  // Q, swizzled as TMA would, a warp some of its rows; the products that read the last item's are done
                 const T* q = static_cast<const T*>(p.a.q) + item.sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
                              query_head * p.a.q_strides[2];
-                uint4 v[D / 16];
-                by_rows<D, 2>(row <= last_row ? q : nullptr, half, [&](int i, int, int c, const uint8_t* at) {
+                uint4 v[D / 8 / kGroups];
+                by_rows<D, kGroups>(row <= last_row ? q : nullptr, group, [&](int i, int, int c, const uint8_t* at) {
                     v[i] = at != nullptr ? reinterpret_cast<const uint4*>(at)[c] : make_uint4(0, 0, 0, 0);
                 });
-                by_rows<D, 2>(nullptr, half, [&](int i, int at, int c, const uint8_t*) { *tile_piece(queries, quarter * 32 + at, c) = v[i]; });
+                by_rows<D, kGroups>(nullptr, group, [&](int i, int at, int c, const uint8_t*) { *tile_piece(queries, quarter * 32 + at, c) = v[i]; });
                 fence_proxy_async();
                 mbar_arrive(&q_full);
             }
             {
                 uint32_t zero[32] = {};
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) tmem_store_32(tmem + mine + (chunk0 + c) * 32, zero);
+                for (int c = 0; c < D / 32; ++c) tmem_store_32(tmem_o + c * 32, zero);
                 tmem_store_wait();
             }
             float m = -INFINITY, l = 0.f;
+            uint32_t own_steps = 0;  // of this group in this item
             for (int tile = 0; tile < item.tiles; ++tile, ++step) {
-                const uint32_t s_at = tmem_s + mine + (step & 1) * 64;
-                uint32_t raw[kHalfKeys];
-                wait(&s_full[step & 1], step >> 1 & 1, 11, tile);
-                tmem_load_32(s_at + half * kHalfKeys, raw);
+                if (step % kGroups != static_cast<uint32_t>(group)) {
+                    if (++stage == kStages) stage = 0;
+                    continue;
+                }
+                const uint32_t s_at = tmem_s + mine + buffer(step) * 64, last_own = step - kGroups;
+                uint32_t raw[64];
+                wait(&s_full[buffer(step)], phase(step), 11, tile);
+                tmem_load_32(s_at, raw);
+                tmem_load_32(s_at + 32, raw + 32);
                 tmem_load_wait();
-                float (&s)[kHalfKeys] = reinterpret_cast<float(&)[kHalfKeys]>(raw);
+                float (&s)[64] = reinterpret_cast<float(&)[64]>(raw);
                 const int key0 = item.start + tile * kTileKeys;
                 const uint64_t present = pipes.present[stage];
                 const bool by_row = key0 < all_from || key0 + kTileKeys > all_to;  // rows see different keys of this step
                 const bool edge = by_row || present != ~0ull;
 #pragma unroll
-                for (int j = 0; j < kHalfKeys; ++j) s[j] *= scale;
+                for (int j = 0; j < 64; ++j) s[j] *= scale;
                 if (edge) {
-                    const int first_key = key0 + half * kHalfKeys;
-                    const int lo = from - first_key, hi = to - first_key;
-                    const uint32_t there = static_cast<uint32_t>(present >> (half * kHalfKeys));
+                    const int lo = from - key0, hi = to - key0;
 #pragma unroll
-                    for (int j = 0; j < kHalfKeys; ++j)
-                        if (j < lo || j >= hi || !(there >> j & 1)) s[j] = -INFINITY;
+                    for (int j = 0; j < 64; ++j)
+                        if (j < lo || j >= hi || !(present >> j & 1)) s[j] = -INFINITY;
                 }
                 float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int j = 4; j < kHalfKeys; ++j) top4[j & 3] = fmaxf(top4[j & 3], s[j]);
-                float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-                tops[step & 1][half][r] = top;
-                pair_sync(quarter);  // also: both have their scores, which the weights overwrite
-                top = fmaxf(top, tops[step & 1][half ^ 1][r]);
+                for (int j = 4; j < 64; ++j) top4[j & 3] = fmaxf(top4[j & 3], s[j]);
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
                 if (__any_sync(0xFFFFFFFFu, top > m + kRescaleAbove || (m == -INFINITY && top > m))) {
                     const float n = fmaxf(m, top);
                     const float f = m == n ? 1.f : exp2_approx(m - n);  // 0 where nothing was there
                     l *= f, m = n;
-                    if (tile > 0) {
-                        wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 12, tile);
+                    if (own_steps > 0) {
+                        wait(&pv_done[buffer(last_own)], phase(last_own), 12, tile);
 #pragma unroll 1
-                        for (int c = 0; c < kChunks; ++c) {
+                        for (int c = 0; c < D / 32; ++c) {
                             uint32_t o[32];
-                            tmem_load_32(tmem + mine + (chunk0 + c) * 32, o);
+                            tmem_load_32(tmem_o + c * 32, o);
                             tmem_load_wait();
 #pragma unroll
                             for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tmem_store_32(tmem + mine + (chunk0 + c) * 32, o);
+                            tmem_store_32(tmem_o + c * 32, o);
                         }
                     }
                 }
                 const float sub = m == -INFINITY ? 0.f : m;
                 float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t weights[kHalfKeys / 2];
+                uint32_t weights[32];
 #pragma unroll
-                for (int j = 0; j < kHalfKeys; j += 2) {
+                for (int j = 0; j < 64; j += 2) {
                     s[j] = exp2_approx(s[j] - sub), s[j + 1] = exp2_approx(s[j + 1] - sub);
                     sum4[j & 3] += s[j], sum4[(j + 1) & 3] += s[j + 1];
                     weights[j / 2] = narrow2<T>(s[j], s[j + 1]);
                 }
                 l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-                tmem_store_16(s_at + half * (kHalfKeys / 2), weights);
+                tmem_store_32(s_at, weights);
                 if (edge) {
                     // Values that are not finite, in keys that some rows see and others do not, or that are not there: 0 * inf
                     // would reach the result. Their keys are found by every warp for itself.
@@ -365,22 +369,19 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                         }
                         bad |= static_cast<uint64_t>(__ballot_sync(0xFFFFFFFFu, any)) << (32 * i);
                     }
-                    if (bad != 0) {  // the same in all eight warps
-                        uint32_t none_of_half = 0;  // keys whose weight is zero here: 0 * inf is NaN
+                    if (bad != 0) {  // the same in all warps of the group
+                        uint64_t weightless = 0;  // keys whose weight is zero here: 0 * inf is NaN
 #pragma unroll
-                        for (int j = 0; j < kHalfKeys; ++j) none_of_half |= static_cast<uint32_t>(s[j] == 0.f) << j;
-                        zeros[half][r] = none_of_half;
-                        pair_sync(quarter);
-                        const uint64_t weightless = static_cast<uint64_t>(zeros[1][r]) << 32 | zeros[0][r];
-                        if (tile > 0) wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 13, tile);
+                        for (int j = 0; j < 64; ++j) weightless |= static_cast<uint64_t>(s[j] == 0.f) << j;
+                        if (own_steps > 0) wait(&pv_done[buffer(last_own)], phase(last_own), 13, tile);
 #pragma unroll 1
                         for (uint64_t left = bad; left != 0; left &= left - 1) {
                             const int key = __ffsll(static_cast<long long>(left)) - 1;
                             const bool see = key0 + key >= from && key0 + key < to && (present >> key & 1);
 #pragma unroll 1
-                            for (int c = chunk0; c < chunk0 + kChunks; ++c) {
+                            for (int c = 0; c < D / 32; ++c) {
                                 uint32_t o[32];
-                                tmem_load_32(tmem + mine + c * 32, o);
+                                tmem_load_32(tmem_o + c * 32, o);
                                 tmem_load_wait();
 #pragma unroll
                                 for (int j = 0; j < 32; j += 2) {
@@ -390,16 +391,16 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                                     if (see && !isfinite(v.x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + v.x * none);
                                     if (see && !isfinite(v.y)) o[j + 1] = __float_as_uint(__uint_as_float(o[j + 1]) + v.y * none);
                                 }
-                                tmem_store_32(tmem + mine + c * 32, o);
+                                tmem_store_32(tmem_o + c * 32, o);
                             }
                             tmem_store_wait();
                         }
-                        mbar_arrive(&aside);  // everybody has read them
-                        wait(&aside, aside_parity, 14, tile);
+                        mbar_arrive(&aside[group]);  // everybody has read them
+                        wait(&aside[group], aside_parity, 14, tile);
                         aside_parity ^= 1;
                         for (uint64_t left = bad; left != 0; left &= left - 1) {
                             const int key = __ffsll(static_cast<long long>(left)) - 1;
-                            if ((key & 7) != warp) continue;
+                            if ((key & 3) != quarter) continue;
                             for (int c = lane; c < D / 8; c += 32) {
                                 uint4 v = *piece(key, c);
                                 v.x &= ~not_finite<T>(v.x), v.y &= ~not_finite<T>(v.y), v.z &= ~not_finite<T>(v.z), v.w &= ~not_finite<T>(v.w);
@@ -411,59 +412,84 @@ __global__ void __launch_bounds__(kBlockThreads, 1) blocks_kernel(const __grid_c
                 }
                 tmem_store_wait();
                 tcgen05_fence_before();
-                mbar_arrive(&p_full[step & 1]);
+                mbar_arrive(&p_full[buffer(step)]);
+                ++own_steps;
                 if (++stage == kStages) stage = 0;
             }
             // -- the row's result ---------------------------------------------------------------------------------------
-            if (item.tiles > 0) wait(&pv_done[(step - 1) & 1], (step - 1) >> 1 & 1, 15, item.tiles);
+            if (own_steps > 0) {
+                const uint32_t last_own = step - 1 - ((step - 1) % kGroups == static_cast<uint32_t>(group) ? 0 : 1);
+                wait(&pv_done[buffer(last_own)], phase(last_own), 15, item.tiles);
+            }
+            // The groups' results together: every group takes its share of the elements, from each group's O.
+            group_stats[group][r] = make_float2(m, l);
+            rows_sync<kGroups>(quarter);
+            float factors[kGroups];
+            m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) m = fmaxf(m, group_stats[i][r].x);
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                factors[i] = group_stats[i][r].x == -INFINITY ? 0.f : exp2_approx(group_stats[i][r].x - m);
+                l += group_stats[i][r].y * factors[i];
+            }
             // Parts of a row go out with rows side by side, [element / 4][row], a finished row by way of the tile of queries, whose
             // products are done: a thread's own row would be 32 lanes' stores far apart (5 us an item instead of 1.5).
-            sums[half][r] = l;
-            pair_sync(quarter);
-            l = sums[0][r] + sums[1][r];
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (row <= last_row && half == 0) {
+            if (row <= last_row && group == 0) {
                 if (!item.whole)
                     *reinterpret_cast<float2*>(p.stats + (static_cast<size_t>(item.piece) * p.rows_cap + r) * 2) = make_float2(m, l);
                 else if (p.a.lse != nullptr)
                     p.a.lse[(static_cast<size_t>(item.sequence) * p.a.tokens + token) * p.a.q_heads + query_head] =
                         l == 0.f ? -INFINITY : (m + log2f(l)) * (1.f / kLog2e);
             }
+            if (item.whole) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) factors[i] *= inv;
+            }
+            constexpr int kChunks = D / 32 / kGroups;
 #pragma unroll 1
-            for (int c = chunk0; c < chunk0 + kChunks; ++c) {
-                uint32_t o[32];
-                tmem_load_32(tmem + mine + c * 32, o);
-                tmem_load_wait();
-                const float (&v)[32] = reinterpret_cast<const float(&)[32]>(o);
+            for (int c = group * kChunks; c < (group + 1) * kChunks; ++c) {
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) {
+                    uint32_t o[32];
+                    tmem_load_32(tmem + mine + i * D + c * 32, o);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = (i == 0 ? 0.f : v[j]) + __uint_as_float(o[j]) * factors[i];
+                }
                 if (item.whole) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        *tile_piece(queries, r, c * 4 + j) =
-                            make_uint4(narrow2<T>(v[8 * j] * inv, v[8 * j + 1] * inv), narrow2<T>(v[8 * j + 2] * inv, v[8 * j + 3] * inv),
-                                       narrow2<T>(v[8 * j + 4] * inv, v[8 * j + 5] * inv), narrow2<T>(v[8 * j + 6] * inv, v[8 * j + 7] * inv));
+                        *tile_piece(queries, r, c * 4 + j) = make_uint4(narrow2<T>(v[8 * j], v[8 * j + 1]), narrow2<T>(v[8 * j + 2], v[8 * j + 3]),
+                                                                        narrow2<T>(v[8 * j + 4], v[8 * j + 5]), narrow2<T>(v[8 * j + 6], v[8 * j + 7]));
                 } else if (row <= last_row) {
                     float4* out = reinterpret_cast<float4*>(p.partial) + static_cast<size_t>(item.piece) * p.rows_cap * (D / 4) + r;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         out[static_cast<size_t>(c * 8 + j) * p.rows_cap] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 }
+                __syncwarp();
             }
             if (item.whole) {
-                pair_sync(quarter);
+                rows_sync<kGroups>(quarter);
+                __syncwarp();
                 T* out = static_cast<T*>(p.a.out) + item.sequence * p.a.out_strides[0] + token * p.a.out_strides[1] +
                          query_head * p.a.out_strides[2];
-                by_rows<D, 2>(row <= last_row ? out : nullptr, half, [&](int, int at, int c, uint8_t* to) {
+                by_rows<D, kGroups>(row <= last_row ? out : nullptr, group, [&](int, int at, int c, uint8_t* to) {
                     if (to != nullptr) reinterpret_cast<uint4*>(to)[c] = *tile_piece(queries, quarter * 32 + at, c);
                 });
+                __syncwarp();
             }
-            pair_sync(quarter);  // the next item's queries and sums take the place of these
+            rows_sync<kGroups>(quarter);  // the next item's queries, statistics and O take the place of these
         }
     }
     tcgen05_fence_before();
     __syncthreads();
-    if (warp == kIssuerWarp) {
+    if (warp == Shape::kIssuerWarp) {
         tcgen05_fence_after();
-        tmem_dealloc(tmem, Shared::kColumns);
+        tmem_dealloc(tmem, Shape::kColumns);
     }
 }
 
@@ -543,7 +569,7 @@ int launch_blocks(const AttendDev& p, const LaunchOpts& o) {
     auto run = [&](auto t, auto dim) {
         using T = decltype(t);
         constexpr int kDim = decltype(dim)::value;
-        const int rc = launch_kernel<blocks_kernel<T, kDim>>(dim3(p.grid), dim3(kBlockThreads), BlockSmem<kDim>::kAll, args, o);
+        const int rc = launch_kernel<blocks_kernel<T, kDim>>(dim3(p.grid), dim3(BlockShape<kDim>::kThreads), BlockShape<kDim>::kAll, args, o);
         if (rc != 0 || p.partial == nullptr) return rc;
         return launch_kernel<join_blocks_kernel<T, kDim>>(dim3(p.by_item ? p.a.batch * p.items : p.grid, (p.rows_cap + kJoinRows - 1) / kJoinRows),
                                                           dim3(kJoinWarps * 32), 0, args, {o.stream, true, false});
