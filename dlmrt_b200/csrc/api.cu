@@ -806,7 +806,7 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
 
 // Everything about an attention call that its device pointers do not decide.
 static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
-    constexpr int kWholeKeys = 512, kBlocksAbove = 32;
+    constexpr int kWholeKeys = 512, kBlocksAbove = 32, kBlocksLead = 8, kAttendLead = 2;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
@@ -832,7 +832,8 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->sms = sms;
     d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
     d->most_waves = d->blocks ? 1 : 5;
-    const long long units = whole ? 1 : (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
+    d->lead = whole ? 0 : d->blocks ? kBlocksLead : kAttendLead;
+    const long long units = whole ? 1 : d->lead + (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
     if (units * a->batch * d->items > INT32_MAX) return DLM_ERR_SHAPE;
     const Cut cut = attend_cut(static_cast<uint32_t>(units * a->batch * d->items), d->resident, d->least_shift, d->most_waves);
     d->grid = cut.across * cut.waves;

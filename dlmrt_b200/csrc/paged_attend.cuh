@@ -7,6 +7,9 @@
 // not read equally fast: with one run for each CTA the slowest came in 30 % behind the others. Requests go on across items and
 // runs. An item that lies in several runs leaves a partial result in each, which join_kernel adds up in their order: the
 // result does not depend on which CTA took which run.
+//
+// An item's beginning and end take time, too: its units begin with `lead` units without keys that stand for it. A run that
+// holds only such units of an item leaves it to the next one.
 #pragma once
 
 #include <climits>
@@ -32,7 +35,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttendDev& p, int index, b
     if (tell && s.length != length) report_index(p.a.cache.status, index, kIndexLength, length);
     s.first_pos = s.length - p.a.tokens;
     s.base = (p.a.window > 0 ? max(0, s.first_pos - p.a.window + 1) : 0) & ~(kTileKeys - 1);
-    s.units = max(1, static_cast<int>((static_cast<uint32_t>(s.length - s.base) + (1u << p.unit_shift) - 1) >> p.unit_shift));
+    s.units = p.lead + max(1, static_cast<int>((static_cast<uint32_t>(s.length - s.base) + (1u << p.unit_shift) - 1) >> p.unit_shift));
     return s;
 }
 // Keys that a token sees: [seen_from, seen_to).
@@ -215,11 +218,12 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
         const int first_row = work.row_tile * p.tile_rows, last_row = min(first_row + p.tile_rows, p.rows) - 1;
         lo = seen_from(p, s.first_pos, token_of(p, first_row));
         const int hi = seen_to(p, s.first_pos, s.length, token_of(p, last_row));
-        work.whole = units == s.units;
-        work.piece = run * 2 + (first == 0);  // a run has at most one that began before it and one that goes on
-        work.start = max(s.base + (first << p.unit_shift), lo & ~(kTileKeys - 1));  // first is 0 if units are whole items
-        work.end = first + units == s.units ? hi : min(hi, s.base + ((first + units) << p.unit_shift));
-        work.tiles = work.end > work.start ? (work.end - work.start + kTileKeys - 1) / kTileKeys : 0;
+        const int end = first + units - p.lead, begin = max(0, first - p.lead);  // in units with keys
+        work.whole = first <= p.lead && first + units == s.units;
+        work.piece = run * 2 + (first <= p.lead);  // a run has at most one that began before it and one that goes on
+        work.start = max(s.base + (begin << p.unit_shift), lo & ~(kTileKeys - 1));  // begin is 0 if units are whole items
+        work.end = first + units == s.units ? hi : min(hi, s.base + (max(0, end) << p.unit_shift));
+        work.tiles = end <= 0 ? -1 : work.end > work.start ? (work.end - work.start + kTileKeys - 1) / kTileKeys : 0;
         tile = 0;
         if (work.tiles > 0) look_up(work.start >> p.page_shift);
     };
@@ -267,6 +271,7 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
         const int now_tile = tile, now_lo = lo;
         const int now_pages = pages, now_window = window;
         more = advance();
+        if (now.tiles < 0) continue;  // the next run's
         if (now_tile == 0) announce(now);
         if (now.tiles == 0) continue;
         const int key0 = now.start + now_tile * kTileKeys;
@@ -332,7 +337,7 @@ struct SplitItem {
             sequence = b / p.items, index = b - sequence * p.items;
             const Sequence s = sequence_of(p, sequence, false);
             const uint32_t begin = line.in_front_of(p, sequence) + index * s.units;
-            run = line.run_of(begin), last = line.run_of(begin + s.units - 1);
+            run = line.run_of(begin + p.lead), last = line.run_of(begin + s.units - 1);
             split = last != run;
         } else {
             run = b;
@@ -344,7 +349,7 @@ struct SplitItem {
             index = static_cast<int>((run_end - 1 - in_front) / static_cast<uint32_t>(s.units));
             const uint32_t begin = in_front + index * s.units;
             last = line.run_of(begin + s.units - 1);
-            split = begin >= run_begin && last != run;
+            split = begin + p.lead >= run_begin && begin + p.lead < run_end && last != run;
         }
         head = index / p.row_tiles, row_tile = index - head * p.row_tiles;
     }
