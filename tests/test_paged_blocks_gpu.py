@@ -94,6 +94,27 @@ def test_the_same_bits_and_graphs():
     assert torch.equal(outs[0], first) and torch.equal(outs[1], want)
 
 
+@pytest.mark.parametrize("t, hq, hk, d", [(1, 8, 2, 128), (64, 8, 2, 128), (64, 8, 2, 64), (48, 8, 2, 256)])
+def test_the_same_bits_whichever_cta_takes_a_run(t, hq, hk, d):
+    """Two calls at once share the SMs, so that runs go to whoever is free, after another number of steps each time."""
+    kv, q, table, lengths = setup([900, 300, 2000], t, hq, hk, d, 16, BF16, BF16)
+    queries = (q, q.flip(0).contiguous())
+    want = [kv.attend(x, table, lengths) for x in queries]
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph, x in zip(graphs, queries):
+        with torch.cuda.graph(graph):
+            outs.append(kv.attend(x, table, lengths))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(100):
+        for _ in range(5):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    kv.check()
+
+
 @pytest.mark.parametrize("t, hq, hk, d", [(1, 8, 2, 128), (40, 2, 1, 64), (64, 8, 2, 128), (70, 4, 2, 256)])
 def test_calls_in_turn_do_not_see_each_others_scratch(t, hq, hk, d):
     """Two calls on other inputs in turn, whose scratch torch's allocator puts in the same place: a result that was joined too
