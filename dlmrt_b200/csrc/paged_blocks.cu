@@ -103,9 +103,8 @@ __device__ __forceinline__ void rows_sync(int quarter) {
         tcgen05_fence_after();
     }
 }
-template <int kGroups>
-__device__ __forceinline__ bool rows_any(int quarter, bool vote) {
-    if constexpr (kGroups == 1) return __any_sync(0xFFFFFFFFu, vote);
+template <int kThreads>
+__device__ __forceinline__ bool any_of(int barrier, bool vote) {
     int any;
     asm volatile(
         "{\n"
@@ -115,10 +114,17 @@ __device__ __forceinline__ bool rows_any(int quarter, bool vote) {
         "selp.s32 %0, 1, 0, q;\n"
         "}\n"
         : "=r"(any)
-        : "r"(static_cast<int>(vote)), "r"(quarter + 1), "n"(kGroups * 32)
+        : "r"(static_cast<int>(vote)), "r"(barrier), "n"(kThreads)
         : "memory");
     return any != 0;
 }
+template <int kGroups>
+__device__ __forceinline__ bool rows_any(int quarter, bool vote) {
+    if constexpr (kGroups == 1) return __any_sync(0xFFFFFFFFu, vote);
+    return any_of<kGroups * 32>(quarter + 1, vote);
+}
+// The warps of a group meet.
+__device__ __forceinline__ bool group_any(int group, bool vote) { return any_of<kGroupThreads>(group + 5, vote); }
 
 // 16-byte piece `c` of row `r` of a tile of 128 rows, in column blocks of 128 bytes under the 128-byte swizzle.
 __device__ __forceinline__ uint4* tile_piece(uint8_t* tile, int r, int c) {
@@ -352,23 +358,32 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                 tmem_store_32(s_at, weights);
                 if (edge) {
                     // Values that are not finite, in keys that some rows see and others do not, or that are not there: 0 * inf
-                    // would reach the result. Their keys are found by every warp for itself.
+                    // would reach the result. Where there are any, every warp finds their keys for itself.
                     uint8_t* values = smem + stage * 2 * kBytes + kBytes;
                     auto piece = [&](int key, int c) {  // 16 bytes of a key's row
                         return reinterpret_cast<uint4*>(values + (c / 8) * kBlockBytes + key * 128 + ((c % 8) ^ (key & 7)) * 16);
                     };
+                    uint32_t odd = 0;  // a quarter of the keys each warp, loads in flight together: 32 in a row took a microsecond
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const int at = i * 32 + lane;
+                        const uint4 v = *piece(quarter * 16 + at / (D / 8), at % (D / 8));
+                        odd |= not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w);
+                    }
                     uint64_t bad = 0;
+                    if (group_any(group, odd != 0)) {
 #pragma unroll 1
-                    for (int i = 0; i < 2; ++i) {
-                        const int key = lane + 32 * i;
-                        bool any = false;
-                        if (by_row || !(present >> key & 1)) {
-                            for (int c = 0; c < D / 8; ++c) {
-                                const uint4 v = *piece(key, c);
-                                any |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
+                        for (int i = 0; i < 2; ++i) {
+                            const int key = lane + 32 * i;
+                            bool any = false;
+                            if (by_row || !(present >> key & 1)) {
+                                for (int c = 0; c < D / 8; ++c) {
+                                    const uint4 v = *piece(key, c);
+                                    any |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
+                                }
                             }
+                            bad |= static_cast<uint64_t>(__ballot_sync(0xFFFFFFFFu, any)) << (32 * i);
                         }
-                        bad |= static_cast<uint64_t>(__ballot_sync(0xFFFFFFFFu, any)) << (32 * i);
                     }
                     if (bad != 0) {  // the same in all warps of the group
                         uint64_t weightless = 0;  // keys whose weight is zero here: 0 * inf is NaN
