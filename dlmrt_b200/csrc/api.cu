@@ -818,7 +818,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->group = a->q_heads / a->cache.heads;
     d->rows = a->tokens * d->group;
     d->blocks = a->cache.type != DLM_E4M3 && d->rows > kBlocksAbove;
-    d->tile_rows = d->blocks ? kBlockRows : kRowTile;
+    d->tile_rows = d->blocks ? kBlockRows : d->rows <= kFewRows ? kFewRows : kRowTile;
     d->row_tiles = (d->rows + d->tile_rows - 1) / d->tile_rows;
     d->rows_cap = d->rows < d->tile_rows ? d->rows : d->tile_rows;
     if (static_cast<long long>(a->cache.heads) * d->row_tiles > 1 << 20) return DLM_ERR_SHAPE;
@@ -830,7 +830,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->unit_shift = whole ? 31 : kUnitShift;
     d->least_shift = whole ? 0 : 1;
     d->sms = sms;
-    d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim);
+    d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim, d->tile_rows);
     d->most_waves = d->blocks ? 1 : 5;
     d->lead = whole ? 0 : d->blocks ? kBlocksLead : kAttendLead;
     const long long units = whole ? 1 : d->lead + (span + kTileKeys - 1) / kTileKeys;  // of an item, at most

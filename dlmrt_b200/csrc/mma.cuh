@@ -42,6 +42,13 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t sme
                  : "memory");
 }
 
+// The 8x8 matrix whose row lane / 4 has this lane's two 16-bit elements in columns 2 (lane % 4) and the next, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+    uint32_t out;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(out) : "r"(v));
+    return out;
+}
+
 // 16 bytes to shared memory past L1; zeros (and no read) where `present` is false.
 __device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem, bool present) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(present ? 16 : 0)

@@ -3,11 +3,12 @@
 //
 //   o = sum_j exp(s_j) v_j / sum_j exp(s_j),   s_j = scale * q . k_j over the keys that the row's token sees
 //
-// One pass over the keys with a running maximum m and sum l per row: a tile's new maximum m' rescales what is there by
-// exp2(m - m') (all exponents in base 2, scale * log2(e) folded into the scores).
+// One pass over the keys with a running maximum m and sum l per row (all exponents in base 2, scale * log2(e) folded into the
+// scores). What is there is rescaled by exp2(m - m') once a new maximum m' is more than 8 above m: weights up to 2^8 fit.
 //
-// The rows that share a key head are its query heads times the new tokens; 16 of them make the M of an mma.sync. A single
-// token fills a few rows and is bound by reading the cache, so the tensor instructions only have to keep up with HBM.
+// The rows that share a key head are its query heads times the new tokens. 8 or 16 of them are the N of an mma.sync, 16 keys
+// (then 16 elements of the output) its M: S^T = K Q^T, O^T = V^T P^T. A single token fills a few rows and is bound by reading
+// the cache, so the tensor instructions only have to keep up with HBM; with rows as M half of them or more would be idle.
 //
 //   warp 4     deals out the work and requests keys and values: steps of 64 keys into a ring of stages, as TMA boxes of a
 //              page's slots (pages in any order; up to 64 slots a box). See paged_attend.cuh.
@@ -24,6 +25,7 @@ namespace {
 constexpr int kConsumers = 4;                            // warps that compute
 constexpr int kAttendThreads = (kConsumers + 1) * 32;
 constexpr int kWarpKeys = kTileKeys / kConsumers;        // 16
+constexpr float kRescaleAbove = 8.f;
 
 // A stage: 64 keys, then 64 values, as TMA writes them: box by box (a page's slots, at most 64), in a box column blocks of up
 // to 128 bytes, in each the rows one after the other with their 16-byte pieces permuted by row (the 128- or 64-byte swizzle),
@@ -55,17 +57,18 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 }
 
 // Shared memory of a CTA, and how many CTAs an SM holds of it (registers are held to what they leave each other).
-template <int D, bool kCodes>
+template <int D, bool kCodes, int kRows>
 struct AttendSmem {
-    static constexpr int kCtas = D == 64 ? 3 : D == 256 && !kCodes ? 1 : 2;
-    static constexpr int kStages = D == 64 ? (kCodes ? 6 : 4) : D == 128 && kCodes ? 6 : 3;
+    static constexpr bool kThree = D == 64 || (D == 256 && kCodes && kRows == 8);
+    static constexpr int kCtas = kThree ? 3 : D == 256 && !kCodes ? 1 : 2;
+    static constexpr int kStages = D == 64 ? (kCodes ? 6 : 4) : D == 128 && kCodes ? 6 : kThree ? 2 : 3;
     static constexpr int kRing = kStages * 2 * Stage<D, kCodes>::kBytes;
     static constexpr int kPitch = D + 4;
     static constexpr int kJoinRows = D == 256 ? 2 : 4;  // rows of a tile that the warps exchange at a time
     static constexpr int kJoin = kConsumers * kJoinRows * kPitch * 4;
     static constexpr bool kQueriesInShared = D == 256;  // 64 registers of queries and 128 of output leave too few
-    static constexpr int kQueries = kQueriesInShared ? D / 16 * 512 : 0;  // A operands of all k16 steps, in the order of lanes
-    static constexpr int kWeights = kConsumers * kRowTile * (kWarpKeys + 1) * 4;
+    static constexpr int kQueries = kQueriesInShared ? D * kRows * 2 : 0;  // B operands of all k16 steps, in the order of lanes
+    static constexpr int kWeights = kConsumers * kRows * (kWarpKeys + 1) * 4;
     static constexpr int kUsed = kQueries + kWeights;    // while keys are read; the join uses the same bytes afterwards
     static constexpr int kBytes = kRing + (kJoin > kUsed ? kJoin : kUsed) + 1024;  // the ring begins at a multiple of 1024
 };
@@ -90,19 +93,21 @@ __device__ __forceinline__ bool consumers_any(bool vote) {
 }  // namespace
 
 // T: type of queries and output. Products are of T, or of halves where the cache holds FP8 codes (every code is a half).
-template <typename T, int D, bool kCodes>
-__global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) attend_kernel(const __grid_constant__ AttendDev p) {
+template <typename T, int D, bool kCodes, int kRows>
+__global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::kCtas) attend_kernel(const __grid_constant__ AttendDev p) {
     using M = typename std::conditional<kCodes, __half, T>::type;
     using S = Stage<D, kCodes>;
-    using Shared = AttendSmem<D, kCodes>;
+    using Shared = AttendSmem<D, kCodes, kRows>;
     constexpr int kStages = Shared::kStages;
     constexpr int kSteps = D / 16;       // k16 steps of q . k
-    constexpr int kOut = D / 8;          // n8 tiles of the output
+    constexpr int kOut = D / 16;         // m16 tiles of the output
+    constexpr int kN = kRows / 8;        // n8 tiles of rows
+    constexpr int kChains = 4 / kN;      // sums of products that go on side by side
     constexpr int kElem = kCodes ? 1 : 2;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ Pipes<kStages> pipes;
-    __shared__ float warp_stats[kConsumers][kRowTile][2];
+    __shared__ float warp_stats[kConsumers][kRows][2];
 
     const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const bool leader = elect_one();
@@ -135,71 +140,61 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
     if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
     if (item.head < 0) return;
     const int sequence = item.sequence, head = item.head, row_tile = item.row_tile;
-    // This thread's two rows: g and g + 8 of the tile.
-    const int row0 = row_tile * kRowTile + g, row1 = row0 + 8;
-    const int token0 = token_of(p, min(row0, p.rows - 1)), token1 = token_of(p, min(row1, p.rows - 1));
-    const int from0 = seen_from(p, item.first_pos, token0), to0 = seen_to(p, item.first_pos, item.length, token0);
-    const int from1 = seen_from(p, item.first_pos, token1), to1 = seen_to(p, item.first_pos, item.length, token1);
-    const int last_row = min(row_tile * kRowTile + kRowTile, p.rows) - 1;
-    const int all_from = seen_from(p, item.first_pos, token_of(p, last_row));                          // from here on every row sees
-    const int all_to = seen_to(p, item.first_pos, item.length, token_of(p, row_tile * kRowTile));    // the keys, up to here
+    const int first_row = row_tile * kRows, last_row = min(first_row + kRows, p.rows) - 1;
+    const int all_from = seen_from(p, item.first_pos, token_of(p, last_row));               // from here on every row sees
+    const int all_to = seen_to(p, item.first_pos, item.length, token_of(p, first_row));   // the keys, up to here
+    // Keys that a row of the tile sees; this thread has the scores of rows 8 n + 2 t + e.
+    auto sees = [&](int row, int* from, int* to) {
+        const int token = token_of(p, min(first_row + row, last_row));
+        *from = seen_from(p, item.first_pos, token), *to = seen_to(p, item.first_pos, item.length, token);
+    };
 
     auto q_row = [&](int row) -> const T* {
         const int token = token_of(p, row), of = row - token * p.group;
         return static_cast<const T*>(p.a.q) + sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
                static_cast<long long>(head * p.group + of) * p.a.q_strides[2];
     };
-    // Queries as the A operand. With FP8 keys a lane's elements of a k16 step are four neighbours (see below).
-    uint32_t q[kSteps][4];
-    const bool has0 = row0 < p.rows, has1 = row1 < p.rows;
-    const T* q0 = has0 ? q_row(row0) : nullptr;
-    const T* q1 = has1 ? q_row(row1) : nullptr;
+    // Queries as the B operand: row 8 n + g. With FP8 keys a lane's elements of a k16 step are four neighbours (see below).
+    uint32_t q[kSteps][kN][2];
+    float scale[kN][2];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int at0 = s * 16 + t * (kCodes ? 4 : 2);
-        const int at1 = at0 + (kCodes ? 2 : 8);
-        q[s][0] = has0 ? *reinterpret_cast<const uint32_t*>(q0 + at0) : 0;
-        q[s][1] = has1 ? *reinterpret_cast<const uint32_t*>(q1 + at0) : 0;
-        q[s][2] = has0 ? *reinterpret_cast<const uint32_t*>(q0 + at1) : 0;
-        q[s][3] = has1 ? *reinterpret_cast<const uint32_t*>(q1 + at1) : 0;
-    }
-    float scale0 = p.a.scale * kLog2e, scale1 = scale0;
-    if constexpr (kCodes) {
-        // A BF16 row may not fit a half: it is scaled by the power of two that brings its largest element below 2 (exact,
-        // but for elements 2^-14 of the largest, whose error is at most 2^-25 of it), and the scores are scaled back. (A query
-        // as the sum of two E4M3 values, and FP8 products: 170 us against 110 for 24 sequences of 12000 keys, heads of 256.)
-        const float key_scale = p.a.cache.k_scale[head];
-        scale0 *= key_scale, scale1 *= key_scale;
-        float top0 = 0.f, top1 = 0.f;
+    for (int n = 0; n < kN; ++n) {
+        const int row = first_row + 8 * n + g;
+        const T* from = row <= last_row ? q_row(row) : nullptr;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                const float2 a = widen2<T>(q[s][i]), b = widen2<T>(q[s][i + 1]);
-                top0 = fmaxf(top0, fmaxf(fabsf(a.x), fabsf(a.y)));
-                top1 = fmaxf(top1, fmaxf(fabsf(b.x), fabsf(b.y)));
-            }
+            const int at = s * 16 + t * (kCodes ? 4 : 2);
+            q[s][n][0] = from != nullptr ? *reinterpret_cast<const uint32_t*>(from + at) : 0;
+            q[s][n][1] = from != nullptr ? *reinterpret_cast<const uint32_t*>(from + at + (kCodes ? 2 : 8)) : 0;
         }
+        scale[n][0] = scale[n][1] = p.a.scale * kLog2e;
+        if constexpr (kCodes) {
+            // A BF16 row may not fit a half: it is scaled by the power of two that brings its largest element below 2 (exact,
+            // but for elements 2^-14 of the largest, whose error is at most 2^-25 of it), and the scores are scaled back. (A
+            // query as the sum of two E4M3 values, and FP8 products: 170 us against 110 for 24 sequences of 12000 keys, heads
+            // of 256.)
+            float top = 0.f;
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            top0 = fmaxf(top0, __shfl_xor_sync(0xFFFFFFFFu, top0, o));
-            top1 = fmaxf(top1, __shfl_xor_sync(0xFFFFFFFFu, top1, o));
-        }
-        // 2^-e and 2^e for the exponent e of the largest element, kept where both are normal numbers.
-        const int e0 = min(max(static_cast<int>(__float_as_uint(top0) >> 23) - 127, -100), 126);
-        const int e1 = min(max(static_cast<int>(__float_as_uint(top1) >> 23) - 127, -100), 126);
-        const float down0 = __uint_as_float(static_cast<uint32_t>(127 - e0) << 23);
-        const float down1 = __uint_as_float(static_cast<uint32_t>(127 - e1) << 23);
-        scale0 *= __uint_as_float(static_cast<uint32_t>(127 + e0) << 23);
-        scale1 *= __uint_as_float(static_cast<uint32_t>(127 + e1) << 23);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 a = widen2<T>(q[s][i]);
-                const float down = i & 1 ? down1 : down0;
-                q[s][i] = narrow2<__half>(a.x * down, a.y * down);
+            for (int s = 0; s < kSteps; ++s) {
+                const float2 a = widen2<T>(q[s][n][0]), b = widen2<T>(q[s][n][1]);
+                top = fmaxf(fmaxf(top, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(b.x), fabsf(b.y)));
             }
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+            // 2^-e and 2^e for the exponent e of the largest element, kept where both are normal numbers.
+            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 126);
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 a = widen2<T>(q[s][n][i]);
+                    q[s][n][i] = narrow2<__half>(a.x * down, a.y * down);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                scale[n][i] = scale[n][i] * p.a.cache.k_scale[head] * __shfl_sync(0xFFFFFFFFu, up, (2 * t + i) * 4);
         }
     }
     const uint32_t* shared_q = nullptr;
@@ -207,17 +202,23 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         uint32_t* to = reinterpret_cast<uint32_t*>(smem + Shared::kRing);
         if (warp == 0) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-                *reinterpret_cast<uint4*>(to + (s * 32 + lane) * 4) = make_uint4(q[s][0], q[s][1], q[s][2], q[s][3]);
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int n = 0; n < kN; ++n) *reinterpret_cast<uint2*>(to + ((s * kN + n) * 32 + lane) * 2) = make_uint2(q[s][n][0], q[s][n][1]);
+            }
         }
         consumers_sync();
-        shared_q = to + lane * 4;
+        shared_q = to + lane * 2;
     }
 
-    float o[kOut][4];
+    float o[kOut][kN][4];  // [element g of 16 (FP8: 2 g)][row 2 t], [the same][2 t + 1], then element g + 8 (2 g + 1)
+    float m[kN][2], l[kN][2];  // l: of this thread's keys
 #pragma unroll
-    for (int i = 0; i < kOut; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+        m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+    }
 
     for (int tile = 0; tile < item.tiles; ++tile) {
         if (!mbar_wait_warp(&pipes.full[stage], parity, deadline) && leader) stalled(p, 4, tile);
@@ -226,86 +227,104 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
         const uint32_t stage_k32 = smem_u32(stage_k), stage_v32 = stage_k32 + S::kBytes;
         const uint32_t present = static_cast<uint32_t>(pipes.present[stage] >> (warp * kWarpKeys)) & 0xFFFFu;
 
-        auto query_step = [&](int k, uint32_t (&a)[4]) {
-            if constexpr (Shared::kQueriesInShared) {
-                const uint4 v = *reinterpret_cast<const uint4*>(shared_q + k * 128);
-                a[0] = v.x, a[1] = v.y, a[2] = v.z, a[3] = v.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = q[k][i];
-            }
+        auto query_step = [&](int k, int n) {
+            if constexpr (Shared::kQueriesInShared) return *reinterpret_cast<const uint2*>(shared_q + (k * kN + n) * 64);
+            else return make_uint2(q[k][n][0], q[k][n][1]);
         };
-        // scores: columns are keys, 0..7 in s[0], 8..15 in s[1]
-        float s[2][4] = {};
+        // scores: [key g][row 2 t], [key g][row 2 t + 1], then key g + 8
+        float s[kN][4], sums[kChains][kN][4];
+        const int r = lane & 15;
+#pragma unroll
+        for (int c = 0; c < kChains; ++c) {
+#pragma unroll
+            for (int n = 0; n < kN; ++n) sums[c][n][0] = sums[c][n][1] = sums[c][n][2] = sums[c][n][3] = 0.f;
+        }
         if constexpr (!kCodes) {
-            const int r = (lane & 7) + ((lane >> 4) << 3);
-            float more_s[2][4] = {};  // odd steps: half as long a chain of dependent products
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-                uint32_t a[4], b[4];
-                query_step(k, a);
-                ldmatrix_x4(b, stage_k32 + rows_of_stage.at(r, 2 * k + ((lane >> 3) & 1)));
-                mma_16816<M>(k & 1 ? more_s[0] : s[0], a, b[0], b[1]);
-                mma_16816<M>(k & 1 ? more_s[1] : s[1], a, b[2], b[3]);
-            }
+                uint32_t a[4];
+                ldmatrix_x4(a, stage_k32 + rows_of_stage.at(r, 2 * k + (lane >> 4)));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i], s[1][i] += more_s[1][i];
+                for (int n = 0; n < kN; ++n) {
+                    const uint2 b = query_step(k, n);
+                    mma_16816<M>(sums[k % kChains][n], a, b.x, b.y);
+                }
+            }
         } else {
             // A 16-byte piece of a key row is one k16 step: lane t of a row holds its elements 4t .. 4t + 3.
-            const int r = (lane & 7) + (((lane >> 3) & 1) << 3);
-            float more_s[2][4] = {};
 #pragma unroll
             for (int k = 0; k < kSteps; k += 2) {
-                uint32_t a0[4], a1[4], b[4];
-                query_step(k, a0);
-                query_step(k + 1, a1);
-                ldmatrix_x4(b, stage_k32 + rows_of_stage.at(r, k + (lane >> 4)));
-                mma_16816<M>(s[0], a0, e4m3x2_to_f16x2(b[0] & 0xFFFFu), e4m3x2_to_f16x2(b[0] >> 16));
-                mma_16816<M>(s[1], a0, e4m3x2_to_f16x2(b[1] & 0xFFFFu), e4m3x2_to_f16x2(b[1] >> 16));
-                mma_16816<M>(more_s[0], a1, e4m3x2_to_f16x2(b[2] & 0xFFFFu), e4m3x2_to_f16x2(b[2] >> 16));
-                mma_16816<M>(more_s[1], a1, e4m3x2_to_f16x2(b[3] & 0xFFFFu), e4m3x2_to_f16x2(b[3] >> 16));
-            }
+                uint32_t w[4];
+                ldmatrix_x4(w, stage_k32 + rows_of_stage.at(r, k + (lane >> 4)));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[0][i] += more_s[0][i], s[1][i] += more_s[1][i];
-        }
-        const bool by_row = key0 < all_from || key0 + kWarpKeys > all_to;  // rows see different keys of this tile
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t a[4] = {e4m3x2_to_f16x2(w[2 * c] & 0xFFFFu), e4m3x2_to_f16x2(w[2 * c + 1] & 0xFFFFu),
+                                           e4m3x2_to_f16x2(w[2 * c] >> 16), e4m3x2_to_f16x2(w[2 * c + 1] >> 16)};
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            s[n][0] *= scale0, s[n][1] *= scale0, s[n][2] *= scale1, s[n][3] *= scale1;
-        }
-        if (by_row || present != 0xFFFFu) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int c = 8 * n + 2 * t + e, key = key0 + c;
-                    const bool there = (present >> c) & 1;
-                    if (!there || key < from0 || key >= to0) s[n][e] = -INFINITY;
-                    if (!there || key < from1 || key >= to1) s[n][2 + e] = -INFINITY;
+                    for (int n = 0; n < kN; ++n) {
+                        const uint2 b = query_step(k + c, n);
+                        mma_16816<M>(sums[(k + c) % kChains][n], a, b.x, b.y);
+                    }
                 }
             }
         }
-        float top0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-        float top1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
 #pragma unroll
-        for (int x = 1; x < 4; x <<= 1) {
-            top0 = fmaxf(top0, __shfl_xor_sync(0xFFFFFFFFu, top0, x));
-            top1 = fmaxf(top1, __shfl_xor_sync(0xFFFFFFFFu, top1, x));
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (kChains == 4) s[n][e] = (sums[0][n][e] + sums[1][n][e]) + (sums[2][n][e] + sums[3][n][e]);
+                else s[n][e] = sums[0][n][e] + sums[1][n][e];
+                s[n][e] *= scale[n][e & 1];
+            }
         }
-        if (__any_sync(0xFFFFFFFFu, top0 > m0 || top1 > m1)) {
-            const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1);
-            const float f0 = m0 == n0 ? 1.f : exp2_approx(m0 - n0), f1 = m1 == n1 ? 1.f : exp2_approx(m1 - n1);
-            m0 = n0, m1 = n1;
-            l0 *= f0, l1 *= f1;
+        const bool by_row = key0 < all_from || key0 + kWarpKeys > all_to;  // rows see different keys of this tile
+        if (by_row || present != 0xFFFFu) {
 #pragma unroll
-            for (int i = 0; i < kOut; ++i) o[i][0] *= f0, o[i][1] *= f0, o[i][2] *= f1, o[i][3] *= f1;
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    int from, to;
+                    sees(8 * n + 2 * t + e, &from, &to);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = g + 8 * h, key = key0 + c;
+                        if (!(present >> c & 1) || key < from || key >= to) s[n][2 * h + e] = -INFINITY;
+                    }
+                }
+            }
         }
-        const float sub0 = m0 == -INFINITY ? 0.f : m0, sub1 = m1 == -INFINITY ? 0.f : m1;
+        bool rescale = false;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            s[n][0] = exp2_approx(s[n][0] - sub0), s[n][1] = exp2_approx(s[n][1] - sub0);
-            s[n][2] = exp2_approx(s[n][2] - sub1), s[n][3] = exp2_approx(s[n][3] - sub1);
-            l0 += s[n][0] + s[n][1], l1 += s[n][2] + s[n][3];
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float top = fmaxf(s[n][e], s[n][2 + e]);
+                rescale |= top > m[n][e] + kRescaleAbove || (m[n][e] == -INFINITY && top > m[n][e]);
+            }
+        }
+        if (__any_sync(0xFFFFFFFFu, rescale)) {
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[n][e], s[n][2 + e]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                    const float now = fmaxf(m[n][e], top), f = m[n][e] == now ? 1.f : exp2_approx(m[n][e] - now);
+                    m[n][e] = now, l[n][e] *= f;
+#pragma unroll
+                    for (int i = 0; i < kOut; ++i) o[i][n][e] *= f, o[i][n][2 + e] *= f;
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float sub = m[n][e] == -INFINITY ? 0.f : m[n][e];
+                s[n][e] = exp2_approx(s[n][e] - sub), s[n][2 + e] = exp2_approx(s[n][2 + e] - sub);
+                l[n][e] += s[n][e] + s[n][2 + e];
+            }
         }
 
         // Values that are not finite, in a key that some rows see and others do not, or that is not there at all: 0 * inf
@@ -320,31 +339,44 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             for (int i = lane; i < kWords; i += 32) apart |= not_finite<M, kCodes>(*word(i)) != 0;
             if (__any_sync(0xFFFFFFFFu, apart)) {
                 float* weights = reinterpret_cast<float*>(smem + Shared::kRing + Shared::kQueries);
-                float(&w)[kRowTile][kWarpKeys + 1] = reinterpret_cast<float(*)[kRowTile][kWarpKeys + 1]>(weights)[warp];
+                float(&w)[kRows][kWarpKeys + 1] = reinterpret_cast<float(*)[kRows][kWarpKeys + 1]>(weights)[warp];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    w[g][8 * n + 2 * t] = s[n][0], w[g][8 * n + 2 * t + 1] = s[n][1];
-                    w[g + 8][8 * n + 2 * t] = s[n][2], w[g + 8][8 * n + 2 * t + 1] = s[n][3];
+                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[8 * n + 2 * t + (e & 1)][g + 8 * (e >> 1)] = s[n][e];
                 }
                 __syncwarp();
 #pragma unroll 1
                 for (int c = 0; c < kWarpKeys; ++c) {
                     const int key = key0 + c;
-                    const bool there = (present >> c) & 1;
-                    const bool see0 = there && key >= from0 && key < to0, see1 = there && key >= from1 && key < to1;
-                    const float w0 = w[g][c], w1 = w[g + 8][c];
+                    float weight[kN][2];
+                    bool see[kN][2];
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            int from, to;
+                            sees(8 * n + 2 * t + e, &from, &to);
+                            see[n][e] = (present >> c & 1) && key >= from && key < to;
+                            weight[n][e] = w[8 * n + 2 * t + e][c];
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < kOut; ++i) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int byte = (kCodes ? (i / 2) * 16 + 4 * t + 2 * e + (i & 1) : 8 * i + 2 * t + e) * kElem;
+                        for (int h = 0; h < 2; ++h) {
+                            const int byte = kCodes ? 16 * i + 2 * g + h : (16 * i + g + 8 * h) * 2;
                             const uint8_t* at = stage_k + S::kBytes + rows_of_stage.at(c, byte / 16) + byte % 16;
                             float v;
                             if constexpr (kCodes) v = widen2<__half>(e4m3x2_to_f16x2(*at)).x;
                             else v = widen2<M>(*reinterpret_cast<const uint16_t*>(at)).x;
                             if (!isfinite(v)) {
-                                if (see0) o[i][e] += w0 * v;
-                                if (see1) o[i][2 + e] += w1 * v;
+#pragma unroll
+                                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e)
+                                        if (see[n][e]) o[i][n][2 * h + e] += weight[n][e] * v;
+                                }
                             }
                         }
                     }
@@ -356,25 +388,35 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
             }
         }
         {
-            uint32_t a[4] = {narrow2<M>(s[0][0], s[0][1]), narrow2<M>(s[0][2], s[0][3]), narrow2<M>(s[1][0], s[1][1]),
-                             narrow2<M>(s[1][2], s[1][3])};
-            const int r = (lane & 7) + (((lane >> 3) & 1) << 3);
+            uint32_t b[kN][2];  // the weights, rows from key g to row g
 #pragma unroll
-            for (int i = 0; i < S::kPieces / 2; ++i) {
-                uint32_t b[4];
-                ldmatrix_x4_trans(b, stage_v32 + rows_of_stage.at(r, 2 * i + (lane >> 4)));
-                if constexpr (!kCodes) {
-                    mma_16816<M>(o[2 * i], a, b[0], b[1]);
-                    mma_16816<M>(o[2 * i + 1], a, b[2], b[3]);
-                } else {
-                    // b[0], b[1]: keys 2t, 2t + 1 (+ 8) of elements 2g and 2g + 1 of a 16-byte piece; b[2], b[3]: the next
-                    // piece. One product takes the even elements, one the odd ones.
+            for (int n = 0; n < kN; ++n) {
+                b[n][0] = transpose_8x8(narrow2<M>(s[n][0], s[n][1]));
+                b[n][1] = transpose_8x8(narrow2<M>(s[n][2], s[n][3]));
+            }
+            if constexpr (!kCodes) {
+                const int key = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                for (int i = 0; i < kOut; ++i) {
+                    uint32_t a[4];
+                    ldmatrix_x4_trans(a, stage_v32 + rows_of_stage.at(key, 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) mma_16816<M>(o[i][n], a, b[n][0], b[n][1]);
+                }
+            } else {
+                // w[0], w[1]: keys 2t, 2t + 1 (+ 8) of elements 2g and 2g + 1 of a 16-byte piece; w[2], w[3]: the next piece. The
+                // even elements are the product's first eight rows, the odd ones its last.
+#pragma unroll
+                for (int i = 0; i < kOut; i += 2) {
+                    uint32_t w[4];
+                    ldmatrix_x4_trans(w, stage_v32 + rows_of_stage.at(r, i + (lane >> 4)));
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const uint32_t even0 = __byte_perm(b[2 * c], 0, 0x4420), odd0 = __byte_perm(b[2 * c], 0, 0x4431);
-                        const uint32_t even1 = __byte_perm(b[2 * c + 1], 0, 0x4420), odd1 = __byte_perm(b[2 * c + 1], 0, 0x4431);
-                        mma_16816<M>(o[4 * i + 2 * c], a, e4m3x2_to_f16x2(even0), e4m3x2_to_f16x2(even1));
-                        mma_16816<M>(o[4 * i + 2 * c + 1], a, e4m3x2_to_f16x2(odd0), e4m3x2_to_f16x2(odd1));
+                        const uint32_t a[4] = {
+                            e4m3x2_to_f16x2(__byte_perm(w[2 * c], 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(w[2 * c], 0, 0x4431)),
+                            e4m3x2_to_f16x2(__byte_perm(w[2 * c + 1], 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(w[2 * c + 1], 0, 0x4431))};
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) mma_16816<M>(o[i + c][n], a, b[n][0], b[n][1]);
                     }
                 }
             }
@@ -386,38 +428,40 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
 
     // -- the four warps' results, a few rows at a time ---------------------------------------------------------------
 #pragma unroll
-    for (int x = 1; x < 4; x <<= 1) {
-        l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, x);
-        l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, x);
-    }
-    if (t == 0) {
-        warp_stats[warp][g][0] = m0, warp_stats[warp][g][1] = l0;
-        warp_stats[warp][g + 8][0] = m1, warp_stats[warp][g + 8][1] = l1;
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xFFFFFFFFu, l[n][e], x);
+            if (g == 0) warp_stats[warp][8 * n + 2 * t + e][0] = m[n][e], warp_stats[warp][8 * n + 2 * t + e][1] = l[n][e];
+        }
     }
     consumers_sync();
-    {
-        float n0 = -INFINITY, n1 = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kConsumers; ++w) n0 = fmaxf(n0, warp_stats[w][g][0]), n1 = fmaxf(n1, warp_stats[w][g + 8][0]);
-        // A warp that met no visible key has all zeros, or NaN times zero from a score that was NaN: kept as it is.
-        const float f0 = m0 == -INFINITY ? 0.f : exp2_approx(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2_approx(m1 - n1);
+    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int i = 0; i < kOut; ++i) o[i][0] *= f0, o[i][1] *= f0, o[i][2] *= f1, o[i][3] *= f1;
+        for (int e = 0; e < 2; ++e) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kConsumers; ++w) top = fmaxf(top, warp_stats[w][8 * n + 2 * t + e][0]);
+            // A warp that met no visible key has all zeros, or NaN times zero from a score that was NaN: kept as it is.
+            const float f = m[n][e] == -INFINITY ? 0.f : exp2_approx(m[n][e] - top);
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) o[i][n][e] *= f, o[i][n][2 + e] *= f;
+        }
     }
-    const int rows = min(kRowTile, p.rows - row_tile * kRowTile);
+    const int rows = last_row + 1 - first_row;
     const float value_scale = kCodes ? p.a.cache.v_scale[head] : 1.f;
     float* joined = reinterpret_cast<float*>(smem + Shared::kRing);
     for (int r0 = 0; r0 < rows; r0 += Shared::kJoinRows) {
-        if ((g & ~(Shared::kJoinRows - 1)) == (r0 & 7)) {
-            float* to = joined + (warp * Shared::kJoinRows + (g & (Shared::kJoinRows - 1))) * Shared::kPitch;
+        if ((2 * t & ~(Shared::kJoinRows - 1)) == (r0 & 7)) {
+            float* to = joined + (warp * Shared::kJoinRows + (2 * t & (Shared::kJoinRows - 1))) * Shared::kPitch;
 #pragma unroll
             for (int i = 0; i < kOut; ++i) {
-                const float x = r0 < 8 ? o[i][0] : o[i][2], y = r0 < 8 ? o[i][1] : o[i][3];
-                if constexpr (!kCodes) {
-                    *reinterpret_cast<float2*>(to + 8 * i + 2 * t) = make_float2(x, y);
-                } else {
-                    const int d = (i / 2) * 16 + 4 * t + (i & 1);
-                    to[d] = x, to[d + 2] = y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 16 * i + (kCodes ? 2 * g + (e >> 1) : g + 8 * (e >> 1));
+                    to[(e & 1) * Shared::kPitch + d] = r0 < 8 ? o[i][0][e] : o[i][kN - 1][e];
                 }
             }
         }
@@ -438,7 +482,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes>::kCtas) 
                 l += warp_stats[w][r][1] * (m == -INFINITY ? 0.f : exp2_approx(m - top));
             }
             if (item.whole) {
-                finish_row<T>(p, sequence, head, row_tile * kRowTile + r, d, sum, top, l, value_scale);
+                finish_row<T>(p, sequence, head, first_row + r, d, sum, top, l, value_scale);
             } else {
                 const int piece = item.piece * p.rows_cap + r;
                 *reinterpret_cast<float4*>(p.partial + static_cast<size_t>(piece) * D + d) = sum;
@@ -463,7 +507,7 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
     float2* stats = reinterpret_cast<float2*>(sums + blockDim.x);
     const int across = D / 4 / gridDim.z, lines = blockDim.x / across;  // threads along a row, and how often
     const SplitItem item(p, blockIdx.x);
-    const int run = item.run, last = item.last, head = item.head, first_row = item.row_tile * kRowTile;
+    const int run = item.run, last = item.last, head = item.head, first_row = item.row_tile * p.tile_rows;
     // Every block waits, those without work too: this kernel's end stands for the end of the one in front.
     pdl_wait();
     pdl_launch_dependents();
@@ -530,10 +574,10 @@ __global__ void __launch_bounds__(kJoinMostThreads) join_kernel(const __grid_con
     }
 }
 
-template <typename T, int D, bool kCodes>
+template <typename T, int D, bool kCodes, int kRows>
 static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
     void* args[] = {const_cast<AttendDev*>(&p)};
-    const int rc = launch_kernel<attend_kernel<T, D, kCodes>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes>::kBytes, args, o);
+    const int rc = launch_kernel<attend_kernel<T, D, kCodes, kRows>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes, kRows>::kBytes, args, o);
     if (rc != 0 || p.partial == nullptr) return rc;
     // With fewer items than runs an item may have hundreds of partial results: large blocks, one for a quarter of each row (293
     // partial results of a row: 7 us in blocks of a whole row, all of it latency). Otherwise it has two or three, and most blocks
@@ -551,12 +595,15 @@ static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
 
 // Calls f with the type and the sizes of a call as compile-time constants.
 template <typename F>
-static int by_type(int type, int cache_type, int head_dim, F f) {
+static int by_type(int type, int cache_type, int head_dim, int tile_rows, F f) {
+    auto by_rows = [&](auto t, auto codes, auto dim) {
+        return tile_rows == kFewRows ? f(t, dim, codes, std::integral_constant<int, kFewRows>{}) : f(t, dim, codes, std::integral_constant<int, kRowTile>{});
+    };
     auto by_dim = [&](auto t, auto codes) {
         switch (head_dim) {
-            case 64: return f(t, std::integral_constant<int, 64>{}, codes);
-            case 128: return f(t, std::integral_constant<int, 128>{}, codes);
-            default: return f(t, std::integral_constant<int, 256>{}, codes);
+            case 64: return by_rows(t, codes, std::integral_constant<int, 64>{});
+            case 128: return by_rows(t, codes, std::integral_constant<int, 128>{});
+            default: return by_rows(t, codes, std::integral_constant<int, 256>{});
         }
     };
     auto by_codes = [&](auto t) { return cache_type == DLM_E4M3 ? by_dim(t, std::true_type{}) : by_dim(t, std::false_type{}); };
@@ -565,14 +612,15 @@ static int by_type(int type, int cache_type, int head_dim, F f) {
 
 int launch_attend(const AttendDev& p, const LaunchOpts& o) {
     if (p.blocks) return launch_blocks(p, o);
-    return by_type(p.a.type, p.a.cache.type, p.a.cache.head_dim, [&](auto t, auto dim, auto codes) {
-        return launch_attend_t<decltype(t), decltype(dim)::value, decltype(codes)::value>(p, o);
+    return by_type(p.a.type, p.a.cache.type, p.a.cache.head_dim, p.tile_rows, [&](auto t, auto dim, auto codes, auto rows) {
+        return launch_attend_t<decltype(t), decltype(dim)::value, decltype(codes)::value, decltype(rows)::value>(p, o);
     });
 }
 
-int attend_ctas_per_sm(int type, int cache_type, int head_dim) {
-    return by_type(type, cache_type, head_dim,
-                   [&](auto, auto dim, auto codes) { return AttendSmem<decltype(dim)::value, decltype(codes)::value>::kCtas; });
+int attend_ctas_per_sm(int type, int cache_type, int head_dim, int tile_rows) {
+    return by_type(type, cache_type, head_dim, tile_rows, [&](auto, auto dim, auto codes, auto rows) {
+        return AttendSmem<decltype(dim)::value, decltype(codes)::value, decltype(rows)::value>::kCtas;
+    });
 }
 
 }  // namespace dlm

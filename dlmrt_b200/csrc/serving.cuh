@@ -20,7 +20,7 @@ __device__ __forceinline__ void report_index(int* status, int row, int kind, int
     }
 }
 
-constexpr int kRowTile = 16;     // rows of an item: the M of its matrix instructions
+constexpr int kFewRows = 8, kRowTile = 16;  // rows of an item: the N of its matrix instructions, once or twice
 constexpr int kBlockRows = 128;  // the same in the kernel for blocks of tokens
 constexpr int kUnitShift = 6, kTileKeys = 1 << kUnitShift;  // keys of a step, and of the units that items are cut into
 
@@ -33,7 +33,7 @@ struct alignas(64) AttendDev {
     int page_shift;
     int group;         // query heads of a key head
     int rows;          // tokens * group rows share a key head's keys
-    int tile_rows;     // rows of an item: kRowTile, or kBlockRows in the kernel for blocks of tokens
+    int tile_rows;     // rows of an item: kFewRows, kRowTile, or kBlockRows in the kernel for blocks of tokens
     int row_tiles;     // of tile_rows rows
     int rows_cap;      // rows of a tile that exist: min(tile_rows, rows)
     int blocks;        // the kernel for blocks of tokens takes this call
@@ -65,7 +65,7 @@ __host__ __device__ inline Cut attend_cut(uint32_t total, int resident, int leas
 int launch_append(const DlmAppend& p, int page_shift, const LaunchOpts& o);
 int launch_attend(const AttendDev& p, const LaunchOpts& o);
 int launch_blocks(const AttendDev& p, const LaunchOpts& o);
-int attend_ctas_per_sm(int type, int cache_type, int head_dim);
+int attend_ctas_per_sm(int type, int cache_type, int head_dim, int tile_rows);
 int launch_adapters(const DlmAdapters& p, const LaunchOpts& o);
 
 }  // namespace dlm
