@@ -806,7 +806,11 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
 
 // Everything about an attention call that its device pointers do not decide.
 static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
-    constexpr int kWholeKeys = 512, kBlocksAbove = 32, kBlocksLead = 8, kAttendLead = 2;
+    // Blocks of tokens have a kernel of their own from more rows on than the other one has in a tile. It reads the cache once for
+    // 128 rows, and takes longer to begin and to end: 64 sequences of up to 6001 keys, 28 rows, heads of 64 / 128 / 256: 33 / 38
+    // / 85 us against 45 / 65 / 141; nine sequences: 14.6 / 20 / 27 against 13.4 / 16 / 32. With 16 rows, one tile: 33 / 37 / 84
+    // against 31 / 45 / 100, and 14.4 / 18 / 26 against 12.5 / 14.4 / 23.
+    constexpr int kWholeKeys = 512, kBlocksAbove = kRowTile, kBlocksLead = 8, kAttendLead = 2;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;

@@ -59,9 +59,9 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 // Shared memory of a CTA, and how many CTAs an SM holds of it (registers are held to what they leave each other).
 template <int D, bool kCodes, int kRows>
 struct AttendSmem {
-    static constexpr bool kThree = D == 64 || (D == 256 && kCodes && kRows == 8);
+    static constexpr bool kThree = D == 64 || (kCodes && kRows == 8);
     static constexpr int kCtas = kThree ? 3 : D == 256 && !kCodes ? 1 : 2;
-    static constexpr int kStages = D == 64 ? (kCodes ? 6 : 4) : D == 128 && kCodes ? 6 : kThree ? 2 : 3;
+    static constexpr int kStages = D == 64 ? (kCodes ? 6 : 4) : D == 128 && kCodes ? (kThree ? 4 : 6) : kThree ? 2 : 3;
     static constexpr int kRing = kStages * 2 * Stage<D, kCodes>::kBytes;
     static constexpr int kPitch = D + 4;
     static constexpr int kJoinRows = D == 256 ? 2 : 4;  // rows of a tile that the warps exchange at a time
@@ -103,7 +103,6 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
     constexpr int kOut = D / 16;         // m16 tiles of the output
     constexpr int kN = kRows / 8;        // n8 tiles of rows
     constexpr int kChains = 4 / kN;      // sums of products that go on side by side
-    constexpr int kElem = kCodes ? 1 : 2;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ Pipes<kStages> pipes;
@@ -579,8 +578,9 @@ static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
     void* args[] = {const_cast<AttendDev*>(&p)};
     const int rc = launch_kernel<attend_kernel<T, D, kCodes, kRows>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes, kRows>::kBytes, args, o);
     if (rc != 0 || p.partial == nullptr) return rc;
-    // With fewer items than runs an item may have hundreds of partial results: large blocks, one for a quarter of each row (293
-    // partial results of a row: 7 us in blocks of a whole row, all of it latency). Otherwise it has two or three, and most blocks
+    // With far fewer items than runs an item may have hundreds of partial results: large blocks, one for a quarter of each row
+    // (293 partial results of a row: 7 us in blocks of a whole row, all of it latency; up to 64 runs an item small blocks are
+    // faster: 18 items in 592 runs, rows of 16: 14.4 us in all against 19.7). Otherwise it has two or three, and most blocks
     // only find out that there is nothing to join (0.5 us; 9000 blocks took 25).
     const long long items = static_cast<long long>(p.a.batch) * p.items;
     const LaunchOpts dependent{o.stream, true, false};  // always a dependent launch of the kernel above
@@ -589,8 +589,9 @@ static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
                                                 threads * 16 + threads * splits / (D / 4) * 8, args, dependent);
     };
     if (!p.by_item) return join(static_cast<unsigned>(p.grid), 1, 1, 256);
-    const int rows = static_cast<int>(p.sms * 2 / items);
-    return p.grid > 32 * items ? join(static_cast<unsigned>(items), rows, 4, kJoinMostThreads) : join(static_cast<unsigned>(items), rows, 1, 256);
+    const bool deep = p.grid > 64 * items;
+    const int splits = deep ? 4 : 1, rows = static_cast<int>(p.sms * 2 / (items * splits));  // two blocks an SM
+    return join(static_cast<unsigned>(items), rows, splits, deep ? kJoinMostThreads : 256);
 }
 
 // Calls f with the type and the sizes of a call as compile-time constants.
