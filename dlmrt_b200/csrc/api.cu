@@ -821,7 +821,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     if (a->cache.type != DLM_E4M3 && a->cache.type != a->type) return DLM_ERR_SHAPE;
     d->group = a->q_heads / a->cache.heads;
     d->rows = a->tokens * d->group;
-    d->blocks = a->cache.type != DLM_E4M3 && d->rows > kBlocksAbove;
+    d->blocks = d->rows > kBlocksAbove;
     d->tile_rows = d->blocks ? kBlockRows : d->rows <= kFewRows ? kFewRows : kRowTile;
     d->row_tiles = (d->rows + d->tile_rows - 1) / d->tile_rows;
     d->rows_cap = d->rows < d->tile_rows ? d->rows : d->tile_rows;

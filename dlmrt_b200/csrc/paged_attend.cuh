@@ -307,7 +307,7 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
         for (int j = 0; j < boxes; ++j) {
             const int from = __shfl_sync(0xFFFFFFFFu, page, j);
             const int at = (key0 + j * box_keys) & slot_mask;
-            const int box = j * box_keys * (kApart ? 128 : kPieces * 16);
+            const int box = j * box_keys * (kApart && kPieces > 8 ? 128 : kPieces * 16);
             if (leader && !failed) {
 #pragma unroll
                 for (int c = 0; c < kBlocks; ++c) {

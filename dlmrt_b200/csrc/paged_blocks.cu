@@ -6,6 +6,8 @@
 //              their sum. Two groups take steps in turn, each with its own maximum, sum and O, and put them together at an
 //              item's end (heads of 256 leave tensor memory for one).
 //   producer   a warp, see paged_attend.cuh.
+//   converters (FP8 cache) warps that widen a step's codes to halves, exactly, and lay them out as TMA lays out 16-bit keys and
+//              values. Queries are halves, too, each row scaled by a power of two.
 //   issuer     a warp that issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory,
 //              V as it lies, its 64 keys down the rows). Each group has two buffers of S: its next step's scores are computed
 //              under this one's softmax.
@@ -25,17 +27,21 @@ namespace {
 constexpr int kGroupThreads = 128;
 constexpr float kRescaleAbove = 8.f;
 
-template <int D>
+template <int D, bool kCodes>
 struct BlockShape {
     static constexpr int kGroups = D == 256 ? 1 : 2;
     static constexpr int kBuffers = 2 * kGroups;              // of S
     static constexpr int kProducerWarp = 4 * kGroups, kIssuerWarp = kProducerWarp + 1;
-    static constexpr int kThreads = kGroups * kGroupThreads + 64;
-    static constexpr int kStages = D == 256 ? 2 : D == 128 ? 5 : 8;
-    static constexpr int kBytes = kTileKeys * D * 2;          // keys, or values, of a stage
-    static constexpr int kRing = kStages * 2 * kBytes;
+    static constexpr int kConverters = !kCodes ? 0 : D == 256 ? 4 : 2;  // 12 warps leave the softmax its 168 registers
+    static constexpr int kThreads = kGroups * kGroupThreads + 64 + kConverters * 32;
+    static constexpr int kSteps = D == 256 ? 2 : kCodes ? (D == 128 ? 3 : 6) : D == 128 ? 5 : 8;  // whose operands are there
+    static constexpr int kStages = !kCodes ? kSteps : D == 256 ? 1 : D == 128 ? 5 : 8;             // of what TMA brings
+    static constexpr int kBytes = kTileKeys * D * 2;          // keys, or values, of a step
+    static constexpr int kCodeBytes = kTileKeys * D;
+    static constexpr int kSteady = kSteps * 2 * kBytes;
     static constexpr int kQueries = kBlockRows * D * 2;
-    static constexpr int kAll = kRing + kQueries + 1024;      // the ring begins at a multiple of 1024
+    static constexpr int kRing = kSteady + kQueries;          // where stages of codes begin
+    static constexpr int kAll = kRing + (kCodes ? kStages * 2 * kCodeBytes : 0) + 1024;  // it begins at a multiple of 1024
     static constexpr uint32_t kColumns = 512;                 // of tensor memory: an O of each group, then the buffers of S
 };
 
@@ -152,27 +158,60 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return __vcmpeq2(w & kExponent, kExponent);
 }
 
+// 8 elements of a row, the rest of which kLanes neighbouring lanes have, to halves: scaled by the power of two that brings the
+// row's largest element below 2 (see attend_kernel). Returns what undoes it.
+template <typename T, int kLanes>
+__device__ __forceinline__ float to_halves(uint4* v) {
+    uint32_t(&w)[4] = reinterpret_cast<uint32_t(&)[4]>(*v);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = widen2<T>(w[i]);
+        top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+    }
+#pragma unroll
+    for (int x = 1; x < kLanes; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 126);
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = widen2<T>(w[i]);
+        w[i] = narrow2<__half>(x.x * down, x.y * down);
+    }
+    return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
 }  // namespace
 
-template <typename T, int D>
-__global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(const __grid_constant__ AttendDev p) {
-    using Shape = BlockShape<D>;
-    constexpr int kStages = Shape::kStages, kBytes = Shape::kBytes, kGroups = Shape::kGroups, kBuffers = Shape::kBuffers;
+// T: type of queries and output. Products are of T, or of halves where the cache holds FP8 codes.
+template <typename T, int D, bool kCodes>
+__global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_kernel(const __grid_constant__ AttendDev p) {
+    using Shape = BlockShape<D, kCodes>;
+    using M = typename std::conditional<kCodes, __half, T>::type;
+    constexpr int kStages = Shape::kStages, kSteps = Shape::kSteps, kBytes = Shape::kBytes, kGroups = Shape::kGroups, kBuffers = Shape::kBuffers;
     constexpr int kBlockBytes = kTileKeys * 128;  // 64 keys of a column block of 64 elements
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* queries = smem + Shape::kRing;
+    uint8_t* queries = smem + Shape::kSteady;
     __shared__ Pipes<kStages> pipes;
     // Queries written; of the step that a buffer of S is for: scores computed, weights written, values consumed; a side step of
     // a group. A wait can only tell a phase from the one before it, which here is kBuffers steps back.
     __shared__ uint64_t q_full, s_full[kBuffers], p_full[kBuffers], pv_done[kBuffers], aside[kGroups];
+    // FP8: what the producer's barriers are to the converters, these are to the issuer.
+    __shared__ uint64_t wide_full[kSteps], wide_empty[kSteps], wide_present[kSteps];
+    uint64_t* const step_full = kCodes ? wide_full : pipes.full;
+    uint64_t* const step_empty = kCodes ? wide_empty : pipes.empty;
+    uint64_t* const step_present = kCodes ? wide_present : pipes.present;
     __shared__ uint32_t tmem_base;
+    __shared__ float row_scale[kCodes ? kBlockRows : 1];
     __shared__ float2 group_stats[kGroups][kBlockRows];  // maximum and sum of a group's steps
 
     const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const bool leader = elect_one();
     if (warp == Shape::kProducerWarp && leader) {
-        pipes.init(1, kGroups * 4 + 1);
+        pipes.init(kCodes ? Shape::kConverters : 1, kGroups * 4 + 1 + Shape::kConverters);
+        if constexpr (kCodes)
+            for (int i = 0; i < kSteps; ++i) mbar_init(&wide_full[i], Shape::kConverters), mbar_init(&wide_empty[i], 1);
         mbar_init(&q_full, kGroups * kGroupThreads);
         for (int i = 0; i < kBuffers; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kGroupThreads), mbar_init(&pv_done[i], 1);
         for (int i = 0; i < kGroups; ++i) mbar_init(&aside[i], kGroupThreads);
@@ -193,10 +232,11 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
     pdl_launch_dependents();
 
     if (warp == Shape::kProducerWarp) {
-        produce<kStages, D / 8, true>(p, smem, pipes, deadline, leader);
+        if constexpr (kCodes) produce<kStages, D / 16, true>(p, smem + Shape::kRing, pipes, deadline, leader);
+        else produce<kStages, D / 8, true>(p, smem, pipes, deadline, leader);
     } else if (warp == Shape::kIssuerWarp) {
         // -- the issuer: a whole warp on uniform values, one lane issuing ------------------------------------------------
-        constexpr uint32_t kIdescS = idesc_f16<T>(kBlockRows, kTileKeys, false), kIdescO = idesc_f16<T>(kBlockRows, D, true);
+        constexpr uint32_t kIdescS = idesc_f16<M>(kBlockRows, kTileKeys, false), kIdescO = idesc_f16<M>(kBlockRows, D, true);
         const uint64_t q_desc = umma_desc_k128(queries);
         int stage = 0, slot = 0, next_stage = 0;
         uint32_t parity = 0, slot_parity = 0, q_parity = 0, step = 0;
@@ -219,7 +259,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
             wait(&q_full, q_parity, 6, tiles);
             q_parity ^= 1;
             auto scores = [&](uint32_t n) {  // of step n, whose keys are the next stage's
-                wait(&pipes.full[next_stage], parity, 7, n);
+                wait(&step_full[next_stage], parity, 7, n);
                 const uint32_t keys = smem_u32(smem) + next_stage * 2 * kBytes;
                 const uint64_t k_desc = (q_desc & 0xFFFFFFFF00000000ull) | (umma_desc_k128(smem) & 0xFFFF0000u) | ((keys & 0x3FFFF) >> 4);
                 if (leader) {
@@ -229,7 +269,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                                   k_desc + (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, kIdescS, k != 0);
                     umma_commit(&s_full[buffer(n)]);
                 }
-                if (++next_stage == kStages) next_stage = 0, parity ^= 1;
+                if (++next_stage == kSteps) next_stage = 0, parity ^= 1;
             };
             for (int ahead = 0; ahead < kGroups && ahead < tiles; ++ahead) scores(step + ahead);
             for (int tile = 0; tile < tiles; ++tile, ++step) {
@@ -246,10 +286,74 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                     for (int k = 0; k < kTileKeys / 16; ++k)
                         umma_f16_ts(tmem + step % kGroups * D, tmem_s + buffer(step) * 64 + k * 8, umma_desc_mn128(values + k * 2048, kBlockBytes),
                                     kIdescO);
-                    umma_commit(&pipes.empty[stage]);
+                    umma_commit(&step_empty[stage]);
                     umma_commit(&pv_done[buffer(step)]);
                 }
-                if (++stage == kStages) stage = 0;
+                if (++stage == kSteps) stage = 0;
+            }
+        }
+    } else if (kCodes && warp > Shape::kIssuerWarp) {
+        // -- the converters: pieces of 16 codes ------------------------------------------------------------------------------
+        constexpr int kPieces = D / 16, kRowBytes = kPieces < 8 ? D : 128, kAtOnce = 4;
+        constexpr int kTurns = 2 * kTileKeys * kPieces / 32 / (kCodes ? Shape::kConverters : 1);  // of a warp; half of them keys
+        const int part = warp - Shape::kIssuerWarp - 1;
+        int stage = 0, step = 0, slot = 0;
+        uint32_t parity = 0, step_parity = 1, slot_parity = 0;
+        while (true) {
+            const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
+            if (!announced) {
+                if (leader) stalled(p, 16, slot);
+                break;
+            }
+            const int head = pipes.works[slot].head, tiles = pipes.works[slot].tiles;
+            __syncwarp();
+            if (leader) mbar_arrive(&pipes.work_empty[slot]);
+            if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
+            if (head < 0) break;
+            for (int tile = 0; tile < tiles; ++tile) {
+                if (!mbar_wait_warp(&pipes.full[stage], parity, deadline) && leader) stalled(p, 17, tile);
+                if (!mbar_wait_warp(&wide_empty[step], step_parity, deadline) && leader) stalled(p, 18, tile);
+                const uint8_t* codes = smem + Shape::kRing + stage * 2 * Shape::kCodeBytes;
+                uint8_t* wide = smem + step * 2 * kBytes;
+                // Eight lanes take four pieces of two keys k and k ^ 5, which puts both their reads and their writes (every other
+                // piece of a row) on different banks.
+                auto place = [&](int i, int* key, int* c) {
+                    const int at = (i * Shape::kConverters + part) * 4 + (lane >> 3), half = at % (kTileKeys / 2);
+                    *key = (half * 2) ^ (lane & 4 ? 5 : 0);
+                    *c = at / (kTileKeys / 2) * 4 + (lane & 3);
+                };
+#pragma unroll 1
+                for (int i0 = 0; i0 < kTurns; i0 += kAtOnce) {
+                    const bool values = i0 >= kTurns / 2;
+                    const uint8_t* from = codes + (values ? Shape::kCodeBytes : 0);
+                    uint8_t* to = wide + (values ? kBytes : 0);
+                    uint4 v[kAtOnce];
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        int key, c;
+                        place(i0 + j - (values ? kTurns / 2 : 0), &key, &c);
+                        const int turn = kPieces < 8 ? (key >> 1) & 3 : key & 7;
+                        v[j] = *reinterpret_cast<const uint4*>(from + (c / 8) * (kTileKeys * 128) + key * kRowBytes + ((c % 8) ^ turn) * 16);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        int key, c;
+                        place(i0 + j - (values ? kTurns / 2 : 0), &key, &c);
+                        uint8_t* row = to + (c / 4) * kBlockBytes + key * 128;
+                        auto pair = [&](uint32_t a, uint32_t b) {
+                            return make_uint4(e4m3x2_to_f16x2(a & 0xFFFFu), e4m3x2_to_f16x2(a >> 16), e4m3x2_to_f16x2(b & 0xFFFFu),
+                                              e4m3x2_to_f16x2(b >> 16));
+                        };
+                        *reinterpret_cast<uint4*>(row + ((2 * c % 8) ^ (key & 7)) * 16) = pair(v[j].x, v[j].y);
+                        *reinterpret_cast<uint4*>(row + ((2 * c % 8 + 1) ^ (key & 7)) * 16) = pair(v[j].z, v[j].w);
+                    }
+                }
+                if (leader && part == 0) wide_present[step] = pipes.present[stage];
+                fence_proxy_async();
+                __syncwarp();
+                if (leader) mbar_arrive(&wide_full[step]), mbar_arrive(&pipes.empty[stage]);
+                if (++stage == kStages) stage = 0, parity ^= 1;
+                if (++step == kSteps) step = 0, step_parity ^= 1;
             }
         }
     } else {
@@ -257,7 +361,6 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
         const int quarter = warp & 3, group = warp >> 2, r = quarter * 32 + lane;
         const uint32_t mine = static_cast<uint32_t>(quarter * 32) << 16;  // this warp's lanes of tensor memory
         const uint32_t tmem_o = tmem + mine + group * D;
-        const float scale = p.a.scale * kLog2e;
         int stage = 0, slot = 0;
         uint32_t slot_parity = 0, step = 0, aside_parity = 0;
         auto wait = [&](uint64_t* bar, uint32_t bar_phase, int who, int at) {
@@ -284,8 +387,10 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                 const T* q = static_cast<const T*>(p.a.q) + item.sequence * p.a.q_strides[0] + token * p.a.q_strides[1] +
                              query_head * p.a.q_strides[2];
                 uint4 v[D / 8 / kGroups];
-                by_rows<D, kGroups>(row <= last_row ? q : nullptr, group, [&](int i, int, int c, const uint8_t* at) {
+                by_rows<D, kGroups>(row <= last_row ? q : nullptr, group, [&](int i, int at_row, int c, const uint8_t* at) {
                     v[i] = at != nullptr ? reinterpret_cast<const uint4*>(at)[c] : make_uint4(0, 0, 0, 0);
+                    // A BF16 row may not fit a half: see attend_kernel. Its D / 8 lanes have a piece each.
+                    if constexpr (kCodes) row_scale[quarter * 32 + at_row] = to_halves<T, D / 8>(&v[i]);
                 });
                 by_rows<D, kGroups>(nullptr, group, [&](int i, int at, int c, const uint8_t*) { *tile_piece(queries, quarter * 32 + at, c) = v[i]; });
                 fence_proxy_async();
@@ -297,12 +402,14 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                 for (int c = 0; c < D / 32; ++c) tmem_store_32(tmem_o + c * 32, zero);
                 tmem_store_wait();
             }
+            const float base_scale = p.a.scale * kLog2e * (kCodes ? p.a.cache.k_scale[item.head] : 1.f);
+            const float value_scale = kCodes ? p.a.cache.v_scale[item.head] : 1.f;
             float m = -INFINITY, l = 0.f;
             uint32_t own_steps = 0;  // of this group in this item
             const uint32_t first_step = step;
             for (int tile = 0; tile < item.tiles; ++tile, ++step) {
                 if (step % kGroups != static_cast<uint32_t>(group)) {
-                    if (++stage == kStages) stage = 0;
+                    if (++stage == kSteps) stage = 0;
                     continue;
                 }
                 const uint32_t s_at = tmem_s + mine + buffer(step) * 64, last_own = step - kGroups;
@@ -313,7 +420,8 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                 tmem_load_wait();
                 float (&s)[64] = reinterpret_cast<float(&)[64]>(raw);
                 const int key0 = item.start + tile * kTileKeys;
-                const uint64_t present = pipes.present[stage];
+                const uint64_t present = step_present[stage];
+                const float scale = kCodes ? base_scale * row_scale[r] : base_scale;  // written before the scores were computed
                 const bool by_row = key0 < all_from || key0 + kTileKeys > all_to;  // rows see different keys of this step
                 const bool edge = by_row || present != ~0ull;
 #pragma unroll
@@ -352,7 +460,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                 for (int j = 0; j < 64; j += 2) {
                     s[j] = exp2_approx(s[j] - sub), s[j + 1] = exp2_approx(s[j + 1] - sub);
                     sum4[j & 3] += s[j], sum4[(j + 1) & 3] += s[j + 1];
-                    weights[j / 2] = narrow2<T>(s[j], s[j + 1]);
+                    weights[j / 2] = narrow2<M>(s[j], s[j + 1]);
                 }
                 l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
                 tmem_store_32(s_at, weights);
@@ -368,7 +476,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                     for (int i = 0; i < D / 16; ++i) {
                         const int at = i * 32 + lane;
                         const uint4 v = *piece(quarter * 16 + at / (D / 8), at % (D / 8));
-                        odd |= not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w);
+                        odd |= not_finite<M>(v.x) | not_finite<M>(v.y) | not_finite<M>(v.z) | not_finite<M>(v.w);
                     }
                     uint64_t bad = 0;
                     if (group_any(group, odd != 0)) {
@@ -379,7 +487,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                             if (by_row || !(present >> key & 1)) {
                                 for (int c = 0; c < D / 8; ++c) {
                                     const uint4 v = *piece(key, c);
-                                    any |= (not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w)) != 0;
+                                    any |= (not_finite<M>(v.x) | not_finite<M>(v.y) | not_finite<M>(v.z) | not_finite<M>(v.w)) != 0;
                                 }
                             }
                             bad |= static_cast<uint64_t>(__ballot_sync(0xFFFFFFFFu, any)) << (32 * i);
@@ -402,7 +510,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
 #pragma unroll
                                 for (int j = 0; j < 32; j += 2) {
                                     const uint32_t w = reinterpret_cast<const uint32_t*>(piece(key, c * 4 + j / 8))[j / 2 % 4];
-                                    const float2 v = widen2<T>(w);
+                                    const float2 v = widen2<M>(w);
                                     const float none = weightless >> key & 1 ? NAN : 1.f;
                                     if (see && !isfinite(v.x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + v.x * none);
                                     if (see && !isfinite(v.y)) o[j + 1] = __float_as_uint(__uint_as_float(o[j + 1]) + v.y * none);
@@ -419,7 +527,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                             if ((key & 3) != quarter) continue;
                             for (int c = lane; c < D / 8; c += 32) {
                                 uint4 v = *piece(key, c);
-                                v.x &= ~not_finite<T>(v.x), v.y &= ~not_finite<T>(v.y), v.z &= ~not_finite<T>(v.z), v.w &= ~not_finite<T>(v.w);
+                                v.x &= ~not_finite<M>(v.x), v.y &= ~not_finite<M>(v.y), v.z &= ~not_finite<M>(v.z), v.w &= ~not_finite<M>(v.w);
                                 *piece(key, c) = v;
                             }
                         }
@@ -430,7 +538,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                 tcgen05_fence_before();
                 mbar_arrive(&p_full[buffer(step)]);
                 ++own_steps;
-                if (++stage == kStages) stage = 0;
+                if (++stage == kSteps) stage = 0;
             }
             // -- the row's result ---------------------------------------------------------------------------------------
             if (own_steps > 0) {
@@ -463,7 +571,7 @@ __global__ void __launch_bounds__(BlockShape<D>::kThreads, 1) blocks_kernel(cons
                         l == 0.f ? -INFINITY : (m + log2f(l)) * (1.f / kLog2e);
             }
             if (item.whole) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = l == 0.f ? 0.f : value_scale / l;
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) factors[i] *= inv;
             }
@@ -568,7 +676,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_blocks_kernel(const __gr
             }
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : (p.a.cache.type == DLM_E4M3 ? p.a.cache.v_scale[item.head] : 1.f) / l;
     const int token = token_of(p, min(row, p.rows - 1)), query_head = item.head * p.group + min(row, p.rows - 1) - token * p.group;
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
@@ -586,22 +694,25 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_blocks_kernel(const __gr
 
 int launch_blocks(const AttendDev& p, const LaunchOpts& o) {
     void* args[] = {const_cast<AttendDev*>(&p)};
-    auto run = [&](auto t, auto dim) {
+    auto run = [&](auto t, auto dim, auto codes) {
         using T = decltype(t);
         constexpr int kDim = decltype(dim)::value;
-        const int rc = launch_kernel<blocks_kernel<T, kDim>>(dim3(p.grid), dim3(BlockShape<kDim>::kThreads), BlockShape<kDim>::kAll, args, o);
+        constexpr bool kCodes = decltype(codes)::value;
+        using Shape = BlockShape<kDim, kCodes>;
+        const int rc = launch_kernel<blocks_kernel<T, kDim, kCodes>>(dim3(p.grid), dim3(Shape::kThreads), Shape::kAll, args, o);
         if (rc != 0 || p.partial == nullptr) return rc;
         return launch_kernel<join_blocks_kernel<T, kDim>>(dim3(p.by_item ? p.a.batch * p.items : p.grid, (p.rows_cap + kJoinRows - 1) / kJoinRows),
                                                           dim3(kJoinWarps * 32), 0, args, {o.stream, true, false});
     };
-    auto by_dim = [&](auto t) {
+    auto by_dim = [&](auto t, auto codes) {
         switch (p.a.cache.head_dim) {
-            case 64: return run(t, std::integral_constant<int, 64>{});
-            case 128: return run(t, std::integral_constant<int, 128>{});
-            default: return run(t, std::integral_constant<int, 256>{});
+            case 64: return run(t, std::integral_constant<int, 64>{}, codes);
+            case 128: return run(t, std::integral_constant<int, 128>{}, codes);
+            default: return run(t, std::integral_constant<int, 256>{}, codes);
         }
     };
-    return p.a.type == DLM_F16 ? by_dim(__half{}) : by_dim(__nv_bfloat16{});
+    auto by_codes = [&](auto t) { return p.a.cache.type == DLM_E4M3 ? by_dim(t, std::true_type{}) : by_dim(t, std::false_type{}); };
+    return p.a.type == DLM_F16 ? by_codes(__half{}) : by_codes(__nv_bfloat16{});
 }
 
 }  // namespace dlm

@@ -9,7 +9,7 @@ import serving_util as su
 from test_paged_attend_gpu import check, setup
 
 pytestmark = pytest.mark.gpu
-BF16, F16 = torch.bfloat16, torch.float16
+BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -21,11 +21,57 @@ def test_one_tile_of_rows(t, hq, hk, d, dtype):
     check(*setup([0, t, 640, 1029], t, hq, hk, d, 32, dtype, dtype))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t, hq, hk", [(17, 1, 1), (32, 8, 2), (43, 3, 1)])
+def test_one_tile_of_rows_over_codes(t, hq, hk, d, dtype):
+    check(*setup([t, 64, 65, 128, 300], t, hq, hk, d, 16, dtype, E4M3))
+    check(*setup([0, t, 640, 1029], t, hq, hk, d, 32, dtype, E4M3))
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("window", [0, 40, 600])
-def test_several_tiles_of_rows(d, causal, window):
-    check(*setup([200, 150, 700, 256], 150, 4, 2, d, 64, BF16, BF16), causal=causal, window=window)
+def test_several_tiles_of_rows(d, causal, window, cache):
+    check(*setup([200, 150, 700, 256], 150, 4, 2, d, 64, BF16, cache), causal=causal, window=window)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [8, 16, 64, 256])
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_pages_of_codes(page, layout, d):
+    check(*setup([70, 257], 40, 2, 1, d, page, BF16, E4M3, layout=layout))
+
+
+def test_queries_beyond_halves_over_codes():
+    """BF16 queries whose products with codes are taken in halves: rows of 1e5, of 1e-7, and one of zeros."""
+    kv, q, table, lengths = setup([300, 130], 40, 2, 1, 128, 16, BF16, E4M3)
+    q[:, 3] *= 1e5
+    q[:, 5] *= 1e-7
+    q[:, 7] = 0
+    for scale in (1e-6, 0.05):
+        check(kv, q[:, 4:], table, lengths, scale=scale)
+    check(kv, q, table, lengths, scale=1e-7)
+
+
+def test_codes_that_are_not_numbers():
+    """NaN codes behind the end, in front of the window and in later tokens' places stay out; a visible one reaches its rows."""
+    kv, q, table, lengths = setup([100, 53], 40, 2, 1, 64, 16, BF16, E4M3)
+    clean = kv.attend(q, table, lengths, causal=True, window=30)
+    used = torch.zeros(kv.keys.shape[0], 16, dtype=torch.bool)
+    for i, n in enumerate(lengths.tolist()):
+        for j in range(max(0, n - 40 - 30 + 1), n):
+            used[table[i, j // 16], j % 16] = True
+    for t in (kv.keys, kv.values):
+        t.view(torch.uint8).transpose(1, 2)[~used.cuda()] = 0x7F
+    assert torch.equal(kv.attend(q, table, lengths, causal=True, window=30), clean)
+    at = 100 - 40 + 35
+    kv.values.view(torch.uint8)[table[0, at // 16], :, at % 16, 5] = 0xFF
+    got = kv.attend(q, table, lengths, causal=True, window=30)
+    assert bool(got[0, 35:, :, 5].isnan().all())
+    got[0, 35:, :, 5] = clean[0, 35:, :, 5]
+    assert torch.equal(got, clean)
 
 
 @pytest.mark.parametrize("page", [8, 16, 64, 256])
