@@ -294,9 +294,13 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
         }
     } else if (kCodes && warp > Shape::kIssuerWarp) {
         // -- the converters: pieces of 16 codes ------------------------------------------------------------------------------
-        constexpr int kPieces = D / 16, kRowBytes = kPieces < 8 ? D : 128, kAtOnce = 4;
-        constexpr int kTurns = 2 * kTileKeys * kPieces / 32 / (kCodes ? Shape::kConverters : 1);  // of a warp; half of them keys
-        const int part = warp - Shape::kIssuerWarp - 1;
+        // Eight lanes take four pieces of two keys k and k ^ 5, which puts both their reads and their writes (every other piece of
+        // a row) on different banks. A turn goes on by a multiple of 8 keys, under the same swizzle, then by four pieces.
+        constexpr int kPieces = D / 16, kRowBytes = kPieces < 8 ? D : 128;
+        constexpr int kKeysATurn = 8 * (kCodes ? Shape::kConverters : 1), kTurns = kTileKeys * (kPieces / 4) / kKeysATurn;
+        const int part = warp - Shape::kIssuerWarp - 1, key0 = (part * 8 + (lane >> 3) * 2) ^ (lane & 4 ? 5 : 0);
+        const int first_code = key0 * kRowBytes + ((lane & 3) ^ (kPieces < 8 ? (key0 >> 1) & 3 : key0 & 7)) * 16;
+        const int first_wide = key0 * 128 + (((lane & 3) * 2) ^ (key0 & 7)) * 16;
         int stage = 0, step = 0, slot = 0;
         uint32_t parity = 0, step_parity = 1, slot_parity = 0;
         while (true) {
@@ -315,37 +319,25 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
                 if (!mbar_wait_warp(&wide_empty[step], step_parity, deadline) && leader) stalled(p, 18, tile);
                 const uint8_t* codes = smem + Shape::kRing + stage * 2 * Shape::kCodeBytes;
                 uint8_t* wide = smem + step * 2 * kBytes;
-                // Eight lanes take four pieces of two keys k and k ^ 5, which puts both their reads and their writes (every other
-                // piece of a row) on different banks.
-                auto place = [&](int i, int* key, int* c) {
-                    const int at = (i * Shape::kConverters + part) * 4 + (lane >> 3), half = at % (kTileKeys / 2);
-                    *key = (half * 2) ^ (lane & 4 ? 5 : 0);
-                    *c = at / (kTileKeys / 2) * 4 + (lane & 3);
-                };
 #pragma unroll 1
-                for (int i0 = 0; i0 < kTurns; i0 += kAtOnce) {
-                    const bool values = i0 >= kTurns / 2;
-                    const uint8_t* from = codes + (values ? Shape::kCodeBytes : 0);
-                    uint8_t* to = wide + (values ? kBytes : 0);
-                    uint4 v[kAtOnce];
+                for (int i = 0; i < 2; ++i) {  // keys, values
+                    const uint8_t* from = codes + i * Shape::kCodeBytes;
+                    uint8_t* to = wide + i * kBytes;
+                    uint4 v[kTurns];
 #pragma unroll
-                    for (int j = 0; j < kAtOnce; ++j) {
-                        int key, c;
-                        place(i0 + j - (values ? kTurns / 2 : 0), &key, &c);
-                        const int turn = kPieces < 8 ? (key >> 1) & 3 : key & 7;
-                        v[j] = *reinterpret_cast<const uint4*>(from + (c / 8) * (kTileKeys * 128) + key * kRowBytes + ((c % 8) ^ turn) * 16);
+                    for (int j = 0; j < kTurns; ++j) {
+                        const int key = j * kKeysATurn % kTileKeys, c = j * kKeysATurn / kTileKeys;  // from the first turn's
+                        v[j] = *reinterpret_cast<const uint4*>(from + (first_code ^ (c % 2 * 64)) + c / 2 * kBlockBytes + key * kRowBytes);
                     }
 #pragma unroll
-                    for (int j = 0; j < kAtOnce; ++j) {
-                        int key, c;
-                        place(i0 + j - (values ? kTurns / 2 : 0), &key, &c);
-                        uint8_t* row = to + (c / 4) * kBlockBytes + key * 128;
+                    for (int j = 0; j < kTurns; ++j) {
+                        const int key = j * kKeysATurn % kTileKeys, c = j * kKeysATurn / kTileKeys;
                         auto pair = [&](uint32_t a, uint32_t b) {
                             return make_uint4(e4m3x2_to_f16x2(a & 0xFFFFu), e4m3x2_to_f16x2(a >> 16), e4m3x2_to_f16x2(b & 0xFFFFu),
                                               e4m3x2_to_f16x2(b >> 16));
                         };
-                        *reinterpret_cast<uint4*>(row + ((2 * c % 8) ^ (key & 7)) * 16) = pair(v[j].x, v[j].y);
-                        *reinterpret_cast<uint4*>(row + ((2 * c % 8 + 1) ^ (key & 7)) * 16) = pair(v[j].z, v[j].w);
+                        *reinterpret_cast<uint4*>(to + first_wide + c * kBlockBytes + key * 128) = pair(v[j].x, v[j].y);
+                        *reinterpret_cast<uint4*>(to + (first_wide ^ 16) + c * kBlockBytes + key * 128) = pair(v[j].z, v[j].w);
                     }
                 }
                 if (leader && part == 0) wide_present[step] = pipes.present[stage];
