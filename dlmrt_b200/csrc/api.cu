@@ -810,7 +810,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     // 128 rows, and takes longer to begin and to end: 64 sequences of up to 6001 keys, 28 rows, heads of 64 / 128 / 256: 33 / 38
     // / 85 us against 45 / 65 / 141; nine sequences: 14.6 / 20 / 27 against 13.4 / 16 / 32. With 16 rows, one tile: 33 / 37 / 84
     // against 31 / 45 / 100, and 14.4 / 18 / 26 against 12.5 / 14.4 / 23.
-    constexpr int kWholeKeys = 512, kBlocksAbove = kRowTile, kBlocksLead = 8, kAttendLead = 2;
+    constexpr int kWholeKeys = 256, kBlocksAbove = kRowTile, kBlocksLead = 6, kAttendLead = 2;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
@@ -830,11 +830,19 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     long long span = keys;  // from the first key that some token sees, aligned down, to the last
     if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kTileKeys < span)
         span = static_cast<long long>(a->window) + a->tokens + kTileKeys;
-    const bool whole = span <= kWholeKeys;
+    // Short sequences: an item is one run, whose result needs no join. One CTA takes 0.8 us for a step of 64 keys in pages of 16;
+    // runs of two steps and their join 2 us in all. Tables of 256 keys, 1 / 8 / 64 sequences, 8 heads of 128: whole 8.2 / 8.5 / 15.6
+    // us, split 8.9 / 10.7 / 21.1; of 512 keys: whole 11.3 / 11.5 / 23.2, split 9.0 / 11.2 / 24.8; of 1024: 17.6 / 17.6 / 37.9
+    // against 9.1 / 11.6 / 34.4.
+    const bool whole = span <= (static_cast<long long>(a->batch) * d->items >= sms ? 2 * kWholeKeys : kWholeKeys);
     d->unit_shift = whole ? 31 : kUnitShift;
     d->least_shift = whole ? 0 : 1;
     d->sms = sms;
     d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim, d->tile_rows);
+    // What an item's beginning and end cost in units of 64 keys: 64 ragged sequences of up to 8192 keys 90.3 / 88.8 / 88.8 us with 0 /
+    // 2 / 4, FP8 heads of 256 85.4 / 84.6 / 88.2; blocks of 32 tokens 74 / 60.2 / 59.2 / 59.0 / 60.6 with 0 / 5 / 6 / 8 / 11, of 28
+    // rows 37.9 / 37.3 / 38.8 / 40.6 with 5 / 6 / 8 / 11. With more than one wave of runs blocks have more to join than they gain:
+    // 59.0 / 65.2 / 72.3 us with one, two, three.
     d->most_waves = d->blocks ? 1 : 5;
     d->lead = whole ? 0 : d->blocks ? kBlocksLead : kAttendLead;
     const long long units = whole ? 1 : d->lead + (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
