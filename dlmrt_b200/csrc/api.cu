@@ -759,6 +759,27 @@ static bool strides_ok(const int64_t* strides, const int* extents, int n, int of
     return true;
 }
 
+// The bytes of a tensor [outer, n, heads, head_dim] of 2-byte elements (strides of the first three; inner contiguous): rows of
+// `width` bytes, `step` apart. step 0: one row, or rows that no single step leads through.
+struct Footprint {
+    uintptr_t begin, end;
+    uint64_t step, width;
+    Footprint(const void* at, int64_t outer, int64_t outer_stride, int64_t n, int64_t stride, int64_t heads, int64_t head_stride, int64_t dim) {
+        width = static_cast<uint64_t>((heads - 1) * head_stride + dim) * 2;
+        begin = reinterpret_cast<uintptr_t>(at);
+        end = begin + static_cast<uint64_t>((outer - 1) * outer_stride + (n - 1) * stride) * 2 + width;
+        step = static_cast<uint64_t>(n > 1 ? stride : outer > 1 ? outer_stride : 0) * 2;
+        if (n > 1 && outer > 1 && stride > 0 && outer_stride % stride) step = 0;
+    }
+    // Whether two tensors share bytes, as far as can be told: rows side by side in the same longer rows do not.
+    bool meets(const Footprint& o) const {
+        if (end <= o.begin || o.end <= begin) return false;
+        if (step == 0 || step != o.step) return true;
+        const uint64_t ahead = o.begin >= begin ? (o.begin - begin) % step : (step - (begin - o.begin) % step) % step;
+        return ahead < width || step - ahead < o.width;
+    }
+};
+
 // log2 of the page size in *shift.
 static int check_pages(const DlmPages* c, int* shift) {
     if (c->keys == nullptr || c->values == nullptr) return DLM_ERR_NULL;
@@ -798,6 +819,16 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
     if (!strides_ok(a->k_strides, kv_extents, 2, 8, 0) || !strides_ok(a->v_strides, kv_extents, 2, 8, 0) ||
         (a->q != nullptr && (!strides_ok(a->q_strides, q_extents, 2, 8, 0) || !strides_ok(a->out_strides, q_extents, 2, 8, 1))))
         return DLM_ERR_ALIGN;
+    if (a->q != nullptr) {
+        const int dim = a->cache.head_dim;
+        const Footprint out(a->q_out, 1, 0, a->n, a->out_strides[0], a->q_heads, a->out_strides[1], dim);
+        const bool in_place = a->q == a->q_out && (a->n == 1 || a->q_strides[0] == a->out_strides[0]) &&
+                              (a->q_heads == 1 || a->q_strides[1] == a->out_strides[1]);
+        if (!in_place && out.meets(Footprint(a->q, 1, 0, a->n, a->q_strides[0], a->q_heads, a->q_strides[1], dim))) return DLM_ERR_OVERLAP;
+        if (out.meets(Footprint(a->k, 1, 0, a->n, a->k_strides[0], a->cache.heads, a->k_strides[1], dim)) ||
+            out.meets(Footprint(a->v, 1, 0, a->n, a->v_strides[0], a->cache.heads, a->v_strides[1], dim)))
+            return DLM_ERR_OVERLAP;
+    }
     DeviceInfo info;
     rc = device_info(&info);
     if (rc != DLM_OK) return rc;
@@ -816,7 +847,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
     if (a->q_heads < 1 || a->q_heads > 1024 || a->q_heads % a->cache.heads) return DLM_ERR_SHAPE;
     const long long keys = static_cast<long long>(a->table_pages) << d->page_shift;
-    if (keys > 1 << 30 || a->window < 0 || a->causal < 0 || a->causal > 1) return DLM_ERR_SHAPE;
+    if (keys > 1 << 30 || a->window < 0 || a->window > 1 << 30 || a->causal < 0 || a->causal > 1) return DLM_ERR_SHAPE;
     if (a->type != DLM_BF16 && a->type != DLM_F16) return DLM_ERR_SHAPE;
     if (a->cache.type != DLM_E4M3 && a->cache.type != a->type) return DLM_ERR_SHAPE;
     d->group = a->q_heads / a->cache.heads;
@@ -906,6 +937,14 @@ int dlm_paged_attend(const DlmAttend* a, dlm_stream_t stream) {
     const int extents[3] = {a->batch, a->tokens, a->q_heads};
     if (!strides_ok(a->q_strides, extents, 3, 8, 0) || !strides_ok(a->out_strides, extents, 3, 8, 1) || a->table_stride < 0)
         return DLM_ERR_ALIGN;
+    {
+        const int64_t *q = a->q_strides, *out = a->out_strides;
+        bool in_place = a->q == a->out;
+        for (int i = 0; i < 3; ++i) in_place = in_place && (extents[i] == 1 || q[i] == out[i]);
+        if (!in_place && Footprint(a->q, a->batch, q[0], a->tokens, q[1], a->q_heads, q[2], a->cache.head_dim)
+                             .meets(Footprint(a->out, a->batch, out[0], a->tokens, out[1], a->q_heads, out[2], a->cache.head_dim)))
+            return DLM_ERR_OVERLAP;
+    }
     DeviceInfo info;
     rc = device_info(&info);
     if (rc == DLM_OK) rc = plan_attend(a, info.sms, &d);
@@ -935,6 +974,10 @@ int dlm_adapters_bf16(const DlmAdapters* a, dlm_stream_t stream) {
     if (!aligned16(a->x) || !aligned16(a->base) || !aligned16(a->out) || !aligned16(a->a) || !aligned16(a->b))
         return DLM_ERR_ALIGN;
     if (a->ldx % 8 || a->ldb % 8 || a->ldo % 8 || a->ldx < 0 || a->ldb < 0 || a->ldo < a->n) return DLM_ERR_ALIGN;
+    const Footprint out(a->out, 1, 0, a->m, a->ldo, 1, 0, a->n);
+    const bool in_place = a->base == a->out && (a->m == 1 || a->ldb == a->ldo);
+    if (out.meets(Footprint(a->x, 1, 0, a->m, a->ldx, 1, 0, a->k)) || (!in_place && out.meets(Footprint(a->base, 1, 0, a->m, a->ldb, 1, 0, a->n))))
+        return DLM_ERR_OVERLAP;
     DeviceInfo info;
     const int rc = device_info(&info);
     if (rc != DLM_OK) return rc;

@@ -1,5 +1,5 @@
 // Warp-level building blocks of the kernels whose rows are too few for a 128-row tensor-memory tile: mma.sync on 16-bit
-// operands with FP32 accumulation, ldmatrix, cp.async with zero fill, FP8 widening; and the launch of one kernel.
+// operands with FP32 accumulation, ldmatrix and movmatrix, FP8 widening; and the launch of one kernel.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -49,15 +49,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     return out;
 }
 
-// 16 bytes to shared memory past L1; zeros (and no read) where `present` is false.
-__device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem, bool present) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(present ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Two E4M3 codes (low byte first) as two halves: exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
     uint32_t h2;
@@ -91,7 +82,6 @@ __device__ __forceinline__ float exp2_approx(float x) {  // relative error about
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-
 
 // Launches `Kernel`; where it takes more dynamic shared memory than any kernel may, its limit is raised once per device, to
 // `smem` (then the same at every call).

@@ -38,7 +38,7 @@ struct alignas(64) AttendDev {
     int rows_cap;      // rows of a tile that exist: min(tile_rows, rows)
     int blocks;        // the kernel for blocks of tokens takes this call
     int items;         // of one sequence: key heads * row tiles
-    int unit_shift;    // log2 of the keys of a unit: kUnitKeys, or more than there are where items are not split
+    int unit_shift;    // log2 of the keys of a unit: kUnitShift, or more than there are where items are not split
     int lead;          // units that an item has in front of those with keys: what its beginning and end cost
     int least_shift;   // log2 of the units of a run of a short line
     int most_waves;

@@ -51,7 +51,7 @@ class Adapters:
 
     def __call__(self, x, ids, base, out=None):
         """out = base + each row's own adapter applied to x. `x` [rows, K], `base` and `out` [rows, N] BF16 with contiguous
-        rows (`out` may be `base`; by default a new tensor), at most 256 rows; `ids` [rows] int32 in any order, negative for
+        rows (`out` may be `base`, but shares no elements with `x`; by default a new tensor), at most 256 rows; `ids` [rows] int32 in any order, negative for
         a row without adapter."""
         key = (x.shape, x.stride(), x.dtype, x.device, ids.shape, ids.stride(), ids.dtype, ids.device, base.shape, base.stride(),
                base.dtype, base.device, None if out is None else (out.shape, out.stride(), out.dtype, out.device))

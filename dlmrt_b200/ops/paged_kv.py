@@ -18,6 +18,7 @@ outside its table touches no memory, and `PagedKV.check()` raises IndexError for
 """
 
 import ctypes as C
+from contextlib import nullcontext
 from struct import Struct
 
 import torch
@@ -125,7 +126,9 @@ class PagedKV:
         page, each at most once in a call; negative: a padded row, which stores nothing. `positions` [n] int32: row of
         `table` (see `rotary_table`, whose width says how many elements of a head are rotated; None: no rotation).
         `interleaved`: pairs are neighbours, not a half apart. `q_norm`, `k_norm` [head dim]: weights of an RMSNorm over each
-        head in front of the rotation. `q_out` may be `q`; by default a new contiguous tensor."""
+        head in front of the rotation. `q_out` may be `q`, but no other
+        tensor that shares elements with `q`, `k` or `v`; by default a new contiguous tensor. `k` and `v` are not part of the
+        cache."""
         key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, slots.shape, slots.stride(),
                slots.dtype, slots.device, eps, interleaved,
                None if table is None else (table.shape, table.stride(), table.dtype, table.device, positions.shape,
@@ -211,7 +214,7 @@ class PagedKV:
         are not read), `lengths` [batch] int32 how many keys it has, the new tokens included. Every token sees all of them
         (a block refined as a whole), with `causal` those up to its own; with `window` only keys less than that many
         positions before it. A token that sees none gets zeros. `scale`: of the scores, head dim ** -0.5 by default. `out`
-        may be `q`. `lse` [batch, tokens, query heads] FP32, if given, takes the logarithm of the softmax's denominator
+        may be `q`, but no other tensor that shares elements with it. `lse` [batch, tokens, query heads] FP32, if given, takes the logarithm of the softmax's denominator
         (-inf for a token that sees no key): what is needed to join the result with attention over other keys."""
         key = (q.shape, q.stride(), q.dtype, q.device, pages.shape, pages.stride(), pages.dtype, pages.device, lengths.shape,
                lengths.stride(), lengths.dtype, lengths.device, scale, window, causal,
@@ -269,7 +272,9 @@ class PagedKV:
             raise ValueError(f"window {window}: expected the number of keys, or 0 for all")
         a.q_strides[:], a.out_strides[:] = (qb, qt, qh), (ob, ot, oh)
         a.table_stride, a.table_pages = pb, pages.shape[1]
-        a.batch, a.tokens, a.q_heads, a.window, a.causal = b, t, hq, window, bool(causal)
+        # A cache has at most 2^30 keys: a longer window is all of them.
+        a.batch, a.tokens, a.q_heads, a.window, a.causal = b, t, hq, min(window, 1 << 30), bool(causal)
         a.scale = d ** -0.5 if scale is None else scale
-        a.workspace_bytes = _lib.lib().dlm_paged_attend_workspace_bytes(a)
+        with torch.cuda.device(self.device) if self.device.type == "cuda" else nullcontext():  # it asks how many SMs there are
+            a.workspace_bytes = _lib.lib().dlm_paged_attend_workspace_bytes(a)
         return a

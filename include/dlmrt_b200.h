@@ -59,7 +59,7 @@ enum {
     DLM_ERR_TIMEOUT = -8,   /* device status: a bounded wait ran out (data from a rank never arrived) */
     DLM_ERR_ARCH = -9,      /* not an sm_100 device */
     DLM_ERR_SCRATCH = -10,  /* dlm_gemm_bf16_noalloc: the requested K splits do not fit the built-in scratch */
-    DLM_ERR_OVERLAP = -11,  /* dlm_rowpar_bf16: the GEMM's input overlaps `rearm` or `out` of the same call */
+    DLM_ERR_OVERLAP = -11,  /* an output overlaps an input of the same call that others may still read (see each entry point) */
     DLM_ERR_INDEX = -12     /* device status: a slot, position, page, length or adapter index lies outside its table */
 };
 
@@ -335,7 +335,8 @@ typedef struct DlmPages {
  *           and i + rotated / 2 (interleaved 0) or 2i and 2i + 1 (interleaved 1), FP32; no rounding in between.
  * Stored in FP8: x / scale[head], at most the largest code in magnitude.
  * A negative slot marks a padded row: nothing is stored for it, its q_out is written. A row whose position or slot lies
- * outside its table is left out altogether. The slots of one call must be distinct. q_out may be q. */
+ * outside its table is left out altogether. The slots of one call must be distinct. q_out may be q (the
+ * same strides); otherwise it shares no bytes with q, k or v (DLM_ERR_OVERLAP). k and v lie outside the cache. */
 typedef struct DlmAppend {
     DlmPages cache;
     const void* q;             /* [n, q_heads, head_dim] `type`, or NULL (then q_out is ignored) */
@@ -364,7 +365,8 @@ DLM_API int dlm_paged_append(const DlmAppend* append, dlm_stream_t stream);
  * (length 0, or causal and in front of the first key) gets zeros, and -inf in lse. A sequence longer than its row of the
  * table is read as far as the table goes. Grouped heads: query head i reads key head i / (q_heads / heads).
  * Keys past the end, pages that are not there and places that the mask hides never reach the result, whatever they hold.
- * Products of `type` with FP32 accumulation, softmax in FP32; FP8 entries are widened exactly. */
+ * Products of `type` with FP32 accumulation, softmax in FP32; FP8 entries are widened exactly to halves. out may be q (the
+ * same strides); otherwise it shares no bytes with q (DLM_ERR_OVERLAP). */
 typedef struct DlmAttend {
     DlmPages cache;
     const void* q;             /* [batch, tokens, q_heads, head_dim] `type` */
@@ -377,7 +379,7 @@ typedef struct DlmAttend {
     int64_t q_strides[3], out_strides[3];  /* sequence, token, head: elements, multiples of 8 */
     int64_t table_stride;
     int32_t batch, tokens, q_heads, type;
-    int32_t table_pages, window, causal;
+    int32_t table_pages, window, causal;   /* window at most 2^30, and so are table_pages * page_size */
     float scale;
     int32_t pdl, reserved;
 } DlmAttend;
@@ -388,7 +390,8 @@ DLM_API int64_t dlm_paged_attend_workspace_bytes(const DlmAttend* attend);
 
 /* ---- low-rank adapters of many requests beside a shared projection ----------------------------------------------
  * out[i] = base[i] + scales[ids[i]] * (x[i] * A[ids[i]]^T) * B[ids[i]]^T; rows with a negative id: out[i] = base[i].
- * No counterpart in the reference. x W^T comes from dlm_gemm_bf16; out may be base. FP32 accumulation, one rounding. */
+ * No counterpart in the reference. x W^T comes from dlm_gemm_bf16; out may be base (the same ldo);
+ * otherwise it shares no bytes with it, and never with x (DLM_ERR_OVERLAP). FP32 accumulation, one rounding. */
 typedef struct DlmAdapters {
     const void* x;             /* [m, k] BF16, rows ldx apart */
     const void* base;          /* [m, n] BF16, rows ldb apart */

@@ -95,6 +95,33 @@ def test_attend_refuses(kw, code):
     assert _lib.lib().dlm_paged_attend(attend(**kw), None) == code
 
 
+@pytest.mark.parametrize("q, q_strides, out, out_strides, batch, tokens, refused", [
+    (0x3000, (256, 256, 64), 0x3000, (256, 256, 64), 2, 1, False),                 # in place
+    (0x3000, (256, 256, 64), 0x3100, (256, 256, 64), 2, 1, True),                  # shifted by two heads
+    (0x3000, (256, 256, 64), 0x3000, (512, 256, 64), 2, 1, True),                  # the same beginning, other rows
+    (0x3000, (512, 256, 64), 0x3200, (512, 256, 64), 4, 1, False),                 # halves of the same longer rows
+    (0x3200, (512, 256, 64), 0x3000, (512, 256, 64), 4, 1, False),
+    (0x3000, (512, 256, 64), 0x3180, (512, 256, 64), 4, 1, True),                  # halves that meet
+    (0x3000, (2048, 512, 64), 0x3200, (2048, 512, 64), 2, 4, False),
+    (0x3000, (2048, 512, 64), 0x3200, (2048, 256, 64), 2, 4, True),                # steps differ: cannot be told
+    (0x3000, (64, 128, 256), 0x3000, (64, 128, 256), 2, 2, False),                 # heads outermost, in place
+])
+def test_attend_results_overlap_no_queries_but_their_own(q, q_strides, out, out_strides, batch, tokens, refused):
+    call = attend(q=q, q_strides=q_strides, out=out, out_strides=out_strides, batch=batch, tokens=tokens, cache=pages(heads=4))
+    code = _lib.lib().dlm_paged_attend(call, None) if refused or not torch.cuda.is_available() else _lib.OK  # never on addresses that are not
+    assert (code == _lib.ERR_OVERLAP) == refused
+
+
+def test_append_results_overlap_no_input_but_their_own():
+    code = lambda **kw: _lib.lib().dlm_paged_append(append(q=0x7000, q_heads=4, **kw), None)
+    rows = dict(n=3, q_strides=(512, 64), out_strides=(512, 64), k_strides=(512, 64), v_strides=(512, 64))
+    assert code(**rows, q_out=0x7040) == _lib.ERR_OVERLAP and code(**rows, q_out=0x6FF0) == _lib.ERR_OVERLAP
+    assert code(**rows, q_out=0x7000, k=0x7100, v=0x7300) == _lib.ERR_OVERLAP  # k inside the row of q that is written
+    if not torch.cuda.is_available():
+        assert code(**rows, q_out=0x7000, k=0x7200, v=0x7300) != _lib.ERR_OVERLAP  # slices of one projection, in place
+        assert code(**rows, q_out=0x9000) != _lib.ERR_OVERLAP
+
+
 def test_attend_workspace_grows_with_what_is_split():
     size = lambda **kw: _lib.lib().dlm_paged_attend_workspace_bytes(attend(**kw))
     assert size(table_pages=1) == 0
@@ -120,6 +147,22 @@ def adapters(**kw):
 ])
 def test_adapters_refuse(kw, code):
     assert _lib.lib().dlm_adapters_bf16(adapters(**kw), None) == code
+
+
+def test_adapters_results_overlap_no_input_but_base():
+    code = lambda **kw: _lib.lib().dlm_adapters_bf16(adapters(**kw), None)
+    assert code(out=0x100000) == _lib.ERR_OVERLAP and code(out=0x200010) == _lib.ERR_OVERLAP
+    assert code(out=0x200000, ldo=128) == _lib.ERR_OVERLAP and code(out=0x200000, ldb=0) == _lib.ERR_OVERLAP
+    if not torch.cuda.is_available():
+        assert code(out=0x200000) != _lib.ERR_OVERLAP and code(x=0x100000, out=0x100080, ldx=128, ldo=128) != _lib.ERR_OVERLAP
+
+
+def test_windows_longer_than_any_cache():
+    assert _lib.lib().dlm_paged_attend(attend(window=(1 << 30) + 1), None) == _lib.ERR_SHAPE
+    keys = torch.zeros(2, 2, 16, 64, dtype=BF16)
+    plan = PagedKV(keys, keys.clone())._plan_attend(torch.zeros(1, 2, 64, dtype=BF16), torch.zeros(1, 2, dtype=torch.int32),
+                                                    torch.zeros(1, dtype=torch.int32), None, None, None, 1 << 33, False)
+    assert plan.window == 1 << 30
 
 
 def test_struct_layouts_match():
