@@ -74,9 +74,10 @@ __global__ void __launch_bounds__(kThreads, adapter_ctas<kTiles>()) adapters_ker
     }
     ids[tid] = id;
     __syncthreads();
-    // Rows of the same adapter in front of this thread's row; the leaders among all rows.
+    // Rows of the same adapter in front of this thread's row; the leaders among all rows. (Warps without rows counting, too: 61
+    // rows 11.6 us instead of 9.3.)
     int before = 0;
-    for (int w = 0; w < warp; ++w) {
+    for (int w = 0; w < warp && warp * 32 < p.m; ++w) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int4 other = sm.ids[w * 8 + i];
