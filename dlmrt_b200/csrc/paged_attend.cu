@@ -116,11 +116,10 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
         tma_prefetch_descriptor(&p.tm_v);
     }
     __syncthreads();
-    const long long deadline = globaltimer() + kDefaultTimeoutNs;
     pdl_wait();
     pdl_launch_dependents();
     if (warp == kConsumers) {
-        produce<kStages, S::kPieces, false>(p, smem, pipes, deadline, leader);
+        produce<kStages, S::kPieces, false>(p, smem, pipes, leader);
         return;
     }
 
@@ -130,6 +129,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
     int stage = 0, slot = 0;
     uint32_t parity = 0, slot_parity = 0;
     while (true) {
+    const long long deadline = item_deadline();
     const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
     if (!announced && leader) stalled(p, 3, slot);
     if (consumers_any(!announced)) return;  // none of the warps may wait for the others any more

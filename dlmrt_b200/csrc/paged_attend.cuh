@@ -171,6 +171,9 @@ __device__ __forceinline__ int cta_of(const uint4* answer) {
 }
 
 
+// Until when a role waits that begins an item now: a call of many items may take longer than a wait that nothing will end.
+__device__ __forceinline__ long long item_deadline() { return globaltimer() + kDefaultTimeoutNs; }
+
 // A wait that runs out is reported; what follows is computed from whatever is there, and nothing more is requested.
 __device__ __forceinline__ void stalled(const AttendDev& p, int who, int at) {
     report(p.a.cache.status, kErrTimeout, who, kPhasePipeline, at);
@@ -179,7 +182,7 @@ __device__ __forceinline__ void stalled(const AttendDev& p, int who, int at) {
 // The producer: a whole warp. A stage of the ring is kPieces * 16 bytes for each of 64 keys, then the same for values. Boxes
 // are a page's slots, at most 64; kApart: of one column block of 128 bytes each, so that a block's 64 rows follow one another.
 template <int kStages, int kPieces, bool kApart>
-__device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes<kStages>& pipes, long long deadline, bool leader) {
+__device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes<kStages>& pipes, bool leader) {
     const int lane = threadIdx.x & 31;
     constexpr int kBytes = kTileKeys * kPieces * 16;
     constexpr int kBlocks = kApart ? (kPieces + 7) / 8 : 1;  // boxes along a row
@@ -189,6 +192,7 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
     int stage = 0, slot = 0, run = blockIdx.x;
     uint32_t parity = 1, slot_parity = 1, answer_parity = 0;  // the first lap of a ring waits for nothing
     bool failed = false;
+    long long deadline = item_deadline();
     auto announce = [&](const Work& work) {
         if (!mbar_wait_warp(&pipes.work_empty[slot], slot_parity, deadline) && !failed) {
             failed = true;
@@ -225,6 +229,7 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
         work.end = first + units == s.units ? hi : min(hi, s.base + (max(0, end) << p.unit_shift));
         work.tiles = end <= 0 ? -1 : work.end > work.start ? (work.end - work.start + kTileKeys - 1) / kTileKeys : 0;
         tile = 0;
+        deadline = item_deadline();
         if (work.tiles > 0) look_up(work.start >> p.page_shift);
     };
     auto begin_run = [&]() -> bool {

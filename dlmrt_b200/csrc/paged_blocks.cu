@@ -227,24 +227,25 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
     const uint32_t tmem_s = tmem + kGroups * D;  // S of step n: + (n % kBuffers) * 64; its weights take the first 32 of these
     auto buffer = [](uint32_t step) { return step % kBuffers; };
     auto phase = [](uint32_t step) { return step / kBuffers & 1; };
-    const long long deadline = globaltimer() + kDefaultTimeoutNs;
     pdl_wait();
     pdl_launch_dependents();
 
     if (warp == Shape::kProducerWarp) {
-        if constexpr (kCodes) produce<kStages, D / 16, true>(p, smem + Shape::kRing, pipes, deadline, leader);
-        else produce<kStages, D / 8, true>(p, smem, pipes, deadline, leader);
+        if constexpr (kCodes) produce<kStages, D / 16, true>(p, smem + Shape::kRing, pipes, leader);
+        else produce<kStages, D / 8, true>(p, smem, pipes, leader);
     } else if (warp == Shape::kIssuerWarp) {
         // -- the issuer: a whole warp on uniform values, one lane issuing ------------------------------------------------
         constexpr uint32_t kIdescS = idesc_f16<M>(kBlockRows, kTileKeys, false), kIdescO = idesc_f16<M>(kBlockRows, D, true);
         const uint64_t q_desc = umma_desc_k128(queries);
         int stage = 0, slot = 0, next_stage = 0;
         uint32_t parity = 0, slot_parity = 0, q_parity = 0, step = 0;
+        long long deadline = 0;
         auto wait = [&](uint64_t* bar, uint32_t bar_phase, int who, int at) {
             if (!mbar_wait_warp(bar, bar_phase, deadline) && leader) stalled(p, who, at);
             tcgen05_fence_after();
         };
         while (true) {
+            deadline = item_deadline();
             const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
             if (!announced) {
                 if (leader) stalled(p, 5, slot);
@@ -303,7 +304,9 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
         const int first_wide = key0 * 128 + (((lane & 3) * 2) ^ (key0 & 7)) * 16;
         int stage = 0, step = 0, slot = 0;
         uint32_t parity = 0, step_parity = 1, slot_parity = 0;
+        long long deadline = 0;
         while (true) {
+            deadline = item_deadline();
             const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
             if (!announced) {
                 if (leader) stalled(p, 16, slot);
@@ -355,12 +358,14 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
         const uint32_t tmem_o = tmem + mine + group * D;
         int stage = 0, slot = 0;
         uint32_t slot_parity = 0, step = 0, aside_parity = 0;
+        long long deadline = 0;
         auto wait = [&](uint64_t* bar, uint32_t bar_phase, int who, int at) {
             if (!mbar_wait(bar, bar_phase, deadline)) stalled(p, who, at);
             __syncwarp();
             tcgen05_fence_after();
         };
         while (true) {
+            deadline = item_deadline();
             const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
             if (!announced && leader) stalled(p, 10, slot);
             if (rows_any<kGroups>(quarter, !announced)) break;  // neither may wait for the other any more

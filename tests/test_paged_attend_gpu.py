@@ -199,6 +199,27 @@ def test_strided_queries_in_place_and_three_dimensions():
     assert torch.equal(kv.attend(q, table[:, :5], lengths), want)  # rows of a wider table
 
 
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("t", [1, 40])
+def test_keys_and_values_in_one_pool(t, cache):
+    """[pages, slot, keys or values, head, head dim], some heads and pages of a larger pool: any strides."""
+    kv, q, table, lengths = setup([150, 70], t, 4, 2, 128, 16, BF16, cache)
+    pages = kv.keys.shape[0]
+    raw = torch.full((2 * pages, 16, 2, 5, 128), 0x7F, device="cuda", dtype=torch.uint8).repeat_interleave(kv.keys.element_size(), -1)
+    both = raw.view(cache)[::2].transpose(1, 3)[:, 1:3]  # [pages, head, keys or values, slot, head dim]
+    for i, pool in enumerate((kv.keys, kv.values)):
+        both[:, :, i].view(torch.uint8).copy_(pool.view(torch.uint8)) if cache == E4M3 else both[:, :, i].copy_(pool)
+    other = PagedKV(both[:, :, 0], both[:, :, 1], kv.k_scale, kv.v_scale)
+    assert torch.equal(other.attend(q, table, lengths), kv.attend(q, table, lengths))
+    k, v = (torch.randn(3, 2, 128, generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i in range(2))
+    slots = torch.tensor([int(table[0, 0]) * 16 + 3, int(table[1, 1]) * 16, -1], device="cuda")
+    for pool in (kv, other):
+        pool.append(k, v, None, slots)
+        pool.check()
+    assert torch.equal(other.attend(q, table, lengths), kv.attend(q, table, lengths))
+    assert bool((raw.view(2 * pages, 16, 2, 5, -1)[1::2] == 0x7F).all()) and bool((raw[:, :, :, [0, 3, 4]] == 0x7F).all())
+
+
 def test_no_pages_and_no_sequences():
     kv, q, table, lengths = setup([4], 1, 4, 2, 64, 16, BF16, BF16)
     none = torch.empty(1, 0, device="cuda", dtype=torch.int32)

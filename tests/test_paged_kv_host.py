@@ -89,6 +89,8 @@ def test_append_refuses(kw, code):
     (dict(tokens=0), _lib.ERR_SHAPE), (dict(batch=-1), _lib.ERR_SHAPE), (dict(batch=65536), _lib.ERR_SHAPE),
     (dict(table_pages=1 << 27), _lib.ERR_SHAPE), (dict(window=-1), _lib.ERR_SHAPE), (dict(causal=2), _lib.ERR_SHAPE),
     (dict(type=_lib.F16), _lib.ERR_SHAPE), (dict(q=0x3004), _lib.ERR_ALIGN), (dict(q_strides=(256, 256, 68)), _lib.ERR_ALIGN),
+    (dict(cache=pages(heads=1024), q_heads=1024, batch=65535, table_pages=1 << 20), _lib.ERR_SHAPE),  # more than 2^31 units of work
+    (dict(tokens=1 << 17), _lib.ERR_SHAPE),
     (dict(out_strides=(256, 256, -64)), _lib.ERR_ALIGN), (dict(q_strides=(-3, 256, 64)), _lib.ERR_ALIGN), (dict(batch=0, q=None), _lib.OK),
 ])
 def test_attend_refuses(kw, code):
