@@ -41,7 +41,7 @@ struct AdapterSmem {
     uint32_t high[kAdapterRows][kTiles * 4 + 4];            // x A^T times the scale, BF16 pairs
     uint32_t low[kAdapterRows][kTiles * 4 + 4];             // what those leave over, BF16 pairs
     int ids[kMostRows];
-    int2 kinds[kWarps][32];  // adapter, rows of it
+    int2 kinds[kWarps][32];  // adapter, rows of it; behind the last one -1
     int kind_count[kWarps];
     int rows[kAdapterRows];
     uint32_t leads[kMostRows / 32];
@@ -76,26 +76,38 @@ __global__ void __launch_bounds__(kThreads, adapter_ctas<kTiles>()) adapters_ker
     }
     ids[tid] = id;
     // Rows of the same adapter in front of this thread's row: in its warp, and, from each warp's list of adapters and how many
-    // rows each has, in the warps in front. (256 comparisons of single rows took 2 us.)
+    // rows each has, in the warps in front; eight entries of every list at once. (256 rows of 8 adapters: comparing single rows
+    // took 2 us, one list after the other 1.1.)
     const uint32_t fellows = __match_any_sync(0xFFFFFFFFu, id), in_front = (1u << lane) - 1;
     int before = __popc(fellows & in_front);
     const uint32_t firsts = __ballot_sync(0xFFFFFFFFu, before == 0 && id >= 0);
+    const int kinds = __popc(firsts);
     if (before == 0 && id >= 0) sm.kinds[warp][__popc(firsts & in_front)] = make_int2(id, __popc(fellows));
-    if (lane == 0) sm.kind_count[warp] = __popc(firsts);
-    __syncthreads();
-    for (int w = 0; w < warp && warp * 32 < p.m; ++w) {
-        const int kinds = sm.kind_count[w];
-#pragma unroll 4
-        for (int i = 0; i < kinds; ++i) {
-            const int2 kind = sm.kinds[w][i];
-            before += kind.x == id ? kind.y : 0;
+    if (lane >= kinds) sm.kinds[warp][lane] = make_int2(-1, 0);
+    if (lane == 0) sm.kind_count[warp] = kinds;
+    const bool some_without = __syncthreads_or(tid < p.m && id < 0);
+    if (warp > 0 && warp * 32 < p.m) {
+        constexpr int kAtOnce = 8;
+        int most = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps - 1; ++w) most = max(most, w < warp ? sm.kind_count[w] : 0);
+        for (int i = 0; i < most; i += kAtOnce) {
+#pragma unroll
+            for (int w = 0; w < kWarps - 1; ++w) {
+                if (w >= warp) break;
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const int2 kind = sm.kinds[w][i + j];
+                    before += kind.x == id ? kind.y : 0;
+                }
+            }
         }
     }
     const bool leads = id >= 0 && before % kAdapterRows == 0;
     const uint32_t leaders = __ballot_sync(0xFFFFFFFFu, leads);
     if (lane == 0) sm.leads[warp] = leaders;
     // Rows without an adapter: out = base, shared out among the clusters.
-    if (base != out) {
+    if (base != out && some_without) {
         for (int row = which; row < p.m; row += clusters) {
             if (ids[row] >= 0) continue;
             for (int c = cta * kThreads + tid; c < p.n / 8; c += kAdapterCtas * kThreads)
