@@ -872,14 +872,11 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim, d->tile_rows);
     // What an item's beginning and end cost in units of 64 keys: 64 ragged sequences of up to 8192 keys 90.3 / 88.8 / 88.8 us with 0 /
     // 2 / 4, FP8 heads of 256 85.4 / 84.6 / 88.2; blocks of 32 tokens 74 / 60.2 / 59.2 / 59.0 / 60.6 with 0 / 5 / 6 / 8 / 11, of 28
-    // rows 37.9 / 37.3 / 38.8 / 40.6 with 5 / 6 / 8 / 11. With more than one wave of runs blocks have more to join than they gain:
-    // 59.0 / 65.2 / 72.3 us with one, two, three.
-    d->most_waves = d->blocks ? 1 : 5;
+    // rows 37.9 / 37.3 / 38.8 / 40.6 with 5 / 6 / 8 / 11.
     d->lead = whole ? 0 : d->blocks ? kBlocksLead : kAttendLead;
     const long long units = whole ? 1 : d->lead + (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
     if (units * a->batch * d->items > INT32_MAX) return DLM_ERR_SHAPE;
-    const Cut cut = attend_cut(static_cast<uint32_t>(units * a->batch * d->items), d->resident, d->least_shift, d->most_waves);
-    d->grid = cut.across * cut.waves;
+    d->grid = attend_runs(static_cast<uint32_t>(units * a->batch * d->items), d->resident, d->least_shift);
     d->by_item = static_cast<long long>(a->batch) * d->items < d->grid;
     return DLM_OK;
 }

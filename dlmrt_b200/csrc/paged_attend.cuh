@@ -1,12 +1,12 @@
 // What both attention kernels over the paged cache share (paged_attend.cu, paged_blocks.cu): how the work is dealt out, the
 // producer that requests keys and values, and how a row is finished.
 //
-// An item is one sequence, key head and row tile. The keys of all items are lined up in units of 64 keys and cut into runs,
-// whatever the lengths of the sequences. The first runs go to as many CTAs as the GPU holds; a CTA that is done takes over
-// the run of a CTA that was not launched yet (cluster launch control). Runs get shorter towards the line's end, because SMs do
-// not read equally fast: with one run for each CTA the slowest came in 30 % behind the others. Requests go on across items and
-// runs. An item that lies in several runs leaves a partial result in each, which join_kernel adds up in their order: the
-// result does not depend on which CTA took which run.
+// An item is one sequence, key head and row tile. The keys of all items are lined up in units of 64 keys and cut evenly into
+// runs, one for each CTA that the GPU holds, whatever the lengths of the sequences. Requests go on across the items of a run. An
+// item that lies in several runs leaves a partial result in each, which join_kernel adds up in their order. (SMs do not read
+// equally fast, up to 30 % apart. Further, shorter runs, taken over by CTAs that get done early, cost more partial results and
+// begun items than they gain: 64 ragged sequences 88.7 us with five waves of runs, 88.0 with two, 87.4 with one; 131071 keys 53.1 /
+// 49.8 / 48.7; 64 sequences of 16 rows 45.1 / 38.8 / 35.4; FP8 heads of 256 84.8 / 80.0 / 80.2.)
 //
 // An item's beginning and end take time, too: its units begin with `lead` units without keys that stand for it. A run that
 // holds only such units of an item leaves it to the next one.
@@ -49,11 +49,10 @@ __device__ __forceinline__ int seen_to(const AttendDev& p, int first_pos, int le
 // The token that a row (query head of the group, token) belongs to.
 __device__ __forceinline__ int token_of(const AttendDev& p, int row) { return p.a.tokens == 1 ? 0 : row / p.group; }
 
-// The line of units and its runs (see attend_cut). Every warp that needs it works it out for itself: a lane looks at a range
+// The line of units and its runs. Every warp that needs it works it out for itself: a lane looks at a range
 // of the sequences. The host has seen to it that there are fewer than 2^31 units.
 struct Line {
     uint32_t total;
-    Cut cut;
     int runs;
     int first, last;    // this lane's sequences
     uint32_t before;    // units in front of them
@@ -74,23 +73,16 @@ struct Line {
         }
         total = __shfl_sync(0xFFFFFFFFu, before, 31);
         before -= mine;
-        cut = attend_cut(total, p.resident, p.least_shift, p.most_waves);
-        runs = cut.across * cut.waves;
+        runs = attend_runs(total, p.resident, p.least_shift);
     }
-    __device__ __forceinline__ uint32_t wave_begin(int wave) const { return wave < cut.waves ? total - (total >> wave) : total; }
-    // The units [begin, end) of a run: a wave's are dealt out evenly, rounded down, and no run is empty.
+    // The units [begin, end) of a run: dealt out evenly, rounded down, and no run is empty.
     __device__ __forceinline__ void range(int run, uint32_t* begin, uint32_t* end) const {
-        const uint32_t across = cut.across, wave = static_cast<uint32_t>(run) / across, i = run - wave * across;
-        const uint32_t from = wave_begin(wave), units = wave_begin(wave + 1) - from, each = units / across, over = units - each * across;
-        *begin = from + each * i + over * i / across;
-        *end = from + each * (i + 1) + over * (i + 1) / across;
+        const uint32_t across = runs, i = run, each = total / across, over = total - each * across;
+        *begin = each * i + over * i / across;
+        *end = each * (i + 1) + over * (i + 1) / across;
     }
     __device__ __forceinline__ int run_of(uint32_t unit) const {
-        int wave = 0;
-        while (wave + 1 < cut.waves && unit >= wave_begin(wave + 1)) ++wave;
-        const uint32_t from = wave_begin(wave);
-        return wave * cut.across +
-               static_cast<int>((static_cast<unsigned long long>(unit - from + 1) * cut.across - 1) / (wave_begin(wave + 1) - from));
+        return static_cast<int>((static_cast<unsigned long long>(unit + 1) * runs - 1) / total);
     }
     // The units in front of a sequence. All lanes of the warp.
     __device__ __forceinline__ uint32_t in_front_of(const AttendDev& p, int sequence) const {
@@ -130,46 +122,17 @@ struct Work {
 // The rings between the producer and the warps that compute: stages of keys and values, and announced items.
 template <int kStages>
 struct alignas(16) Pipes {
-    uint4 answer;
     uint64_t full[kStages], empty[kStages], present[kStages];  // present: bit j says that the stage's key j is there
-    uint64_t work_full[kWorkSlots], work_empty[kWorkSlots], answered;
+    uint64_t work_full[kWorkSlots], work_empty[kWorkSlots];
     Work works[kWorkSlots];
 
     // One thread; `readers` arrive for every stage that they are done with, `listeners` for every item.
     __device__ __forceinline__ void init(int readers, int listeners) {
         for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], readers);
         for (int i = 0; i < kWorkSlots; ++i) mbar_init(&work_full[i], 1), mbar_init(&work_empty[i], listeners);
-        mbar_init(&answered, 1);
         fence_barrier_init();
     }
 };
-
-// Asks for the block index of a CTA that was not launched yet, which then never will be: 16 bytes that arrive on `bar`.
-__device__ __forceinline__ void ask_for_cta(uint4* answer, uint64_t* bar) {
-    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
-                 "r"(smem_u32(bar))
-                 : "memory");
-}
-// The block index of an answer, or -1 where every CTA has been launched.
-__device__ __forceinline__ int cta_of(const uint4* answer) {
-    uint32_t x, got;
-    asm volatile(
-        "{\n"
-        ".reg .b128 a;\n"
-        ".reg .pred p;\n"
-        ".reg .b32 y, z, w;\n"
-        "ld.shared.b128 a, [%2];\n"
-        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
-        "selp.u32 %1, 1, 0, p;\n"
-        "mov.u32 %0, 0;\n"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, a;\n"
-        "}\n"
-        : "=&r"(x), "=&r"(got)
-        : "r"(smem_u32(answer))
-        : "memory");
-    return got ? static_cast<int>(x) : -1;
-}
-
 
 // Until when a role waits that begins an item now: a call of many items may take longer than a wait that nothing will end.
 __device__ __forceinline__ long long item_deadline() { return globaltimer() + kDefaultTimeoutNs; }
@@ -189,8 +152,9 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
     const Line line(p, blockIdx.x == 0);
     const int box_keys = min(kTileKeys, 1 << p.page_shift), boxes = kTileKeys / box_keys;
     const int slot_mask = (1 << p.page_shift) - 1;
-    int stage = 0, slot = 0, run = blockIdx.x;
-    uint32_t parity = 1, slot_parity = 1, answer_parity = 0;  // the first lap of a ring waits for nothing
+    const int run = blockIdx.x;
+    int stage = 0, slot = 0;
+    uint32_t parity = 1, slot_parity = 1;  // the first lap of a ring waits for nothing
     bool failed = false;
     long long deadline = item_deadline();
     auto announce = [&](const Work& work) {
@@ -204,8 +168,8 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
         }
         if (++slot == kWorkSlots) slot = 0, slot_parity ^= 1;
     };
-    // Where the next step is: a run, an item in it, a step of 64 keys in that. Pages are looked up a step ahead of their
-    // use, across items and runs, 32 entries of the table at once: lane j holds entry `window` + j.
+    // Where the next step is: an item in the run, a step of 64 keys in that. Pages are looked up a step ahead of their use,
+    // across items, 32 entries of the table at once: lane j holds entry `window` + j.
     uint32_t unit = 0, last_unit = 0;
     int sequence = 0, index = 0, first = 0, units = 0, lo = 0, tile = 0, window = 0, pages = 0;
     Sequence s{};
@@ -233,12 +197,7 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
         if (work.tiles > 0) look_up(work.start >> p.page_shift);
     };
     auto begin_run = [&]() -> bool {
-        if (run < 0 || run >= line.runs) return false;
-        if (leader) {
-            fence_proxy_async();  // the last answer has been read
-            mbar_expect_tx(&pipes.answered, sizeof(pipes.answer));
-            ask_for_cta(&pipes.answer, &pipes.answered);
-        }
+        if (run >= line.runs) return false;
         line.range(run, &unit, &last_unit);
         uint32_t in_front;
         sequence = line.sequence_at(p, unit, &in_front);
@@ -261,14 +220,7 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
             begin_item();
             return true;
         }
-        if (!mbar_wait_warp(&pipes.answered, answer_parity, deadline)) {
-            if (leader) stalled(p, 2, run);
-            return false;
-        }
-        answer_parity ^= 1;
-        run = cta_of(&pipes.answer);
-        __syncwarp();
-        return begin_run();
+        return false;
     };
     bool more = begin_run();
     while (more) {

@@ -403,7 +403,6 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
             const float value_scale = kCodes ? p.a.cache.v_scale[item.head] : 1.f;
             float m = -INFINITY, l = 0.f;
             uint32_t own_steps = 0;  // of this group in this item
-            const uint32_t first_step = step;
             for (int tile = 0; tile < item.tiles; ++tile, ++step) {
                 if (step % kGroups != static_cast<uint32_t>(group)) {
                     if (++stage == kSteps) stage = 0;
@@ -542,10 +541,7 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
                 const uint32_t last_own = step - 1 - ((step - 1) % kGroups == static_cast<uint32_t>(group) ? 0 : 1);
                 wait(&pv_done[buffer(last_own)], phase(last_own), 15, item.tiles);
             }
-            // The groups' results together: every group takes its share of the elements, from each group's O. The group that had
-            // the item's first step comes first: which one that was depends on what this CTA did before, and a sum of products
-            // that is rounded once at its end is another one in the other order.
-            auto nth = [&](int i) { return static_cast<int>((first_step + i) % kGroups); };
+            // The groups' results together: every group takes its share of the elements, from each group's O.
             group_stats[group][r] = make_float2(m, l);
             rows_sync<kGroups>(quarter);
             float factors[kGroups];
@@ -554,7 +550,7 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
             for (int i = 0; i < kGroups; ++i) m = fmaxf(m, group_stats[i][r].x);
 #pragma unroll
             for (int i = 0; i < kGroups; ++i) {
-                const float2 stats = group_stats[nth(i)][r];
+                const float2 stats = group_stats[i][r];
                 factors[i] = stats.x == -INFINITY ? 0.f : exp2_approx(stats.x - m);
                 l += stats.y * factors[i];
             }
@@ -579,7 +575,7 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i) {
                     uint32_t o[32];
-                    tmem_load_32(tmem + mine + nth(i) * D + c * 32, o);
+                    tmem_load_32(tmem + mine + i * D + c * 32, o);
                     tmem_load_wait();
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = (i == 0 ? 0.f : v[j]) + __uint_as_float(o[j]) * factors[i];

@@ -41,25 +41,17 @@ struct alignas(64) AttendDev {
     int unit_shift;    // log2 of the keys of a unit: kUnitShift, or more than there are where items are not split
     int lead;          // units that an item has in front of those with keys: what its beginning and end cost
     int least_shift;   // log2 of the units of a run of a short line
-    int most_waves;
     int resident;      // CTAs that the GPU holds
-    int grid;          // runs that there are at most
+    int grid;          // CTAs, and runs that there are at most
     int by_item;       // the join has a block for each item, not for each run
     int sms;
 };
 
-// How a line of `total` units is cut into runs: `waves` waves of `across` runs each. The first wave takes half of the line, the
-// second a quarter and so on, the last what is left: CTAs take runs in order as they get done, and what they take last is
-// short. No wave is shorter than two units a run; a line of less than that has runs of about 2^least_shift units.
-struct Cut {
-    int across, waves;
-};
-__host__ __device__ inline Cut attend_cut(uint32_t total, int resident, int least_shift, int most_waves) {
-    Cut c{resident, 1};
-    while (c.waves < most_waves && (total >> c.waves) >= 2u * static_cast<uint32_t>(resident)) ++c.waves;
+// How many runs a line of `total` units is cut into: one for each CTA that the GPU holds, a short line into runs of about
+// 2^least_shift units.
+__host__ __device__ inline int attend_runs(uint32_t total, int resident, int least_shift) {
     const uint32_t most = (total + (1u << least_shift) - 1) >> least_shift;
-    if (c.waves == 1 && most < static_cast<uint32_t>(resident)) c.across = most < 1 ? 1 : static_cast<int>(most);
-    return c;
+    return most < 1 ? 1 : most < static_cast<uint32_t>(resident) ? static_cast<int>(most) : resident;
 }
 
 int launch_append(const DlmAppend& p, int page_shift, const LaunchOpts& o);

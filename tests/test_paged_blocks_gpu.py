@@ -141,8 +141,8 @@ def test_the_same_bits_and_graphs():
 
 
 @pytest.mark.parametrize("t, hq, hk, d", [(1, 8, 2, 128), (64, 8, 2, 128), (64, 8, 2, 64), (48, 8, 2, 256)])
-def test_the_same_bits_whichever_cta_takes_a_run(t, hq, hk, d):
-    """Two calls at once share the SMs, so that runs go to whoever is free, after another number of steps each time."""
+def test_the_same_bits_beside_another_call(t, hq, hk, d):
+    """Two calls at once share the SMs: what a CTA computes does not depend on when or where it runs."""
     kv, q, table, lengths = setup([900, 300, 2000], t, hq, hk, d, 16, BF16, BF16)
     queries = (q, q.flip(0).contiguous())
     want = [kv.attend(x, table, lengths) for x in queries]
