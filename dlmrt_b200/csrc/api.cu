@@ -837,11 +837,13 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
 
 // Everything about an attention call that its device pointers do not decide.
 static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
-    // Blocks of tokens have a kernel of their own from more rows on than the other one has in a tile. It reads the cache once for
-    // 128 rows, and takes longer to begin and to end: 64 sequences of up to 6001 keys, 28 rows, heads of 64 / 128 / 256: 33 / 38
-    // / 85 us against 45 / 65 / 141; nine sequences: 14.6 / 20 / 27 against 13.4 / 16 / 32. With 16 rows, one tile: 33 / 37 / 84
-    // against 31 / 45 / 100, and 14.4 / 18 / 26 against 12.5 / 14.4 / 23.
-    constexpr int kWholeKeys = 256, kBlocksAbove = kRowTile, kBlocksLead = 6, kAttendLead = 2;
+    // Blocks of tokens have a kernel of their own, from more rows on than one or two tiles of the other one hold. It reads the
+    // cache once for 128 rows, and takes longer to begin and to end. 64 sequences of up to 6001 keys, 28 rows (two tiles), heads of
+    // 64 / 128 / 256: 31.8 / 36.2 / 81.8 us against 29.2 / 42.8 / 101.8; nine sequences: 14.2 / 19.1 / 27.0 against 13.5 / 15.0 /
+    // 23.8; 16 rows (one tile) 32.9 / 36.9 / 84.2 against 22.2 / 31.6 / 63.9. Codes it has to widen first: 32 sequences of up to 8224
+    // keys, 32 rows: 23.3 / 36.9 / 84.0 against 21.8 / 30.2 / 65.9; 48 rows: 23.2 / 37.5 / 84.3 against 26.4 / 39.7 / 88.3. Heads of 64
+    // with 40 rows: 81.2 against 96.7.
+    constexpr int kWholeKeys = 256, kBlocksAbove = kRowTile, kBlocksAboveTwo = 2 * kRowTile, kBlocksLead = 6, kAttendLead = 3, kDearLead = 6;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
@@ -852,7 +854,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     if (a->cache.type != DLM_E4M3 && a->cache.type != a->type) return DLM_ERR_SHAPE;
     d->group = a->q_heads / a->cache.heads;
     d->rows = a->tokens * d->group;
-    d->blocks = d->rows > kBlocksAbove;
+    d->blocks = d->rows > (a->cache.type == DLM_E4M3 || a->cache.head_dim == 64 ? kBlocksAboveTwo : kBlocksAbove);
     d->tile_rows = d->blocks ? kBlockRows : d->rows <= kFewRows ? kFewRows : kRowTile;
     d->row_tiles = (d->rows + d->tile_rows - 1) / d->tile_rows;
     d->rows_cap = d->rows < d->tile_rows ? d->rows : d->tile_rows;
@@ -862,21 +864,20 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kTileKeys < span)
         span = static_cast<long long>(a->window) + a->tokens + kTileKeys;
     // Short sequences: an item is one run, whose result needs no join. One CTA takes 0.8 us for a step of 64 keys in pages of 16;
-    // runs of two steps and their join 2 us in all. Tables of 256 keys, 1 / 8 / 64 sequences, 8 heads of 128: whole 8.2 / 8.5 / 15.6
-    // us, split 8.9 / 10.7 / 21.1; of 512 keys: whole 11.3 / 11.5 / 23.2, split 9.0 / 11.2 / 24.8; of 1024: 17.6 / 17.6 / 37.9
-    // against 9.1 / 11.6 / 34.4.
-    const bool whole = span <= (static_cast<long long>(a->batch) * d->items >= sms ? 2 * kWholeKeys : kWholeKeys);
+    // runs of a step or two and their join 2 us in all. Tables of 256 keys, 1 / 8 / 64 sequences, 8 heads of 128: whole 7.9 / 8.2 /
+    // 15.6 us, split 8.7 / 10.5 / 17.7; of 512 keys: whole 11.0 / 11.1 / 23.0, split 8.3 / 10.7 / 22.8.
+    const bool whole = span <= kWholeKeys;
     d->unit_shift = whole ? 31 : kUnitShift;
-    d->least_shift = whole ? 0 : 1;
     d->sms = sms;
     d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim, d->tile_rows);
-    // What an item's beginning and end cost in units of 64 keys: 64 ragged sequences of up to 8192 keys 90.3 / 88.8 / 88.8 us with 0 /
-    // 2 / 4, FP8 heads of 256 85.4 / 84.6 / 88.2; blocks of 32 tokens 74 / 60.2 / 59.2 / 59.0 / 60.6 with 0 / 5 / 6 / 8 / 11, of 28
-    // rows 37.9 / 37.3 / 38.8 / 40.6 with 5 / 6 / 8 / 11.
-    d->lead = whole ? 0 : d->blocks ? kBlocksLead : kAttendLead;
+    // What an item's beginning and end cost in units of 64 keys; more where a step is short (codes) or a tile's end long (16 rows).
+    // 64 ragged sequences of up to 8192 keys 88.0 / 87.7 / 87.1 / 88.8 us with 1 / 2 / 3 / 4; FP8 heads of 256 81.7 / 81.4 / 78.2 / 79.0
+    // with 2 / 4 / 6 / 8, 64 sequences of 16 rows 35.0 / 32.3 / 31.6 / 31.6; blocks of 32 tokens 74 / 60.2 / 59.2 / 59.0 / 60.6 with 0 /
+    // 5 / 6 / 8 / 11, of 28 rows 37.9 / 37.3 / 38.8 / 40.6 with 5 / 6 / 8 / 11.
+    d->lead = whole ? 0 : d->blocks ? kBlocksLead : a->cache.type == DLM_E4M3 || d->tile_rows > kFewRows ? kDearLead : kAttendLead;
     const long long units = whole ? 1 : d->lead + (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
     if (units * a->batch * d->items > INT32_MAX) return DLM_ERR_SHAPE;
-    d->grid = attend_runs(static_cast<uint32_t>(units * a->batch * d->items), d->resident, d->least_shift);
+    d->grid = attend_runs(static_cast<uint32_t>(units * a->batch * d->items), d->resident);
     d->by_item = static_cast<long long>(a->batch) * d->items < d->grid;
     return DLM_OK;
 }

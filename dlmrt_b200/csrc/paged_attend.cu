@@ -578,10 +578,9 @@ static int launch_attend_t(const AttendDev& p, const LaunchOpts& o) {
     void* args[] = {const_cast<AttendDev*>(&p)};
     const int rc = launch_kernel<attend_kernel<T, D, kCodes, kRows>>(dim3(p.grid), dim3(kAttendThreads), AttendSmem<D, kCodes, kRows>::kBytes, args, o);
     if (rc != 0 || p.partial == nullptr) return rc;
-    // With far fewer items than runs an item may have hundreds of partial results: large blocks, one for a quarter of each row
-    // (293 partial results of a row: 7 us in blocks of a whole row, all of it latency; up to 64 runs an item small blocks are
-    // faster: 18 items in 592 runs, rows of 16: 14.4 us in all against 19.7). Otherwise it has two or three, and most blocks
-    // only find out that there is nothing to join (0.5 us; 9000 blocks took 25).
+    // With far fewer items than runs an item has many partial results: large blocks, one for a quarter of each row (four items in
+    // 296 runs, 131071 keys: 48.6 us in all, 49.5 with small blocks; 18 items in 444 runs: 18.2 against 12.1). Otherwise it has
+    // two or three, and most blocks only find out that there is nothing to join (0.5 us; 9000 blocks took 25).
     const long long items = static_cast<long long>(p.a.batch) * p.items;
     const LaunchOpts dependent{o.stream, true, false};  // always a dependent launch of the kernel above
     auto join = [&](unsigned blocks, int rows, int splits, int threads) {

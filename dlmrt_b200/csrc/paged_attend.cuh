@@ -73,7 +73,7 @@ struct Line {
         }
         total = __shfl_sync(0xFFFFFFFFu, before, 31);
         before -= mine;
-        runs = attend_runs(total, p.resident, p.least_shift);
+        runs = attend_runs(total, p.resident);
     }
     // The units [begin, end) of a run: dealt out evenly, rounded down, and no run is empty.
     __device__ __forceinline__ void range(int run, uint32_t* begin, uint32_t* end) const {

@@ -40,18 +40,15 @@ struct alignas(64) AttendDev {
     int items;         // of one sequence: key heads * row tiles
     int unit_shift;    // log2 of the keys of a unit: kUnitShift, or more than there are where items are not split
     int lead;          // units that an item has in front of those with keys: what its beginning and end cost
-    int least_shift;   // log2 of the units of a run of a short line
     int resident;      // CTAs that the GPU holds
     int grid;          // CTAs, and runs that there are at most
     int by_item;       // the join has a block for each item, not for each run
     int sms;
 };
 
-// How many runs a line of `total` units is cut into: one for each CTA that the GPU holds, a short line into runs of about
-// 2^least_shift units.
-__host__ __device__ inline int attend_runs(uint32_t total, int resident, int least_shift) {
-    const uint32_t most = (total + (1u << least_shift) - 1) >> least_shift;
-    return most < 1 ? 1 : most < static_cast<uint32_t>(resident) ? static_cast<int>(most) : resident;
+// How many runs a line of `total` units is cut into: one for each CTA that the GPU holds, or for each unit of a short line.
+__host__ __device__ inline int attend_runs(uint32_t total, int resident) {
+    return total < static_cast<uint32_t>(resident) ? static_cast<int>(total) : resident;
 }
 
 int launch_append(const DlmAppend& p, int page_shift, const LaunchOpts& o);

@@ -14,16 +14,16 @@ BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("t, hq, hk", [(33, 1, 1), (32, 8, 2), (43, 3, 1)])
+@pytest.mark.parametrize("t, hq, hk", [(17, 1, 1), (33, 1, 1), (32, 8, 2), (43, 3, 1)])
 def test_one_tile_of_rows(t, hq, hk, d, dtype):
-    """Rows just above 32, exactly 128, and one row more; lengths around the step of 64 keys, whole and split."""
+    """Rows just above 16 and 32, exactly 128, and one row more; lengths around the step of 64 keys, whole and split."""
     check(*setup([t, 64, 65, 128, 300], t, hq, hk, d, 16, dtype, dtype))
     check(*setup([0, t, 640, 1029], t, hq, hk, d, 32, dtype, dtype))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("t, hq, hk", [(17, 1, 1), (32, 8, 2), (43, 3, 1)])
+@pytest.mark.parametrize("t, hq, hk", [(32, 1, 1), (33, 1, 1), (32, 8, 2), (43, 3, 1)])
 def test_one_tile_of_rows_over_codes(t, hq, hk, d, dtype):
     check(*setup([t, 64, 65, 128, 300], t, hq, hk, d, 16, dtype, E4M3))
     check(*setup([0, t, 640, 1029], t, hq, hk, d, 32, dtype, E4M3))
