@@ -843,7 +843,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     // 23.8; 16 rows (one tile) 32.9 / 36.9 / 84.2 against 22.2 / 31.6 / 63.9. Codes it has to widen first: 32 sequences of up to 8224
     // keys, 32 rows: 23.3 / 36.9 / 84.0 against 21.8 / 30.2 / 65.9; 48 rows: 23.2 / 37.5 / 84.3 against 26.4 / 39.7 / 88.3. Heads of 64
     // with 40 rows: 81.2 against 96.7.
-    constexpr int kWholeKeys = 256, kBlocksAbove = kRowTile, kBlocksAboveTwo = 2 * kRowTile, kBlocksLead = 6, kAttendLead = 3, kDearLead = 6;
+    constexpr int kWholeKeys = 384, kBlocksAbove = kRowTile, kBlocksAboveTwo = 2 * kRowTile, kBlocksLead = 6, kAttendLead = 3, kDearLead = 6;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
     if (a->batch < 1 || a->batch > 65535 || a->tokens < 1 || a->tokens > 1 << 16 || a->table_pages < 0) return DLM_ERR_SHAPE;
@@ -864,8 +864,9 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     if (a->window > 0 && static_cast<long long>(a->window) + a->tokens + kTileKeys < span)
         span = static_cast<long long>(a->window) + a->tokens + kTileKeys;
     // Short sequences: an item is one run, whose result needs no join. One CTA takes 0.8 us for a step of 64 keys in pages of 16;
-    // runs of a step or two and their join 2 us in all. Tables of 256 keys, 1 / 8 / 64 sequences, 8 heads of 128: whole 7.9 / 8.2 /
-    // 15.6 us, split 8.7 / 10.5 / 17.7; of 512 keys: whole 11.0 / 11.1 / 23.0, split 8.3 / 10.7 / 22.8.
+    // runs of a step or two and their join 2 us in all (and 4 us more of the caller's time). Tables of 384 keys, 1 / 8 / 64
+    // sequences, 8 heads of 128: whole 8.3 / 8.9 / 19.6 us, split 7.0 / 10.6 / 20.8; of 512 keys: whole 11.0 / 11.1 / 23.0, split 8.2 /
+    // 10.7 / 22.8.
     const bool whole = span <= kWholeKeys;
     d->unit_shift = whole ? 31 : kUnitShift;
     d->sms = sms;
