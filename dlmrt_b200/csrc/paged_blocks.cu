@@ -18,6 +18,9 @@
 // One CTA an SM; shared memory holds 2 to 8 steps of 64 keys. A step is 2 * 128 * 64 * head_dim multiply-adds (512 cycles of the
 // tensor pipe at 128) and 8192 exponentials (512 cycles). A group takes 1300 cycles for a step, most of it latency, which is as
 // long as a step's 32 KB take from HBM: with one group nothing is left to catch up with what an item's beginning and end cost.
+// 16 sequences of 1056 to 8224 keys, blocks of 32 tokens, 8 key heads of 128 with four query heads each: 59 us, 4.1 TB/s (HBM at 91 %
+// while steps run; start 4.5 us, 3.5 between items, join 3); the same over an FP8 cache 83 us, the converters' two warps being what
+// takes longest.
 #include "paged_attend.cuh"
 
 namespace dlm {
