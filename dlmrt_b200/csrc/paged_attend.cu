@@ -29,7 +29,6 @@ namespace {
 constexpr int kConsumers = 4;                            // warps that compute
 constexpr int kAttendThreads = (kConsumers + 1) * 32;
 constexpr int kWarpKeys = kTileKeys / kConsumers;        // 16
-constexpr float kRescaleAbove = 8.f;
 
 // A stage: 64 keys, then 64 values, as TMA writes them: box by box (a page's slots, at most 64), in a box column blocks of up
 // to 128 bytes, in each the rows one after the other with their 16-byte pieces permuted by row (the 128- or 64-byte swizzle),
@@ -304,7 +303,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float top = fmaxf(s[n][e], s[n][2 + e]);
-                rescale |= top > m[n][e] + kRescaleAbove || (m[n][e] == -INFINITY && top > m[n][e]);
+                rescale |= top > m[n][e] + (kRescaleAbove + kHeadroom<M>) || (m[n][e] == -INFINITY && top > m[n][e]);
             }
         }
         if (__any_sync(0xFFFFFFFFu, rescale)) {
@@ -315,7 +314,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
                     float top = fmaxf(s[n][e], s[n][2 + e]);
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-                    const float now = fmaxf(m[n][e], top), f = m[n][e] == now ? 1.f : exp2_approx(m[n][e] - now);
+                    const float now = fmaxf(m[n][e], top - kHeadroom<M>), f = m[n][e] == now ? 1.f : exp2_approx(m[n][e] - now);
                     m[n][e] = now, l[n][e] *= f;
 #pragma unroll
                     for (int i = 0; i < kOut; ++i) o[i][n][e] *= f, o[i][n][2 + e] *= f;

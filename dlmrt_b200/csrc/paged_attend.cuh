@@ -22,6 +22,14 @@ namespace dlm {
 constexpr int kWorkSlots = 4;  // items that may be announced ahead
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Weights are exp2(s - m) for a reference m that follows the running maximum: it is set to the maximum less kHeadroom, and anew
+// when a score is more than kRescaleAbove past that. Weights then lie below 2^15. Halves end at 2^-24: with the largest weight at
+// 2^7 the many small ones of a long cache keep 7 bits more (with m the maximum itself, keys 2^26 times lighter than the heaviest
+// counted for nothing, and half of what 8000 of them add was lost). BF16 has the range of FP32.
+constexpr float kRescaleAbove = 8.f;
+template <typename M>
+constexpr float kHeadroom = std::is_same<M, __half>::value ? 7.f : 0.f;
+
 // A sequence's keys: how many, the position of its first new token, where its units begin, and how many an item of it has.
 struct Sequence {
     int length, first_pos, base, units;

@@ -28,7 +28,6 @@ namespace dlm {
 namespace {
 
 constexpr int kGroupThreads = 128;
-constexpr float kRescaleAbove = 8.f;
 
 template <int D, bool kCodes>
 struct BlockShape {
@@ -435,8 +434,8 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
 #pragma unroll
                 for (int j = 4; j < 64; ++j) top4[j & 3] = fmaxf(top4[j & 3], s[j]);
                 const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-                if (__any_sync(0xFFFFFFFFu, top > m + kRescaleAbove || (m == -INFINITY && top > m))) {
-                    const float n = fmaxf(m, top);
+                if (__any_sync(0xFFFFFFFFu, top > m + (kRescaleAbove + kHeadroom<M>) || (m == -INFINITY && top > m))) {
+                    const float n = fmaxf(m, top - kHeadroom<M>);
                     const float f = m == n ? 1.f : exp2_approx(m - n);  // 0 where nothing was there
                     l *= f, m = n;
                     if (own_steps > 0) {

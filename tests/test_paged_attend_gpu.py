@@ -277,6 +277,28 @@ def test_the_join_of_two_halves_is_the_whole():
     su.assert_within((parts[0][0] * w[0] + parts[1][0] * w[1]), want, 2 * bound)
 
 
+@pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("cache", [F16, E4M3, BF16])
+def test_many_keys_of_small_weight(cache, t):
+    """One key outweighs each of the others by e^18, about 2^26. Weights are taken as halves (BF16 without FP8 or FP16), at
+    least 2^7 for the heaviest key: half a step of the smallest is 2^-25, that of a light weight 2^7 e^-18 within 1 / 64 of it."""
+    n, d, b = 8000, 64, 40
+    kv, q, table, lengths = setup([n], t, 8, 8, d, 64, BF16 if cache == BF16 else F16, cache)
+    q, table, lengths = q.repeat(b, 1, 1, 1), table.repeat(b, 1), lengths.repeat(b)  # more heads than CTAs: each meets all keys
+    kv.keys.zero_(), kv.values.fill_(8), q.zero_()
+    if cache == E4M3:
+        kv.k_scale.fill_(1), kv.v_scale.fill_(1)
+    q[..., 0] = 1
+    first = table[0, 0]
+    kv.keys[first, :, 0, 0] = 18
+    kv.values[first, :, 0] = 0
+    light = (n - 1) * math.exp(-18)
+    want = 8 * light / (1 + light)
+    got = kv.attend(q, table, lengths, scale=1.0).double()
+    assert float((got / want - 1).abs().max()) <= 1 / 64 + 2 * su.HALF[q.dtype]
+    kv.check()
+
+
 def test_offsets_past_32_bits():
     """A pool of more than 2^31 elements, read at its end."""
     pages, page, hk, d = 33000, 128, 4, 128
