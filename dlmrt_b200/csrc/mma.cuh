@@ -77,6 +77,13 @@ __device__ __forceinline__ uint32_t narrow2(float x, float y) {
     return out;
 }
 
+// Two halves rounded towards zero.
+__device__ __forceinline__ uint32_t narrow2_to_zero(float x, float y) {
+    uint32_t out;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(out) : "f"(y), "f"(x));
+    return out;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {  // relative error about 2^-22, exp2(-inf) = 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

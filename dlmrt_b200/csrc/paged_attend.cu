@@ -3,8 +3,9 @@
 //
 //   o = sum_j exp(s_j) v_j / sum_j exp(s_j),   s_j = scale * q . k_j over the keys that the row's token sees
 //
-// One pass over the keys with a running maximum m and sum l per row (all exponents in base 2, scale * log2(e) folded into the
-// scores). What is there is rescaled by exp2(m - m') once a new maximum m' is more than 8 above m: weights up to 2^8 fit.
+// One pass over the keys with a running reference m and sum l per row (all exponents in base 2, scale * log2(e) folded into the
+// scores). What is there is rescaled by exp2(m - m') when a score is more than kRescaleAbove + kHeadroom above m; m' is then the
+// new maximum less kHeadroom (see paged_attend.cuh). Weights enter the second product in a high and a low part.
 //
 // The rows that share a key head are its query heads times the new tokens. 8 or 16 of them are the N of an mma.sync, 16 keys
 // (then 16 elements of the output) its M: S^T = K Q^T, O^T = V^T P^T. A single token fills a few rows and is bound by reading
@@ -392,11 +393,14 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
             }
         }
         {
-            uint32_t b[kN][2];  // the weights, rows from key g to row g
+            uint32_t b[kN][2], low[kN][2];  // the weights, high and low parts, rows from key g to row g
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
-                b[n][0] = transpose_8x8(narrow2<M>(s[n][0], s[n][1]));
-                b[n][1] = transpose_8x8(narrow2<M>(s[n][2], s[n][3]));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    split_weights<M, kCodes>(s[n][2 * h], s[n][2 * h + 1], &b[n][h], &low[n][h]);
+                    b[n][h] = transpose_8x8(b[n][h]), low[n][h] = transpose_8x8(low[n][h]);
+                }
             }
             if constexpr (!kCodes) {
                 const int key = (lane & 7) + ((lane >> 4) << 3);
@@ -404,6 +408,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
                 for (int i = 0; i < kOut; ++i) {
                     uint32_t a[4];
                     ldmatrix_x4_trans(a, stage_v32 + rows_of_stage.at(key, 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) mma_16816<M>(o[i][n], a, low[n][0], low[n][1]);
 #pragma unroll
                     for (int n = 0; n < kN; ++n) mma_16816<M>(o[i][n], a, b[n][0], b[n][1]);
                 }
@@ -419,6 +425,8 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
                         const uint32_t a[4] = {
                             e4m3x2_to_f16x2(__byte_perm(w[2 * c], 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(w[2 * c], 0, 0x4431)),
                             e4m3x2_to_f16x2(__byte_perm(w[2 * c + 1], 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(w[2 * c + 1], 0, 0x4431))};
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) mma_16816<M>(o[i + c][n], a, low[n][0], low[n][1]);
 #pragma unroll
                         for (int n = 0; n < kN; ++n) mma_16816<M>(o[i + c][n], a, b[n][0], b[n][1]);
                     }

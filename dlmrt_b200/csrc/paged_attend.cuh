@@ -23,12 +23,42 @@ constexpr int kWorkSlots = 4;  // items that may be announced ahead
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Weights are exp2(s - m) for a reference m that follows the running maximum: it is set to the maximum less kHeadroom, and anew
-// when a score is more than kRescaleAbove past that. Weights then lie below 2^15. Halves end at 2^-24: with the largest weight at
-// 2^7 the many small ones of a long cache keep 7 bits more (with m the maximum itself, keys 2^26 times lighter than the heaviest
-// counted for nothing, and half of what 8000 of them add was lost). BF16 has the range of FP32.
+// when a score is more than kRescaleAbove past that. Weights then lie below 2^8, those that are taken as halves below 2^15. Halves
+// end at 2^-24: with the largest weight at 2^7 the many small ones of a long cache keep 7 bits more (with m the maximum itself, keys
+// 2^26 times lighter than the heaviest counted for nothing, and half of what 8000 of them add was lost). BF16 has the range of FP32.
 constexpr float kRescaleAbove = 8.f;
 template <typename M>
 constexpr float kHeadroom = std::is_same<M, __half>::value ? 7.f : 0.f;
+static_assert(kRescaleAbove + kHeadroom<__half> <= 15.f, "weights fit halves");
+
+// Two weights as the product with the values takes them, which knows 16-bit types only: each as a high and a low part, whose
+// products are added in FP32. One value alone is off by up to 2^-8 of the weight (BF16; halves 2^-11), which is more than the rounding
+// of a result in which values partly cancel; both parts together are off by 2^-15 (halves: 2^-20, and 2^-25 of 1).
+//
+// Values of a 16-bit cache may be infinite. Neither part may then make a NaN of infinity, by its sign or by being zero: the high
+// part is rounded towards zero, and less than the weight by 2^-12 of it and a step of halves at least; for BF16 2^-20 of the
+// weight is added to the low part instead. FP8 has no infinity.
+//
+// What the second product costs: nothing where HBM bounds a call (64 ragged sequences 87.5 us with one part and with two, 131071
+// keys 48.2 / 48.4, FP8 heads of 256 77.8 / 78.6), most where 16 rows share FP8 keys (heads of 256 78.5 / 86.0, of 128 33.6 / 35.9).
+template <typename M, bool kCodes>
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t* high, uint32_t* low) {
+    if constexpr (!std::is_same<M, __half>::value) {
+        constexpr float kMore = 1.f + 0x1p-20f;
+        const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+        *high = __byte_perm(a, b, 0x7632);
+        *low = narrow2<M>(fmaf(x, kMore, -__uint_as_float(a & 0xFFFF0000u)), fmaf(y, kMore, -__uint_as_float(b & 0xFFFF0000u)));
+    } else {
+        if constexpr (kCodes) {
+            *high = narrow2<M>(x, y);
+        } else {
+            constexpr float kLess = 1.f - 0x1p-12f, kStep = -0x1p-24f;
+            *high = narrow2_to_zero(fmaxf(x * 0.5f, fmaf(x, kLess, kStep)), fmaxf(y * 0.5f, fmaf(y, kLess, kStep)));
+        }
+        const float2 h = widen2<M>(*high);
+        *low = narrow2<M>(x - h.x, y - h.y);
+    }
+}
 
 // A sequence's keys: how many, the position of its first new token, where its units begin, and how many an item of it has.
 struct Sequence {
