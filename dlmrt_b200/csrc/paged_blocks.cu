@@ -8,19 +8,19 @@
 //   producer   a warp, see paged_attend.cuh.
 //   converters (FP8 cache) warps that widen a step's codes to halves, exactly, and lay them out as TMA lays out 16-bit keys and
 //              values. Queries are halves, too, each row scaled by a power of two.
-//   issuer     a warp that issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory,
-//              V as it lies, its 64 keys down the rows). Each group has two buffers of S: its next step's scores are computed
-//              under this one's softmax.
+//   issuer     a warp that issues S = Q K^T (M = 128 rows, N = 64 keys) and O += P V (M = 128, N = head_dim; P from tensor memory in
+//              a high and a low part, V as it lies, its 64 keys down the rows). Each group has two buffers of S: its next step's
+//              scores are computed under this one's softmax.
 //
-// m is the running maximum when O was last rescaled: O, which lives in tensor memory, is multiplied by exp2(m - m') only when
-// some row's maximum has grown by more than 8 (a factor of 256, which the weights and their FP32 sum have room for).
+// m is the reference that weights are relative to when O was last rescaled (see paged_attend.cuh): O, which lives in tensor memory, is
+// multiplied by exp2(m - m') only when some row's maximum is more than kRescaleAbove + kHeadroom past m.
 //
-// One CTA an SM; shared memory holds 2 to 8 steps of 64 keys. A step is 2 * 128 * 64 * head_dim multiply-adds (512 cycles of the
-// tensor pipe at 128) and 8192 exponentials (512 cycles). A group takes 1300 cycles for a step, most of it latency, which is as
-// long as a step's 32 KB take from HBM: with one group nothing is left to catch up with what an item's beginning and end cost.
-// 16 sequences of 1056 to 8224 keys, blocks of 32 tokens, 8 key heads of 128 with four query heads each: 59 us, 4.1 TB/s (HBM at 91 %
-// while steps run; start 4.5 us, 3.5 between items, join 3); the same over an FP8 cache 83 us, the converters' two warps being what
-// takes longest.
+// One CTA an SM; shared memory holds 2 to 8 steps of 64 keys. A step is 3 * 128 * 64 * head_dim multiply-adds (768 cycles of the
+// tensor pipe at 128) and 8192 exponentials (512 cycles). A group takes longer for a step than the step's 32 KB take from HBM, most
+// of it latency (1300 cycles against 1400 before weights had a low part): with one group nothing is left to catch up with what an
+// item's beginning and end cost. 16 sequences of 1056 to 8224 keys, blocks of 32 tokens, 8 key heads of 128 with four query heads
+// each: 64 us, 3.8 TB/s (start 4.5 us, 3.5 between items, join 3); the same over an FP8 cache 84 us, the converters' two warps being
+// what takes longest.
 #include "paged_attend.cuh"
 
 namespace dlm {
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem = uniform(tmem_base);
-    const uint32_t tmem_s = tmem + kGroups * D;  // S of step n: + (n % kBuffers) * 64; its weights take the first 32 of these
+    const uint32_t tmem_s = tmem + kGroups * D;  // S of step n: + (n % kBuffers) * 64; its weights take the place, high parts, then low ones
     auto buffer = [](uint32_t step) { return step % kBuffers; };
     auto phase = [](uint32_t step) { return step / kBuffers & 1; };
     pdl_wait();
@@ -286,9 +286,11 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
                 const uint32_t values = smem_u32(smem) + stage * 2 * kBytes + kBytes;
                 if (leader) {
 #pragma unroll
-                    for (int k = 0; k < kTileKeys / 16; ++k)
-                        umma_f16_ts(tmem + step % kGroups * D, tmem_s + buffer(step) * 64 + k * 8, umma_desc_mn128(values + k * 2048, kBlockBytes),
-                                    kIdescO);
+                    for (int k = 0; k < kTileKeys / 16; ++k) {
+                        const uint64_t v_desc = umma_desc_mn128(values + k * 2048, kBlockBytes);
+                        umma_f16_ts(tmem + step % kGroups * D, tmem_s + buffer(step) * 64 + k * 8, v_desc, kIdescO);
+                        umma_f16_ts(tmem + step % kGroups * D, tmem_s + buffer(step) * 64 + 32 + k * 8, v_desc, kIdescO);
+                    }
                     umma_commit(&step_empty[stage]);
                     umma_commit(&pv_done[buffer(step)]);
                 }
@@ -453,15 +455,16 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
                 }
                 const float sub = m == -INFINITY ? 0.f : m;
                 float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t weights[32];
+                uint32_t high[32], low[32];
 #pragma unroll
                 for (int j = 0; j < 64; j += 2) {
                     s[j] = exp2_approx(s[j] - sub), s[j + 1] = exp2_approx(s[j + 1] - sub);
                     sum4[j & 3] += s[j], sum4[(j + 1) & 3] += s[j + 1];
-                    weights[j / 2] = narrow2<M>(s[j], s[j + 1]);
+                    split_weights<M, kCodes>(s[j], s[j + 1], &high[j / 2], &low[j / 2]);
                 }
                 l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-                tmem_store_32(s_at, weights);
+                tmem_store_32(s_at, high);
+                tmem_store_32(s_at + 32, low);
                 if (edge) {
                     // Values that are not finite, in keys that some rows see and others do not, or that are not there: 0 * inf
                     // would reach the result. Where there are any, every warp finds their keys for itself.

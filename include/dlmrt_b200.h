@@ -365,9 +365,9 @@ DLM_API int dlm_paged_append(const DlmAppend* append, dlm_stream_t stream);
  * (length 0, or causal and in front of the first key) gets zeros, and -inf in lse. A sequence longer than its row of the
  * table is read as far as the table goes. Grouped heads: query head i reads key head i / (q_heads / heads).
  * Keys past the end, pages that are not there and places that the mask hides never reach the result, whatever they hold.
- * Products of `type` with FP32 accumulation, softmax in FP32; FP8 entries are widened exactly to halves. The weights of up to 16
- * rows (query heads of a key head times tokens; 32 for heads of 64 and FP8) enter the product with the values as two 16-bit parts:
- * 15 bits of each (halves 20). out may be q (the same strides); otherwise it shares no bytes with q (DLM_ERR_OVERLAP). */
+ * Products of `type` with FP32 accumulation, softmax in FP32; FP8 entries are widened exactly to halves. Weights enter the product
+ * with the values as two 16-bit parts each, 15 bits of a weight (halves 20). out may be q (the same strides); otherwise it shares
+ * no bytes with q (DLM_ERR_OVERLAP). */
 typedef struct DlmAttend {
     DlmPages cache;
     const void* q;             /* [batch, tokens, q_heads, head_dim] `type` */

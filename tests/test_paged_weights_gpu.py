@@ -73,3 +73,13 @@ def test_few_rows(t, hq, d, dtype, cache):
     cache = E4M3 if cache == "e4m3" else dtype
     check(setup([0, 5, 63, 300], t, hq, 2, d, 16, dtype, cache), causal=t > 1)
     check(setup([700, 2, 1500, 64], t, hq, 2, d, 32, dtype, cache), window=900)
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_blocks_of_tokens(d, dtype, cache):
+    """The kernel for more rows than two tiles hold, whole and split."""
+    cache = E4M3 if cache == "e4m3" else dtype
+    check(setup([40, 63, 300], 40, 4, 2, d, 16, dtype, cache), causal=True)
+    check(setup([700, 41, 1500], 33, 2, 1, d, 32, dtype, cache), window=900)
