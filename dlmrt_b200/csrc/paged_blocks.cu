@@ -499,6 +499,7 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
 #pragma unroll
                         for (int j = 0; j < 64; ++j) weightless |= static_cast<uint64_t>(s[j] == 0.f) << j;
                         if (own_steps > 0) wait(&pv_done[buffer(last_own)], phase(last_own), 13, tile);
+                        tmem_store_wait();  // O may just have been rescaled
 #pragma unroll 1
                         for (uint64_t left = bad; left != 0; left &= left - 1) {
                             const int key = __ffsll(static_cast<long long>(left)) - 1;
