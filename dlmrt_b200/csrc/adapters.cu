@@ -50,6 +50,14 @@ struct AdapterSmem {
     int lead, lead_before;
 };
 
+// A value as the sum of two BF16 ones. The high part is the nearest, or the largest below a finite value that would become
+// infinite; of an infinity both parts are infinite (inf - inf would be NaN).
+__device__ __forceinline__ float high_part(float v) {
+    const float nearest = __bfloat162float(__float2bfloat16_rn(v));
+    return isinf(nearest) && !isinf(v) ? __uint_as_float(__float_as_uint(v) & 0xFFFF0000u) : nearest;
+}
+__device__ __forceinline__ float low_part(float v, float high) { return isinf(v) ? v : v - high; }
+
 }  // namespace
 
 template <int kTiles>
@@ -207,10 +215,9 @@ __global__ void __launch_bounds__(kThreads, adapter_ctas<kTiles>()) adapters_ker
 #pragma unroll
             for (int from = 0; from < kAdapterCtas; ++from) v.x += s[from].x, v.y += s[from].y;
             v.x *= scale, v.y *= scale;
-            const uint32_t high = narrow2<__nv_bfloat16>(v.x, v.y);
-            const float2 h = widen2<__nv_bfloat16>(high);
-            sm.high[r][c / 2] = high;
-            sm.low[r][c / 2] = narrow2<__nv_bfloat16>(v.x - h.x, v.y - h.y);
+            const float2 h = make_float2(high_part(v.x), high_part(v.y));
+            sm.high[r][c / 2] = narrow2<__nv_bfloat16>(h.x, h.y);
+            sm.low[r][c / 2] = narrow2<__nv_bfloat16>(low_part(v.x, h.x), low_part(v.y, h.y));
         }
     }
     auto read_all = cluster.barrier_arrive();  // no CTA leaves while another still reads its sums

@@ -392,7 +392,8 @@ DLM_API int64_t dlm_paged_attend_workspace_bytes(const DlmAttend* attend);
 /* ---- low-rank adapters of many requests beside a shared projection ----------------------------------------------
  * out[i] = base[i] + scales[ids[i]] * (x[i] * A[ids[i]]^T) * B[ids[i]]^T; rows with a negative id: out[i] = base[i].
  * No counterpart in the reference. x W^T comes from dlm_gemm_bf16; out may be base (the same ldo);
- * otherwise it shares no bytes with it, and never with x (DLM_ERR_OVERLAP). FP32 accumulation, one rounding. */
+ * otherwise it shares no bytes with it, and never with x (DLM_ERR_OVERLAP). FP32 accumulation, one rounding; the low-rank
+ * vector times the scale enters the second product as two BF16 values each (16 bits), so B has to be finite. */
 typedef struct DlmAdapters {
     const void* x;             /* [m, k] BF16, rows ldx apart */
     const void* base;          /* [m, n] BF16, rows ldb apart */
