@@ -10,6 +10,8 @@
 // HBM for prompts: each lane has up to four heads' loads on the way at once, before the token's position and slot are known,
 // and registers are held to five blocks an SM (8189 tokens of 32 head rows of 256: 98 us with one row a lane, 65 with four at
 // three blocks an SM, 54 at five).
+#include <climits>
+
 #include "../../include/dlmrt_b200.h"
 #include "mma.cuh"
 #include "serving.cuh"
@@ -70,9 +72,12 @@ __global__ void __launch_bounds__(kAppendMostThreads, kCodes ? 4 : 5) append_ker
         const bool bad_slot = slot >= static_cast<long long>(p.cache.pages) << page_shift;
         const bool bad_pos = p.rotated && (pos < 0 || pos >= p.table_rows);
         if (bad_slot || bad_pos) {  // nothing of this token is written
-            if (threadIdx.x == 0)
-                report_index(p.cache.status, static_cast<int>(token), bad_slot ? kIndexSlot : kIndexPosition,
-                             bad_slot ? static_cast<int>(slot >> page_shift) : pos);
+            if (threadIdx.x == 0 && bad_slot)
+                report_index(p.cache.status, static_cast<int>(token), kIndexSlot,
+                             static_cast<int>(min(slot >> page_shift, static_cast<long long>(INT_MAX))),
+                             static_cast<int>(slot & ((1ll << page_shift) - 1)));
+            else if (threadIdx.x == 0)
+                report_index(p.cache.status, static_cast<int>(token), kIndexPosition, pos);
             return;
         }
         // This lane's cosines and sines; partner: the lane that holds the other halves of its pairs.

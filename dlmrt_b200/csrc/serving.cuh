@@ -7,15 +7,16 @@
 
 namespace dlm {
 
-// Which index was out of range: the `slot` of the status words (their `block` is the row or sequence, `epoch` the value).
+// Which index was out of range: the `slot` of the status words (their `block` is the row or sequence, `epoch` the value; of a slot
+// of the cache `epoch` is its page and `phase` the place in it).
 enum IndexKind { kIndexSlot = 1, kIndexPosition = 2, kIndexPage = 3, kIndexLength = 4, kIndexAdapter = 5 };
 
 // First error wins, as report(). The words describe a row instead of a block.
-__device__ __forceinline__ void report_index(int* status, int row, int kind, int value) {
+__device__ __forceinline__ void report_index(int* status, int row, int kind, int value, int place = 0) {
     if (status == nullptr) return;
     if (atomicCAS(status, 0, DLM_ERR_INDEX) == 0) {
         status[1] = (row << 8) | kind;
-        status[2] = 0;
+        status[2] = place;
         status[3] = value;
     }
 }

@@ -29,6 +29,7 @@ from .._lib import DlmAppend, DlmAttend, DlmPages, DlmStatus
 # The pointers that every call brings, which lie side by side in the descriptors.
 _APPEND, _APPEND_AT = Struct("9Q"), DlmAppend.q.offset
 _ATTEND, _ATTEND_AT = Struct("7Q"), DlmAttend.q.offset
+_MOST_INT = (1 << 31) - 1  # what a larger page is reported as
 _MOST_PLANS = 4096  # of one cache: sizes of calls that are remembered
 
 _INDEX = {1: "slot", 2: "position", 3: "page", 4: "length", 5: "adapter"}
@@ -47,12 +48,15 @@ def rotary_table(rotated, positions, theta=10000.0, device="cuda", inverse_frequ
     return torch.cat((angle.cos(), angle.sin()), 1).float()
 
 
-def _index_error(status, where):
+def _index_error(status, where, page_size=0):
     """Reads `status` (and clears it); IndexError where a kernel met an index outside its table."""
     read = DlmStatus()
     _lib.check(_lib.lib().dlm_status_read(status.data_ptr(), C.byref(read), _lib.stream(status)), where)
     if read.code == _lib.ERR_INDEX:
-        raise IndexError(f"{where}: row {read.block}: {_INDEX.get(read.slot, 'index')} {read.epoch} lies outside its table")
+        kind, value = _INDEX.get(read.slot, "index"), str(read.epoch)
+        if kind == "slot":  # as a page and the place in it, which is how a slot is made up
+            value = f"{'at least ' if read.epoch == _MOST_INT else ''}{read.epoch} * {page_size} + {read.phase}"
+        raise IndexError(f"{where}: row {read.block}: {kind} {value} lies outside its table")
     _lib.check(read.code, where)
 
 
@@ -84,7 +88,7 @@ class PagedKV:
                                       or scale.device != keys.device):
                 raise ValueError(f"scales must be contiguous FP32 [{heads}] tensors on {keys.device}")
         self.keys, self.values, self.k_scale, self.v_scale = keys, values, k_scale, v_scale
-        self.device, self.dtype, self.heads, self.head_dim = keys.device, keys.dtype, heads, head_dim
+        self.device, self.dtype, self.heads, self.page_size, self.head_dim = keys.device, keys.dtype, heads, page_size, head_dim
         self.status = torch.zeros(_lib.STATUS_WORDS, device=keys.device, dtype=torch.int32)
         p = DlmPages()
         p.keys, p.values, p.status = keys.data_ptr(), values.data_ptr(), self.status.data_ptr()
@@ -105,7 +109,7 @@ class PagedKV:
     def check(self):
         """Raises IndexError for the first slot, position, page or length outside its table since the last check
         (synchronises the current stream)."""
-        _index_error(self.status, "PagedKV")
+        _index_error(self.status, "PagedKV", self.page_size)
 
     def _given(self, name, t, dtype, shape):
         if t.dtype != dtype or t.shape != shape or t.device != self.device:

@@ -204,7 +204,7 @@ typedef struct DlmMoeFront {
 
 /* Device status read back by dlm_status_read(). */
 typedef struct DlmStatus {
-    int32_t code;   /* DLM_OK or DLM_ERR_TIMEOUT */
+    int32_t code;   /* DLM_OK, DLM_ERR_TIMEOUT or DLM_ERR_INDEX */
     int32_t block;  /* CTA that gave up */
     int32_t slot;   /* rank slot it was waiting for */
     int32_t phase;  /* 1 = receive slots (reduce-scatter), 2 = own OUT copy (all-gather), 3 = GEMM pipeline */
@@ -308,7 +308,8 @@ DLM_API int dlm_all_gather_loopback(const void* const* x, int64_t bytes, const D
  * split over the keys and a combine pass (dlmrt/models/sdar/engine.py:127-132, dlmrt/ops/triton/attention.py).
  *
  * Indices that live on the device are checked there: an entry outside its table touches no memory, is treated as if it
- * were not there, and leaves DLM_ERR_INDEX in the status words (block = which row or sequence, slot = which index). */
+ * were not there, and leaves DLM_ERR_INDEX in the status words (block = which row or sequence, slot = which index, epoch = its
+ * value; of a slot epoch = its page, at most INT32_MAX, and phase = the place in the page). */
 enum { DLM_BF16 = 0, DLM_F16 = 1, DLM_E4M3 = 2 };
 
 #define DLM_MIN_PAGE 8
