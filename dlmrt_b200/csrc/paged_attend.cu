@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kAttendThreads, AttendSmem<D, kCodes, kRows>::
 #pragma unroll
             for (int x = 1; x < 4; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
             // 2^-e and 2^e for the exponent e of the largest element, kept where both are normal numbers.
-            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 126);
+            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
             const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {

@@ -173,7 +173,7 @@ __device__ __forceinline__ float to_halves(uint4* v) {
     }
 #pragma unroll
     for (int x = 1; x < kLanes; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 126);
+    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import serving_util as su
-from test_paged_attend_gpu import setup
+from test_paged_attend_gpu import check as check_against_64_bits, setup
 
 pytestmark = pytest.mark.gpu
 BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
@@ -83,3 +83,12 @@ def test_blocks_of_tokens(d, dtype, cache):
     cache = E4M3 if cache == "e4m3" else dtype
     check(setup([40, 63, 300], 40, 4, 2, d, 16, dtype, cache), causal=True)
     check(setup([700, 41, 1500], 33, 2, 1, d, 32, dtype, cache), window=900)
+
+
+@pytest.mark.parametrize("size", [1e-35, 1e-36, 1e-37, 3e36])
+@pytest.mark.parametrize("t, hq", [(1, 4), (40, 4)])
+def test_queries_at_both_ends_of_bf16_over_codes(t, hq, size):
+    """Rows whose largest element is near 2^-126 or 2^126 are brought into the range of halves as any others."""
+    kv, q, table, lengths = setup([90, 333], t, hq, 2, 64, 16, BF16, E4M3)
+    q[:, 0, 1] = 0
+    check_against_64_bits(kv, (q * size).to(BF16), table, lengths, scale=0.1 / size)
