@@ -759,26 +759,63 @@ static bool strides_ok(const int64_t* strides, const int* extents, int n, int of
     return true;
 }
 
-// The bytes of a tensor [outer, n, heads, head_dim] of 2-byte elements (strides of the first three; inner contiguous): rows of
-// `width` bytes, `step` apart. step 0: one row, or rows that no single step leads through.
+// The bytes of a tensor of 2-byte elements: up to three strided dimensions, outermost first, in front of a contiguous one.
 struct Footprint {
-    uintptr_t begin, end;
-    uint64_t step, width;
-    Footprint(const void* at, int64_t outer, int64_t outer_stride, int64_t n, int64_t stride, int64_t heads, int64_t head_stride, int64_t dim) {
-        width = static_cast<uint64_t>((heads - 1) * head_stride + dim) * 2;
-        begin = reinterpret_cast<uintptr_t>(at);
-        end = begin + static_cast<uint64_t>((outer - 1) * outer_stride + (n - 1) * stride) * 2 + width;
-        step = static_cast<uint64_t>(n > 1 ? stride : outer > 1 ? outer_stride : 0) * 2;
-        if (n > 1 && outer > 1 && stride > 0 && outer_stride % stride) step = 0;
-    }
-    // Whether two tensors share bytes, as far as can be told: rows side by side in the same longer rows do not.
-    bool meets(const Footprint& o) const {
-        if (end <= o.begin || o.end <= begin) return false;
-        if (step == 0 || step != o.step) return true;
-        const uint64_t ahead = o.begin >= begin ? (o.begin - begin) % step : (step - (begin - o.begin) % step) % step;
-        return ahead < width || step - ahead < o.width;
+    uintptr_t at;
+    int64_t extent[3], stride[3], width;  // strides and width in bytes; a dimension along which nothing moves has extent 1
+
+    Footprint(const void* base, const int* extents, const int64_t* strides, int dims, int64_t inner)
+        : at(reinterpret_cast<uintptr_t>(base)), extent{1, 1, 1}, stride{0, 0, 0}, width(inner * 2) {
+        for (int i = 0; i < dims; ++i)
+            if (extents[i] > 1 && strides[i] > 0) extent[i] = extents[i], stride[i] = strides[i] * 2;
     }
 };
+
+// A dimension that two tensors step along by the same stride: the difference of their indices lies in [from, to].
+struct Steps {
+    int64_t stride, from, to;
+};
+
+// Whether offset + sum_i index_i * stride_i falls between lo and hi (both excluded) for some indices. Dimensions by falling stride,
+// so that few indices of each are worth looking at; true where that are too many (`budget`).
+static bool steps_reach(const Steps* dims, int n, int64_t offset, int64_t lo, int64_t hi, int* budget) {
+    int64_t least = offset, most = offset;
+    for (int i = 0; i < n; ++i) least += dims[i].from * dims[i].stride, most += dims[i].to * dims[i].stride;
+    if (most <= lo || least >= hi) return false;
+    if (n == 0) return true;
+    if (--*budget < 0) return true;
+    // what the other dimensions add, and the indices that leave them a chance
+    const int64_t s = dims->stride, rest_least = least - dims->from * s, rest_most = most - dims->to * s;
+    auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    int64_t from = floor_div(lo - rest_most, s) + 1, to = -floor_div(rest_least - hi, s) - 1;
+    if (from < dims->from) from = dims->from;
+    if (to > dims->to) to = dims->to;
+    for (int64_t i = from; i <= to; ++i)
+        if (steps_reach(dims + 1, n - 1, offset + i * s, lo, hi, budget)) return true;
+    return false;
+}
+
+// Whether two tensors share bytes: exact where they step alike (slices of one projection, their heads side by side or in turn),
+// otherwise whether their ranges meet.
+static bool meet(const Footprint& a, const Footprint& b) {
+    Steps dims[3];
+    int n = 0;
+    bool alike = true;
+    int64_t a_span = a.width, b_span = b.width;
+    for (int i = 0; i < 3; ++i) {
+        a_span += (a.extent[i] - 1) * a.stride[i], b_span += (b.extent[i] - 1) * b.stride[i];
+        if (a.extent[i] == 1 && b.extent[i] == 1) continue;
+        alike = alike && (a.extent[i] == 1 || b.extent[i] == 1 || a.stride[i] == b.stride[i]);
+        const Steps d{a.extent[i] > 1 ? a.stride[i] : b.stride[i], 1 - b.extent[i], a.extent[i] - 1};
+        int at = n++;
+        for (; at > 0 && dims[at - 1].stride < d.stride; --at) dims[at] = dims[at - 1];
+        dims[at] = d;
+    }
+    const int64_t ahead = static_cast<int64_t>(a.at - b.at);
+    if (ahead >= b_span || -ahead >= a_span) return false;
+    int budget = 4096;
+    return !alike || steps_reach(dims, n, ahead, -a.width, b.width, &budget);
+}
 
 // log2 of the page size in *shift.
 static int check_pages(const DlmPages* c, int* shift) {
@@ -821,12 +858,11 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
         return DLM_ERR_ALIGN;
     if (a->q != nullptr) {
         const int dim = a->cache.head_dim;
-        const Footprint out(a->q_out, 1, 0, a->n, a->out_strides[0], a->q_heads, a->out_strides[1], dim);
+        const Footprint out(a->q_out, q_extents, a->out_strides, 2, dim);
         const bool in_place = a->q == a->q_out && (a->n == 1 || a->q_strides[0] == a->out_strides[0]) &&
                               (a->q_heads == 1 || a->q_strides[1] == a->out_strides[1]);
-        if (!in_place && out.meets(Footprint(a->q, 1, 0, a->n, a->q_strides[0], a->q_heads, a->q_strides[1], dim))) return DLM_ERR_OVERLAP;
-        if (out.meets(Footprint(a->k, 1, 0, a->n, a->k_strides[0], a->cache.heads, a->k_strides[1], dim)) ||
-            out.meets(Footprint(a->v, 1, 0, a->n, a->v_strides[0], a->cache.heads, a->v_strides[1], dim)))
+        if (!in_place && meet(out, Footprint(a->q, q_extents, a->q_strides, 2, dim))) return DLM_ERR_OVERLAP;
+        if (meet(out, Footprint(a->k, kv_extents, a->k_strides, 2, dim)) || meet(out, Footprint(a->v, kv_extents, a->v_strides, 2, dim)))
             return DLM_ERR_OVERLAP;
     }
     DeviceInfo info;
@@ -940,8 +976,7 @@ int dlm_paged_attend(const DlmAttend* a, dlm_stream_t stream) {
         const int64_t *q = a->q_strides, *out = a->out_strides;
         bool in_place = a->q == a->out;
         for (int i = 0; i < 3; ++i) in_place = in_place && (extents[i] == 1 || q[i] == out[i]);
-        if (!in_place && Footprint(a->q, a->batch, q[0], a->tokens, q[1], a->q_heads, q[2], a->cache.head_dim)
-                             .meets(Footprint(a->out, a->batch, out[0], a->tokens, out[1], a->q_heads, out[2], a->cache.head_dim)))
+        if (!in_place && meet(Footprint(a->q, extents, q, 3, a->cache.head_dim), Footprint(a->out, extents, out, 3, a->cache.head_dim)))
             return DLM_ERR_OVERLAP;
     }
     DeviceInfo info;
@@ -973,9 +1008,9 @@ int dlm_adapters_bf16(const DlmAdapters* a, dlm_stream_t stream) {
     if (!aligned16(a->x) || !aligned16(a->base) || !aligned16(a->out) || !aligned16(a->a) || !aligned16(a->b))
         return DLM_ERR_ALIGN;
     if (a->ldx % 8 || a->ldb % 8 || a->ldo % 8 || a->ldx < 0 || a->ldb < 0 || a->ldo < a->n) return DLM_ERR_ALIGN;
-    const Footprint out(a->out, 1, 0, a->m, a->ldo, 1, 0, a->n);
+    const Footprint out(a->out, &a->m, &a->ldo, 1, a->n);
     const bool in_place = a->base == a->out && (a->m == 1 || a->ldb == a->ldo);
-    if (out.meets(Footprint(a->x, 1, 0, a->m, a->ldx, 1, 0, a->k)) || (!in_place && out.meets(Footprint(a->base, 1, 0, a->m, a->ldb, 1, 0, a->n))))
+    if (meet(out, Footprint(a->x, &a->m, &a->ldx, 1, a->k)) || (!in_place && meet(out, Footprint(a->base, &a->m, &a->ldb, 1, a->n))))
         return DLM_ERR_OVERLAP;
     DeviceInfo info;
     const int rc = device_info(&info);

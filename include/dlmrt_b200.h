@@ -312,6 +312,8 @@ DLM_API int dlm_all_gather_loopback(const void* const* x, int64_t bytes, const D
  * value; of a slot epoch = its page, at most INT32_MAX, and phase = the place in the page). */
 enum { DLM_BF16 = 0, DLM_F16 = 1, DLM_E4M3 = 2 };
 
+/* Results that may lie beside inputs in one buffer (DLM_ERR_OVERLAP): tensors that step by the same strides are told apart
+ * element by element, others count as sharing bytes where their ranges meet. */
 #define DLM_MIN_PAGE 8
 #define DLM_MAX_PAGE 4096
 
