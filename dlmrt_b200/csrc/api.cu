@@ -1075,16 +1075,16 @@ int dlm_abi_check_moe(size_t sizeof_moe) { return sizeof_moe == sizeof(DlmMoe) ?
 const char* dlm_strerror(int code) {
     switch (code) {
         case DLM_OK: return "ok";
-        case DLM_ERR_SHAPE: return "unsupported shape (hidden size a multiple of 256, at most 8192; m a multiple of 16, at most 256; k a multiple of 64)";
+        case DLM_ERR_SHAPE: return "a size that this entry point does not take (include/dlmrt_b200.h; of projections and reductions: hidden size a multiple of 256, at most 8192; m a multiple of 16, at most 256; k a multiple of 64)";
         case DLM_ERR_ALIGN: return "address or leading dimension not 16-byte aligned";
         case DLM_ERR_WORLD: return "rows must split over ranks; at most 8 ranks; rank within the world";
         case DLM_ERR_NULL: return "required pointer is null";
         case DLM_ERR_GRID: return "grid cannot be co-resident on this GPU";
         case DLM_ERR_CUDA: return "CUDA call failed (dlm_last_cuda_error)";
         case DLM_ERR_WORKSPACE: return "workspace too small (dlm_workspace_bytes)";
-        case DLM_ERR_TIMEOUT: return "device wait ran out: data from a rank never arrived";
+        case DLM_ERR_TIMEOUT: return "device wait ran out: data from a rank, or from memory, never arrived";
         case DLM_ERR_ARCH: return "not an sm_100 device";
-        case DLM_ERR_OVERLAP: return "the fused GEMM's input overlaps a buffer the same launch re-arms or writes (rearm, out)";
+        case DLM_ERR_OVERLAP: return "an output, or a buffer that the same launch re-arms, overlaps an input";
         case DLM_ERR_SCRATCH: return "requested K splits need more than the library's built-in scratch (DLM_NOALLOC_SCRATCH_BYTES)";
         case DLM_ERR_INDEX: return "a slot, position, page, length or adapter index lies outside its table";
         default: return "unknown error";
