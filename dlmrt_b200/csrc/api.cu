@@ -1007,7 +1007,7 @@ int dlm_adapters_bf16(const DlmAdapters* a, dlm_stream_t stream) {
     if (a->rank < 8 || a->rank % 8 || a->rank > 128 || a->count < 1) return DLM_ERR_SHAPE;
     if (!aligned16(a->x) || !aligned16(a->base) || !aligned16(a->out) || !aligned16(a->a) || !aligned16(a->b))
         return DLM_ERR_ALIGN;
-    if (a->ldx % 8 || a->ldb % 8 || a->ldo % 8 || a->ldx < 0 || a->ldb < 0 || a->ldo < a->n) return DLM_ERR_ALIGN;
+    if (a->m > 1 && (a->ldx % 8 || a->ldb % 8 || a->ldo % 8 || a->ldx < 0 || a->ldb < 0 || a->ldo < a->n)) return DLM_ERR_ALIGN;
     const Footprint out(a->out, &a->m, &a->ldo, 1, a->n);
     const bool in_place = a->base == a->out && (a->m == 1 || a->ldb == a->ldo);
     if (meet(out, Footprint(a->x, &a->m, &a->ldx, 1, a->k)) || (!in_place && meet(out, Footprint(a->base, &a->m, &a->ldb, 1, a->n))))

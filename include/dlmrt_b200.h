@@ -406,7 +406,7 @@ typedef struct DlmAdapters {
     const void* b;             /* [count, n, rank] BF16 contiguous */
     const float* scales;       /* [count] */
     int32_t* status;           /* [DLM_STATUS_WORDS] or NULL; an id past `count` is DLM_ERR_INDEX and counts as none */
-    int64_t ldx, ldb, ldo;     /* multiples of 8 */
+    int64_t ldx, ldb, ldo;     /* multiples of 8; of a single row they say nothing */
     int32_t m, n, k, rank;     /* 1 <= m <= 256; n, k, rank multiples of 8; rank <= 128 */
     int32_t count, pdl;
 } DlmAdapters;
