@@ -194,6 +194,15 @@ def launch(name, descriptor, device):
         return getattr(_lib, name)(descriptor, torch._C._cuda_getCurrentRawStream(index))
 
 
+def read_status(status, where):
+    """The DlmStatus of `status`, which is cleared, once what the current stream of its device holds is done. A default stream's
+    handle means that of the current device, so the device is made the current one."""
+    read = DlmStatus()
+    with torch.cuda.device(status.device):
+        check(lib().dlm_status_read(status.data_ptr(), C.byref(read), stream(status)), where)
+    return read
+
+
 def scratch(held, nbytes, device):
     """Adds zero-initialised scratch of at least `nbytes` to `held`, a list that belongs to one object and whose buffers
     are all too small. The older ones stay: graphs captured with them still write there. Sizes at least double, so the

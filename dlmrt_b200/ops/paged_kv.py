@@ -17,14 +17,13 @@ from torch's allocator. Indices (slots, positions, pages, lengths) live on the d
 outside its table touches no memory, and `PagedKV.check()` raises IndexError for the first of them.
 """
 
-import ctypes as C
 from contextlib import nullcontext
 from struct import Struct
 
 import torch
 
 from .. import _lib
-from .._lib import DlmAppend, DlmAttend, DlmPages, DlmStatus
+from .._lib import DlmAppend, DlmAttend, DlmPages
 
 # The pointers that every call brings, which lie side by side in the descriptors.
 _APPEND, _APPEND_AT = Struct("9Q"), DlmAppend.q.offset
@@ -50,8 +49,7 @@ def rotary_table(rotated, positions, theta=10000.0, device="cuda", inverse_frequ
 
 def _index_error(status, where, page_size=0):
     """Reads `status` (and clears it); IndexError where a kernel met an index outside its table."""
-    read = DlmStatus()
-    _lib.check(_lib.lib().dlm_status_read(status.data_ptr(), C.byref(read), _lib.stream(status)), where)
+    read = _lib.read_status(status, where)
     if read.code == _lib.ERR_INDEX:
         kind, value = _INDEX.get(read.slot, "index"), str(read.epoch)
         if kind == "slot":  # as a page and the place in it, which is how a slot is made up

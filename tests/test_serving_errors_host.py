@@ -23,3 +23,37 @@ def test_the_distance_of_a_single_row_to_the_next_is_nobodys_business():
     odd = dict(ldx=61, ldb=-3, ldo=1)
     assert call(m=1, **odd) != _lib.ERR_ALIGN
     assert all(call(m=2, **{name: value}) == _lib.ERR_ALIGN for name, value in odd.items())
+
+
+def test_the_status_of_another_device_is_read_on_that_device(monkeypatch):
+    """A default stream's handle is 0 on every device: what it means is the current device's."""
+    kv = PagedKV(torch.zeros(2, 1, 16, 64, dtype=BF16), torch.zeros(2, 1, 16, 64, dtype=BF16))
+    current, read = [0], []
+
+    class Current:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Status:
+        device = torch.device("cuda:1")
+        get_device = staticmethod(lambda: 1)
+        data_ptr = staticmethod(lambda: 0x1000)
+
+    class Library:
+        @staticmethod
+        def dlm_status_read(address, out, stream):
+            read.append((address, stream, current[0]))
+            return _lib.OK
+
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    monkeypatch.setattr(_lib, "lib", lambda: Library)
+    kv.status = Status()
+    kv.check()
+    assert read == [(0x1000, 0, 1)] and current == [0]
