@@ -126,11 +126,14 @@ class PagedKV:
         `k`, `v` [n, kv heads, head dim], `q` [n, query heads, head dim]: BF16 or FP16, any strides that are multiples of 8
         with a contiguous head dimension (slices of one qkv projection). `slots` [n] int64: page * page size + place in the
         page, each at most once in a call; negative: a padded row, which stores nothing. `positions` [n] int32: row of
-        `table` (see `rotary_table`, whose width says how many elements of a head are rotated; None: no rotation).
+        `table` (see `rotary_table`, whose width says how many elements of a head are rotated; None: no rotation, and positions are
+        not looked at).
         `interleaved`: pairs are neighbours, not a half apart. `q_norm`, `k_norm` [head dim]: weights of an RMSNorm over each
         head in front of the rotation. `q_out` may be `q`, but no other
         tensor that shares elements with `q`, `k` or `v`; by default a new contiguous tensor. `k` and `v` are not part of the
         cache."""
+        if table is not None and positions is None:
+            raise ValueError("a rotation by `table` needs positions")
         key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, slots.shape, slots.stride(),
                slots.dtype, slots.device, eps, interleaved,
                None if table is None else (table.shape, table.stride(), table.dtype, table.device, positions.shape,

@@ -57,3 +57,10 @@ def test_the_status_of_another_device_is_read_on_that_device(monkeypatch):
     kv.status = Status()
     kv.check()
     assert read == [(0x1000, 0, 1)] and current == [0]
+
+
+def test_a_rotation_needs_positions():
+    kv = PagedKV(torch.zeros(2, 1, 16, 64, dtype=BF16), torch.zeros(2, 1, 16, 64, dtype=BF16))
+    k, slots = torch.zeros(3, 1, 64, dtype=BF16), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="positions"):
+        kv.append(k, k, None, slots, torch.zeros(5, 64))
