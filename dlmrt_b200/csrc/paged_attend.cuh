@@ -176,6 +176,9 @@ struct alignas(16) Pipes {
 // Until when a role waits that begins an item now: a call of many items may take longer than a wait that nothing will end.
 __device__ __forceinline__ long long item_deadline() { return globaltimer() + kDefaultTimeoutNs; }
 
+// How long a block whose waits ran out waits for what it has on the way itself.
+constexpr long long kDrainNs = 1000000000ll;
+
 // A wait that runs out is reported; what follows is computed from whatever is there, and nothing more is requested.
 __device__ __forceinline__ void stalled(const AttendDev& p, int who, int at) {
     report(p.a.cache.status, kErrTimeout, who, kPhasePipeline, at);
@@ -313,6 +316,12 @@ __device__ __forceinline__ void produce(const AttendDev& p, uint8_t* ring, Pipes
             }
         }
         if (++stage == kStages) stage = 0, parity ^= 1;
+    }
+    if (failed) {
+        // Copies that are still on the way would otherwise land in memory that another block has by then. `stage` is the next one to
+        // be filled: those in front of it were filled in this lap, the others in the one before.
+        const long long limit = globaltimer() + kDrainNs;
+        for (int i = 0; i < kStages; ++i) mbar_wait(&pipes.full[i], i < stage ? parity ^ 1 : parity, limit);
     }
     Work none;
     none.head = -1;

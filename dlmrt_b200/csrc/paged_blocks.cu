@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
     // Queries written; of the step that a buffer of S is for: scores computed, weights written, values consumed; a side step of
     // a group. A wait can only tell a phase from the one before it, which here is kBuffers steps back.
     __shared__ uint64_t q_full, s_full[kBuffers], p_full[kBuffers], pv_done[kBuffers], aside[kGroups];
+    __shared__ uint64_t drained;  // what the issuer has on the way, where a wait of its ran out
     // FP8: what the producer's barriers are to the converters, these are to the issuer.
     __shared__ uint64_t wide_full[kSteps], wide_empty[kSteps], wide_present[kSteps];
     uint64_t* const step_full = kCodes ? wide_full : pipes.full;
@@ -217,6 +218,7 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
         mbar_init(&q_full, kGroups * kGroupThreads);
         for (int i = 0; i < kBuffers; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kGroupThreads), mbar_init(&pv_done[i], 1);
         for (int i = 0; i < kGroups; ++i) mbar_init(&aside[i], kGroupThreads);
+        mbar_init(&drained, 1);
         fence_barrier_init();
         tma_prefetch_descriptor(&p.tm_k);
         tma_prefetch_descriptor(&p.tm_v);
@@ -242,14 +244,19 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
         int stage = 0, slot = 0, next_stage = 0;
         uint32_t parity = 0, slot_parity = 0, q_parity = 0, step = 0;
         long long deadline = 0;
+        bool failed = false;
         auto wait = [&](uint64_t* bar, uint32_t bar_phase, int who, int at) {
-            if (!mbar_wait_warp(bar, bar_phase, deadline) && leader) stalled(p, who, at);
+            if (!mbar_wait_warp(bar, bar_phase, deadline)) {
+                failed = true;
+                if (leader) stalled(p, who, at);
+            }
             tcgen05_fence_after();
         };
         while (true) {
             deadline = item_deadline();
             const bool announced = mbar_wait_warp(&pipes.work_full[slot], slot_parity, deadline);
             if (!announced) {
+                failed = true;
                 if (leader) stalled(p, 5, slot);
                 break;
             }
@@ -296,6 +303,10 @@ __global__ void __launch_bounds__(BlockShape<D, kCodes>::kThreads, 1) blocks_ker
                 }
                 if (++stage == kSteps) stage = 0;
             }
+        }
+        if (failed) {  // products still read shared memory and write tensor memory, which the block is about to give back
+            if (leader) umma_commit(&drained);
+            mbar_wait_warp(&drained, 0, globaltimer() + kDrainNs);
         }
     } else if (kCodes && warp > Shape::kIssuerWarp) {
         // -- the converters: pieces of 16 codes ------------------------------------------------------------------------------
