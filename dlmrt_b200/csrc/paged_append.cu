@@ -8,8 +8,8 @@
 // head_dim / 8 lanes, 16 bytes each: the partner of a rotated element sits in another lane of the same group (one shuffle per
 // element) or, for neighbouring pairs, in the same lane, and a lane's cosines and sines are the same for all heads. Bound by
 // HBM for prompts: each lane has up to four heads' loads on the way at once, before the token's position and slot are known,
-// and registers are held to five blocks an SM (8189 tokens of 32 head rows of 256: 98 us with one row a lane, 65 with four at
-// three blocks an SM, 54 at five).
+// and registers are held to five blocks an SM, although 16-bit caches then spill 184 bytes a thread (8189 tokens of 32 head rows of
+// 256: 98 us with one row a lane, 65 with four at three blocks an SM, 53.5 at five). FP8 caches, at four, do not spill.
 #include <climits>
 
 #include "../../include/dlmrt_b200.h"
@@ -36,6 +36,16 @@ __device__ __forceinline__ void unpack8(const uint4& raw, float (&v)[8]) {
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
     return make_uint4(narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3]), narrow2<T>(v[4], v[5]), narrow2<T>(v[6], v[7]));
+}
+
+// Apart from the kernel, whose registers are few.
+__device__ __noinline__ void report_token(int* status, int token, bool bad_slot, long long slot, int page_shift, int pos) {
+    const long long page = slot >> page_shift;
+    if (bad_slot)
+        report_index(status, token, kIndexSlot, page > INT_MAX ? INT_MAX : static_cast<int>(page),
+                     static_cast<int>(slot & ((1ll << page_shift) - 1)));
+    else
+        report_index(status, token, kIndexPosition, pos);
 }
 
 }  // namespace
@@ -72,12 +82,7 @@ __global__ void __launch_bounds__(kAppendMostThreads, kCodes ? 4 : 5) append_ker
         const bool bad_slot = slot >= static_cast<long long>(p.cache.pages) << page_shift;
         const bool bad_pos = p.rotated && (pos < 0 || pos >= p.table_rows);
         if (bad_slot || bad_pos) {  // nothing of this token is written
-            if (threadIdx.x == 0 && bad_slot)
-                report_index(p.cache.status, static_cast<int>(token), kIndexSlot,
-                             static_cast<int>(min(slot >> page_shift, static_cast<long long>(INT_MAX))),
-                             static_cast<int>(slot & ((1ll << page_shift) - 1)));
-            else if (threadIdx.x == 0)
-                report_index(p.cache.status, static_cast<int>(token), kIndexPosition, pos);
+            if (threadIdx.x == 0) report_token(p.cache.status, static_cast<int>(token), bad_slot, slot, page_shift, pos);
             return;
         }
         // This lane's cosines and sines; partner: the lane that holds the other halves of its pairs.
