@@ -875,10 +875,10 @@ int dlm_paged_append(const DlmAppend* a, dlm_stream_t stream) {
 static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     // Blocks of tokens have a kernel of their own, from more rows on than one or two tiles of the other one hold. It reads the
     // cache once for 128 rows, and takes longer to begin and to end. 64 sequences of up to 6001 keys, 28 rows (two tiles), heads of
-    // 64 / 128 / 256: 31.8 / 36.2 / 81.8 us against 29.2 / 42.8 / 101.8; nine sequences: 14.2 / 19.1 / 27.0 against 13.5 / 15.0 /
-    // 23.8; 16 rows (one tile) 32.9 / 36.9 / 84.2 against 22.2 / 31.6 / 63.9. Codes it has to widen first: 32 sequences of up to 8224
-    // keys, 32 rows: 23.3 / 36.9 / 84.0 against 21.8 / 30.2 / 65.9; 48 rows: 23.2 / 37.5 / 84.3 against 26.4 / 39.7 / 88.3. Heads of 64
-    // with 40 rows: 81.2 against 96.7.
+    // 64 / 128 / 256: 33.3 / 39.0 / 91.5 us against 30.2 / 43.8 / 105; nine sequences: 14.5 / 19.5 / 29.1 against 13.3 / 15.5 / 24.5; 16
+    // rows (one tile) 33.1 / 36.7 / 88.9 against 22.3 / 31.9 / 64.4. Codes it has to widen first: 32 sequences of up to 8224 keys, 32
+    // rows: 24.8 / 38.2 / 86.2 against 23.1 / 31.7 / 71.1; 48 rows: 24.8 / 38.2 / 86.9 against 28.4 / 41.9 / 96.1. Heads of 64 with 40
+    // rows: 86 to 97 against 103 to 110.
     constexpr int kWholeKeys = 384, kBlocksAbove = kRowTile, kBlocksAboveTwo = 2 * kRowTile, kBlocksLead = 6, kAttendLead = 3, kDearLead = 6;
     int rc = check_pages(&a->cache, &d->page_shift);
     if (rc != DLM_OK) return rc;
@@ -908,9 +908,9 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->sms = sms;
     d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim, d->tile_rows);
     // What an item's beginning and end cost in units of 64 keys; more where a step is short (codes) or a tile's end long (16 rows).
-    // 64 ragged sequences of up to 8192 keys 88.0 / 87.7 / 87.1 / 88.8 us with 1 / 2 / 3 / 4; FP8 heads of 256 81.7 / 81.4 / 78.2 / 79.0
-    // with 2 / 4 / 6 / 8, 64 sequences of 16 rows 35.0 / 32.3 / 31.6 / 31.6; blocks of 32 tokens 74 / 60.2 / 59.2 / 59.0 / 60.6 with 0 /
-    // 5 / 6 / 8 / 11, of 28 rows 37.9 / 37.3 / 38.8 / 40.6 with 5 / 6 / 8 / 11.
+    // 64 ragged sequences of up to 8192 keys 87.5 / 88.4 / 88.4 us with 2 / 3 / 4 (boxes differ by as much); FP8 heads of 256 78.1 /
+    // 79.0 / 79.1 with 4 / 6 / 8, 64 sequences of 16 rows 33.3 / 32.6 / 32.4; blocks of 32 tokens 73.1 / 64.1 / 63.0 / 62.3 / 64.1 with
+    // 0 / 5 / 6 / 8 / 11, of 28 rows 52.3 / 39.4 / 38.9 / 39.7 / 41.4, of 32 tokens over FP8 97.9 / 84.3 / 83.0 / 84.9 / 87.9.
     d->lead = whole ? 0 : d->blocks ? kBlocksLead : a->cache.type == DLM_E4M3 || d->tile_rows > kFewRows ? kDearLead : kAttendLead;
     const long long units = whole ? 1 : d->lead + (span + kTileKeys - 1) / kTileKeys;  // of an item, at most
     if (units * a->batch * d->items > INT32_MAX) return DLM_ERR_SHAPE;

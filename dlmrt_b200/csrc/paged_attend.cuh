@@ -41,7 +41,8 @@ static_assert(kRescaleAbove + kHeadroom<__half> <= 15.f, "weights fit halves");
 //
 // What the second product costs: nothing where HBM bounds a call (64 ragged sequences 87.5 us with one part and with two, 131071
 // keys 48.2 / 48.4, FP8 heads of 256 77.8 / 78.6), more where 16 rows share FP8 keys (heads of 256 78.5 / 86.0, of 128 33.6 / 35.9) and
-// in blocks of tokens (16 of 32 tokens 58.7 / 64.1, half of it the product, half the parting; a prompt of 2048 tokens 108 / 123).
+// in blocks of tokens (16 of 32 tokens 58.7 / 63.0 us, call after call 64.9 / 73.1, most of it the product's tensor cycles; a prompt
+// of 2048 tokens 108 / 118).
 template <typename M, bool kCodes>
 __device__ __forceinline__ void split_weights(float x, float y, uint32_t* high, uint32_t* low) {
     if constexpr (!std::is_same<M, __half>::value) {

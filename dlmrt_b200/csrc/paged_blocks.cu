@@ -19,7 +19,7 @@
 // tensor pipe at 128) and 8192 exponentials (512 cycles). A group takes longer for a step than the step's 32 KB take from HBM, most
 // of it latency (1300 cycles against 1400 before weights had a low part): with one group nothing is left to catch up with what an
 // item's beginning and end cost. 16 sequences of 1056 to 8224 keys, blocks of 32 tokens, 8 key heads of 128 with four query heads
-// each: 64 us, 3.8 TB/s (start 4.5 us, 3.5 between items, join 3); the same over an FP8 cache 84 us, the converters' two warps being
+// each: 63 us, 3.8 TB/s (start 4.5 us, 3.5 between items, join 3); the same over an FP8 cache 84 us, the converters' two warps being
 // what takes longest.
 #include "paged_attend.cuh"
 

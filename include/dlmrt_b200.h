@@ -369,7 +369,8 @@ DLM_API int dlm_paged_append(const DlmAppend* append, dlm_stream_t stream);
  * table is read as far as the table goes. Grouped heads: query head i reads key head i / (q_heads / heads).
  * Keys past the end, pages that are not there and places that the mask hides never reach the result, whatever they hold.
  * Products of `type` with FP32 accumulation, softmax in FP32; FP8 entries are widened exactly to halves. Weights enter the product
- * with the values as two 16-bit parts each, 15 bits of a weight (halves 20). out may be q (the same strides); otherwise it shares
+ * with the values as two 16-bit parts each, 15 bits of a weight (halves 20). The largest weight of a row is between 1 and 2^8 (halves
+ * 2^7 and 2^15) until the row's sum divides it: BF16 values from 2^100 on may overflow in between. out may be q (the same strides); otherwise it shares
  * no bytes with q (DLM_ERR_OVERLAP). */
 typedef struct DlmAttend {
     DlmPages cache;
@@ -382,7 +383,7 @@ typedef struct DlmAttend {
     int64_t workspace_bytes;
     int64_t q_strides[3], out_strides[3];  /* sequence, token, head: elements, multiples of 8 */
     int64_t table_stride;
-    int32_t batch, tokens, q_heads, type;
+    int32_t batch, tokens, q_heads, type;  /* at most 65535, 65536 and 1024 */
     int32_t table_pages, window, causal;   /* window at most 2^30, and so are table_pages * page_size */
     float scale;
     int32_t pdl, reserved;

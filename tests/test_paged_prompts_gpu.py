@@ -81,3 +81,33 @@ def test_a_prompt_enters_the_cache(cache):
     for pool, x, w, t, scale in ((kv.keys, k, wk, table, kv.k_scale), (kv.values, v, None, None, kv.v_scale)):
         want, bound = su.stored(*su.turned(x, w, t, positions, 1e-6, False), cache, scale)
         su.assert_within(pool.cpu().double()[at // page, :, at % page], want[:-5], bound[:-5])
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("t, hq, hk", [(1, 8, 2), (6, 4, 2), (50, 2, 1)])
+@pytest.mark.parametrize("page", [8, 64, 128])
+def test_pages_in_front_of_the_window_may_be_gone(page, t, hq, hk, cache):
+    """A sliding window gives pages back: entries that no token's window reaches are not looked at, whatever they say."""
+    kv, q, table, lengths = setup([900, 300, 1 + t, 2000], t, hq, hk, 64, page, BF16, cache)
+    window = 200
+    want = kv.attend(q, table, lengths, window=window)
+    gone = table.clone()
+    for i, n in enumerate(lengths.tolist()):
+        first = max(0, n - t - window + 1) // page  # the page of the first token's oldest key
+        gone[i, :first] = torch.tensor([-1, 1 << 30, kv.keys.shape[0]], dtype=torch.int32, device="cuda").repeat(first)[:first]
+    assert torch.equal(kv.attend(q, gone, lengths, window=window), want)
+    kv.check()
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_sequences_share_the_pages_of_a_prefix(t):
+    kv, q, table, lengths = setup([640, 700, 655], t, 4, 2, 64, 16, BF16, BF16)
+    shared = table.clone()
+    shared[1:, :37] = table[0, :37]
+    check(kv, q, shared, lengths, causal=True)
+    lengths[2] = lengths[0]
+    shared[2] = shared[0]
+    q[2] = q[0]
+    got = kv.attend(q, shared, lengths, causal=True)
+    # cut into other runs: two roundings of sums whose weights (2^-15) and values (below 8) are the same
+    su.assert_within(got[2], got[0].cpu().double(), 2 * su.HALF[BF16] * got[0].cpu().double().abs() + 2.0 ** -12)
