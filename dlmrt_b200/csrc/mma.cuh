@@ -77,10 +77,10 @@ __device__ __forceinline__ uint32_t narrow2(float x, float y) {
     return out;
 }
 
-// Two halves rounded towards zero.
-__device__ __forceinline__ uint32_t narrow2_to_zero(float x, float y) {
+// Two halves rounded towards zero; zero for what is below.
+__device__ __forceinline__ uint32_t narrow2_down_to_zero(float x, float y) {
     uint32_t out;
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(out) : "f"(y), "f"(x));
+    asm("cvt.rz.relu.f16x2.f32 %0, %1, %2;" : "=r"(out) : "f"(y), "f"(x));
     return out;
 }
 

@@ -55,7 +55,7 @@ __device__ __forceinline__ void split_weights(float x, float y, uint32_t* high, 
             *high = narrow2<M>(x, y);
         } else {
             constexpr float kLess = 1.f - 0x1p-12f, kStep = -0x1p-24f;
-            *high = narrow2_to_zero(fmaxf(x * 0.5f, fmaf(x, kLess, kStep)), fmaxf(y * 0.5f, fmaf(y, kLess, kStep)));
+            *high = narrow2_down_to_zero(fmaf(x, kLess, kStep), fmaf(y, kLess, kStep));
         }
         const float2 h = widen2<M>(*high);
         *low = narrow2<M>(x - h.x, y - h.y);
