@@ -12,7 +12,8 @@
 // adapter, and cluster c takes the c-th leader's adapter and that row's next fellows, up to 16. No sort, no host round trip,
 // any order of ids. There are at most count + m / 16 leaders.
 //
-// 61 rows of 48 adapters, rank 16, k 2560, n 9728: 9.3 us (2.3 TB/s); 256 rows of 8 adapters, rank 64, k 9728, n 2560: 13.5 us.
+// 61 rows of 48 adapters, rank 16, k 2560, n 9728: 9.3 to 9.6 us (2.3 TB/s); 256 rows of 8 adapters, rank 64, k 9728, n 2560:
+// 13.4 to 14.2 us.
 #include <cooperative_groups.h>
 
 #include "mma.cuh"
