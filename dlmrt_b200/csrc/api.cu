@@ -795,26 +795,24 @@ static bool steps_reach(const Steps* dims, int n, int64_t offset, int64_t lo, in
     return false;
 }
 
-// Whether two tensors share bytes: exact where they step alike (slices of one projection, their heads side by side or in turn),
-// otherwise whether their ranges meet.
-static bool meet(const Footprint& a, const Footprint& b) {
+// Whether two tensors share bytes: exact where they step alike (slices of one projection, their heads side by side or in turn). A
+// dimension that they step along differently counts as filled without gaps in both.
+static bool meet(Footprint a, Footprint b) {
     Steps dims[3];
     int n = 0;
-    bool alike = true;
-    int64_t a_span = a.width, b_span = b.width;
     for (int i = 0; i < 3; ++i) {
-        a_span += (a.extent[i] - 1) * a.stride[i], b_span += (b.extent[i] - 1) * b.stride[i];
         if (a.extent[i] == 1 && b.extent[i] == 1) continue;
-        alike = alike && (a.extent[i] == 1 || b.extent[i] == 1 || a.stride[i] == b.stride[i]);
+        if (a.extent[i] > 1 && b.extent[i] > 1 && a.stride[i] != b.stride[i]) {
+            a.width += (a.extent[i] - 1) * a.stride[i], b.width += (b.extent[i] - 1) * b.stride[i];
+            continue;
+        }
         const Steps d{a.extent[i] > 1 ? a.stride[i] : b.stride[i], 1 - b.extent[i], a.extent[i] - 1};
         int at = n++;
         for (; at > 0 && dims[at - 1].stride < d.stride; --at) dims[at] = dims[at - 1];
         dims[at] = d;
     }
-    const int64_t ahead = static_cast<int64_t>(a.at - b.at);
-    if (ahead >= b_span || -ahead >= a_span) return false;
     int budget = 4096;
-    return !alike || steps_reach(dims, n, ahead, -a.width, b.width, &budget);
+    return steps_reach(dims, n, static_cast<int64_t>(a.at - b.at), -a.width, b.width, &budget);
 }
 
 // log2 of the page size in *shift.
@@ -908,7 +906,7 @@ static int plan_attend(const DlmAttend* a, int sms, AttendDev* d) {
     d->sms = sms;
     d->resident = d->blocks ? sms : sms * attend_ctas_per_sm(a->type, a->cache.type, a->cache.head_dim, d->tile_rows);
     // What an item's beginning and end cost in units of 64 keys; more where a step is short (codes) or a tile's end long (16 rows).
-    // 64 ragged sequences of up to 8192 keys 87.5 / 88.4 / 88.4 us with 2 / 3 / 4 (boxes differ by as much); FP8 heads of 256 78.1 /
+    // 64 ragged sequences of up to 8192 keys 87.5 / 88.4 / 88.4 us with 2 / 3 / 4 (GPUs differ by as much); FP8 heads of 256 78.1 /
     // 79.0 / 79.1 with 4 / 6 / 8, 64 sequences of 16 rows 33.3 / 32.6 / 32.4; blocks of 32 tokens 73.1 / 64.1 / 63.0 / 62.3 / 64.1 with
     // 0 / 5 / 6 / 8 / 11, of 28 rows 52.3 / 39.4 / 38.9 / 39.7 / 41.4, of 32 tokens over FP8 97.9 / 84.3 / 83.0 / 84.9 / 87.9.
     d->lead = whole ? 0 : d->blocks ? kBlocksLead : a->cache.type == DLM_E4M3 || d->tile_rows > kFewRows ? kDearLead : kAttendLead;

@@ -16,10 +16,10 @@
 // multiplied by exp2(m - m') only when some row's maximum is more than kRescaleAbove + kHeadroom past m.
 //
 // One CTA an SM; shared memory holds 2 to 8 steps of 64 keys. A step is 3 * 128 * 64 * head_dim multiply-adds (768 cycles of the
-// tensor pipe at 128) and 8192 exponentials (512 cycles). A group takes longer for a step than the step's 32 KB take from HBM, most
-// of it latency (1300 cycles against 1400 before weights had a low part): with one group nothing is left to catch up with what an
-// item's beginning and end cost. 16 sequences of 1056 to 8224 keys, blocks of 32 tokens, 8 key heads of 128 with four query heads
-// each: 63 us, 3.8 TB/s (start 4.5 us, 3.5 between items, join 3); the same over an FP8 cache 84 us, the converters' two warps being
+// tensor pipe at 128) and 8192 exponentials (512 cycles). A group took 1300 cycles for a step when weights had one part, most of it
+// latency, which is as long as a step's 32 KB take from HBM: with one group nothing would be left to catch up with what an item's
+// beginning and end cost. 16 sequences of 1056 to 8224 keys, blocks of 32 tokens, 8 key heads of 128 with four query heads
+// each: 63 us, 3.8 TB/s (start 4.5 us, 3.5 between items, join 3); the same over an FP8 cache 83 us, the converters' two warps being
 // what takes longest.
 #include "paged_attend.cuh"
 

@@ -313,7 +313,7 @@ DLM_API int dlm_all_gather_loopback(const void* const* x, int64_t bytes, const D
 enum { DLM_BF16 = 0, DLM_F16 = 1, DLM_E4M3 = 2 };
 
 /* Results that may lie beside inputs in one buffer (DLM_ERR_OVERLAP): tensors that step by the same strides are told apart
- * element by element, others count as sharing bytes where their ranges meet. */
+ * element by element; a dimension with other strides counts as filled without gaps. */
 #define DLM_MIN_PAGE 8
 #define DLM_MAX_PAGE 4096
 
@@ -370,8 +370,8 @@ DLM_API int dlm_paged_append(const DlmAppend* append, dlm_stream_t stream);
  * Keys past the end, pages that are not there and places that the mask hides never reach the result, whatever they hold.
  * Products of `type` with FP32 accumulation, softmax in FP32; FP8 entries are widened exactly to halves. Weights enter the product
  * with the values as two 16-bit parts each, 15 bits of a weight (halves 20). The largest weight of a row is between 1 and 2^8 (halves
- * 2^7 and 2^15) until the row's sum divides it: BF16 values from 2^100 on may overflow in between. out may be q (the same strides); otherwise it shares
- * no bytes with q (DLM_ERR_OVERLAP). */
+ * 2^7 and 2^15) until the row's sum divides it: BF16 values from 2^100 on may overflow in between. out may be q (the same strides);
+ * otherwise it shares no bytes with q (DLM_ERR_OVERLAP). */
 typedef struct DlmAttend {
     DlmPages cache;
     const void* q;             /* [batch, tokens, q_heads, head_dim] `type` */

@@ -37,6 +37,18 @@ def test_a_projection_with_its_heads_in_turn_takes_rotated_queries_in_place():
         assert refused(_lib.lib().dlm_paged_append(call, None))
 
 
+def test_rows_side_by_side_may_space_their_heads_otherwise():
+    """Halves of the same longer rows: 4 heads of queries 64 apart, results 128 apart behind them; and keys 72 apart in front."""
+    d, row = 64, 4 * 64 + 4 * 128 + 2 * 72
+    call = append(n=3, q=BASE, q_out=BASE + 2 * 4 * d, q_heads=4, k=BASE + 2 * (4 * 64 + 4 * 128), v=BASE + (1 << 18), q_strides=(row, 64),
+                  out_strides=(row, 128), k_strides=(row, 72))
+    assert not refused(_lib.lib().dlm_paged_append(call, None))
+    call.q_out = BASE + 2 * 4 * d - 16
+    assert refused(_lib.lib().dlm_paged_append(call, None))
+    two = attend(cache=pages(heads=4), q=BASE, out=BASE + 2 * 4 * d, q_heads=4, batch=3, q_strides=(row, row, 64), out_strides=(row, row, 128))
+    assert not refused(_lib.lib().dlm_paged_attend(two, None))
+
+
 @pytest.mark.parametrize("seed", range(10))
 def test_append_refuses_what_shares_elements(seed):
     rng = random.Random(seed)
